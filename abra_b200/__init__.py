@@ -44,6 +44,14 @@ from .q4k import (
     rmsnorm_quantize_q8_1,
     slice_start,
 )
+from .paged import (
+    PagedKV,
+    paged_append,
+    paged_attention,
+    paged_attention_workspace,
+    paged_evict,
+    paged_evict_workspace,
+)
 from .q6k import (
     Q6K_BYTES,
     Q6KCandidateSpec,

@@ -94,6 +94,14 @@ SIGNATURES: dict[str, tuple] = {
     "abra_tp_tensor_slice": (C.c_int, [_vp, _i32, _i32, _i32, _i32, _vp]),
     "abra_model_path": (C.c_int, [_vp, C.POINTER(C.c_int32)]),
     "abra_persist_plan": (C.c_int, [_vp, _i32, _vp]),
+    # paged cache
+    "abra_paged_append": (C.c_int, [_vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _i32, _fp, _fp,
+                                    _f32, _fp, _i32, _vp, _i64, _vp]),
+    "abra_paged_attention_workspace": (C.c_int64, [_vp, _i32, _i32, _i32]),
+    "abra_paged_attention": (C.c_int, [_vp, _vp, _i64, _i32, _i32, _f32, _vp, _i32, _i64, _fp, _i32, _vp,
+                                       _i64, _vp]),
+    "abra_paged_evict_workspace": (C.c_int64, [_vp, _i32]),
+    "abra_paged_evict": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _i64, _vp]),
 }
 
 

@@ -406,10 +406,12 @@ int abra_model_info(void *model, void **stream, uint64_t *weight_bytes, uint64_t
 #define ABRA_TENSOR_ATTN_V 10
 #define ABRA_TENSOR_TOKEN_EMBD 1  /* layer -1 */
 #define ABRA_TENSOR_OUTPUT_NORM 2 /* layer -1 */
-/* ggml tensor types a slot can hold */
+/* ggml tensor types a slot can hold (F16 and BF16: a paged cache) */
 #define ABRA_GGML_F32 0
+#define ABRA_GGML_F16 1   /* paged caches and their queries */
 #define ABRA_GGML_Q4_K 12
 #define ABRA_GGML_Q6_K 14
+#define ABRA_GGML_BF16 30 /* paged caches and their queries */
 /* Copy one tensor's data, as stored in a GGUF file (ggml layout: N rows of
  * K/256 blocks for a [K, N] weight; fp32 vectors for norms), from host
  * memory into the model, overwriting the seeded weights.  ggml_type and
@@ -484,6 +486,91 @@ int abra_model_tp_connect(void *model, const void *handles, int32_t size_each);
  * with abra_model_tp_handle / abra_model_tp_connect as above. */
 int abra_model_create_batched_tp(const abra_model_config *cfg, int32_t batch, int32_t rank,
                                  int32_t world, void **model);
+
+/* ---------------------------------------------------- paged cache ------ */
+/* A serving program's key-value cache of one layer, kept in pages: sequence s
+ * holds lens[s] slots, slot t of it lies in page table[s * table_stride + t /
+ * page_size] at offset t % page_size, for every kv head.  The pools hold the
+ * caller's memory in any order of pages, heads and offsets: element i of
+ * (page, head, offset) is at page * page_stride + head * head_stride + offset
+ * * slot_stride + i (elements; rows of head_dim are contiguous).  The
+ * reference leaves the cache to llama.cpp and has one contiguous cache per
+ * layer (kernels/q4k/abra-attention.cuh:3-127); the decode model here keeps
+ * that form, these calls are for callers with many sequences.
+ *
+ * lens counts a step's new tokens already: append writes the last slots of
+ * each sequence, attention reads them all.  A page has one owner wherever a
+ * call writes to it.  Lengths beyond max_pages * page_size (or below 0) and
+ * page numbers outside the pool set bit 4 of the device error word: the length
+ * is clamped, a write is skipped, a read takes page 0.
+ * Table entries past a sequence's last page are not read. */
+typedef struct {
+    void *k, *v;             /* the pools, 16-byte aligned */
+    float *acc;              /* accumulated weights [n_pages][n_kv_heads][page_size], or NULL */
+    int32_t *pos;            /* positions of the slots, same layout, or NULL */
+    const int32_t *table;    /* pages, [n_seqs] rows of table_stride, max_pages used */
+    const int32_t *lens;     /* slots of each sequence */
+    const int32_t *next_pos; /* position after each sequence's newest token; NULL: lens */
+    int64_t k_page_stride, k_head_stride, k_slot_stride; /* elements, multiples of 8 */
+    int64_t v_page_stride, v_head_stride, v_slot_stride;
+    int64_t table_stride;
+    int32_t type;     /* of the pools: ABRA_GGML_F16 or ABRA_GGML_BF16 */
+    int32_t n_pages, n_kv_heads, head_dim, page_size, n_seqs, max_pages;
+} abra_paged_kv;
+
+/* New tokens into the cache.  Token t of n_tokens has n_heads query heads at
+ * q + t * ldq, n_kv_heads key heads at k + t * ldk and value heads at v + t *
+ * ldv (elements of in_type F32, F16 or BF16; one fused q|k|v row will do).
+ * Tokens lie sequence after sequence: cu_new[s] is sequence s's first token
+ * and cu_new[n_seqs] = n_tokens; NULL gives every sequence n_tokens / n_seqs.
+ * A sequence's m tokens go to slots lens - m .. lens - 1 at positions next_pos
+ * - m .. next_pos - 1.  Queries and keys get their RMSNorm over the head (x /
+ * sqrt(mean(x^2) + eps) times the head_dim weights; NULL: none) and then the
+ * rotation of the pairs (i, i + head_dim/2) by the row of its position in rope
+ * [rope_len][head_dim/2][cos, sin] (NULL: none), in fp32, rounded once to the
+ * pools' type.  q_out (row stride ldqo) takes the queries in the pools' type;
+ * q and q_out may both be NULL.  acc (if not NULL) becomes 0 and pos (if not
+ * NULL) the position at the new slots.  The paged form of the decode model's
+ * norm-rope-append step.  head_dim 64, 96 or 128. */
+int abra_paged_append(const abra_paged_kv *kv, const void *q, const void *k, const void *v,
+                      int32_t in_type, int64_t ldq, int64_t ldk, int64_t ldv, int32_t n_heads,
+                      const int32_t *cu_new, int32_t n_tokens, const float *q_norm,
+                      const float *k_norm, float eps, const float *rope, int32_t rope_len,
+                      void *q_out, int64_t ldqo, void *stream);
+
+/* Attention of each sequence's newest n_q tokens over its cache: query j (0 ..
+ * n_q - 1) of sequence s sees slots 0 .. lens[s] - n_q + j, q head h reads kv
+ * head h / (n_heads / n_kv_heads), out = sum_t softmax_t(scale q.k_t) v_t.
+ * q (the pools' type) and out (out_type: the pools' type or F32) have row (s *
+ * n_q + j) at stride ldq / ldo; lse (or NULL), fp32 [n_seqs][n_q][n_heads],
+ * takes log sum_t exp(scale q.k_t).  A query that sees no slot gives zeros and
+ * -infinity.  With ABRA_PAGED_ACCUMULATE every slot's softmax weight, summed
+ * over the n_q queries and the group's heads, is added to acc.
+ * workspace (256-byte aligned, abra_paged_attention_workspace bytes) must be
+ * zero before its first use; each call leaves it ready for the next one of the
+ * same arguments.  Calls that can overlap need a workspace each.
+ * head_dim 64, 96 or 128. */
+#define ABRA_PAGED_ACCUMULATE 1
+int64_t abra_paged_attention_workspace(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q,
+                                       int32_t flags); /* bytes, or ABRA_E_* */
+int abra_paged_attention(const abra_paged_kv *kv, const void *q, int64_t ldq, int32_t n_heads,
+                         int32_t n_q, float scale, void *out, int32_t out_type, int64_t ldo,
+                         float *lse, int32_t flags, void *workspace, int64_t workspace_bytes,
+                         void *stream);
+
+/* Cuts every sequence with more than `budget` slots down to `budget`, for each
+ * kv head by itself: kept are the slots with pos < n_sink, those with pos >=
+ * next_pos - n_recent, and of the others the ones with the largest acc (ties
+ * to the lowest slot; NaN counts as -infinity) until budget are.  Kept slots
+ * below the budget stay; the i-th evicted slot below the budget takes the rows,
+ * acc and pos of the i-th kept slot above it.  What lies from slot `budget` on
+ * is then free.  new_lens[s] = min(lens[s], budget); lens itself is left as it
+ * is (another layer may still need it), so new_lens must be other memory.
+ * Needs acc and pos, n_sink + n_recent <= budget, and workspace (16-byte
+ * aligned, abra_paged_evict_workspace bytes, any contents). */
+int64_t abra_paged_evict_workspace(const abra_paged_kv *kv, int32_t budget);
+int abra_paged_evict(const abra_paged_kv *kv, int32_t budget, int32_t n_sink, int32_t n_recent,
+                     int32_t *new_lens, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
