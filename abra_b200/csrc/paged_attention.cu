@@ -15,13 +15,11 @@
 // Layout: both products run on the tensor cores with the slots (16 a warp) as
 // the tall side and the rows (8 a tile) as the narrow one, S^T = K Q^T and O^T
 // = V^T P^T, so that a group of four heads wastes half a tile and not three
-// quarters.  No shared memory: the order of the contracted index is free as
-// long as both operands agree, so lane (g, c) = (lane / 4, lane % 4) reads 16
-// contiguous bytes of K rows g and g + 8 (elements 32 i + 8 c ..) and takes
-// them as the A fragments of two k-steps, with Q read the same way; of V it
-// reads rows 2c, 2c+1, 2c+8, 2c+9 (elements 64 j + 8 g ..) and pairs slots
-// with byte permutes.  Each lane's next K tile is in flight while this tile's
-// softmax runs, and its next V tile during the next scores.
+// quarters.  Each warp has a ring of tiles of its own in shared memory, filled
+// by asynchronous 16-byte copies (zeros past the end) that run ahead across the
+// ends of the rows; no warp waits for another before a row ends.  Rows in the
+// ring are padded by 16 bytes, so the eight rows of an ldmatrix lie in distinct
+// banks.
 #include "paged_kv.cuh"
 
 namespace abra {
@@ -34,7 +32,6 @@ constexpr int SCAN = AT_THREADS;          // sequences of one block scan
 // A row's maximum is raised only when a score passes it by 2^RAISE: weights
 // stay below 2^RAISE (well inside fp16), and most tiles need no reduction.
 constexpr float RAISE = 10.0f;
-constexpr int MAX_CTAS = 4;  // a multiprocessor
 
 struct AttendArgs {
     PagedKv kv;
@@ -53,13 +50,12 @@ struct AttendArgs {
 };
 
 // ------------------------------------------------------------------ PTX ---
-__device__ __forceinline__ uint4 ld_stream(const void *p) {
-    uint4 x;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                 : "l"(p));
-    return x;
+// 16 bytes into shared memory past L1; `bytes` 0 writes zeros and reads nothing.
+__device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 template <typename T>
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                             uint32_t b0, uint32_t b1);
@@ -80,6 +76,19 @@ __device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d)[4], uint32
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four 8x8 matrices of 16-bit values, lane l naming row l % 8 of matrix l / 8.
+__device__ __forceinline__ void ldm(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void ldm_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
 }
 // Transpose of an 8x8 matrix of 16-bit values spread over the warp.
 __device__ __forceinline__ uint32_t trans8x8(uint32_t a) {
@@ -117,36 +126,72 @@ template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t x
 }
 
 // ------------------------------------------------------------ the line ---
-// Where CTA `cta` of `ctas` starts on the line of steps.
-struct Line {
-    int64_t total;  // steps of all triples
-    int ctas;       // pieces; each has at least one step
-    __device__ __forceinline__ int64_t begin(int cta) const { return cta * total / ctas; }
-    // the piece that holds step x
-    __device__ __forceinline__ int piece(int64_t x) const { return static_cast<int>(((x + 1) * ctas - 1) / total); }
-};
 __device__ __forceinline__ int steps_of(int len) { return (len + STEP - 1) / STEP; }
 
-struct Start {
-    int seq;        // the sequence of the piece's first step
-    int64_t steps;  // steps of the sequences before it (for one unit)
+struct Line {
+    int total;  // steps of all triples
+    int ctas;   // pieces; each has at least one step
+    __device__ __forceinline__ int begin(int cta) const {
+        return static_cast<int>(static_cast<int64_t>(cta) * total / ctas);
+    }
+    // the piece that holds step x
+    __device__ __forceinline__ int piece(int x) const {
+        return static_cast<int>((static_cast<int64_t>(x + 1) * ctas - 1) / total);
+    }
 };
 
-// Sums the sequences' steps and finds the one that this CTA's piece begins in.
-// `units` triples share a sequence's length.  All threads of the block.
-__device__ __forceinline__ Line find_start(const PagedKv &kv, int units, Start &at) {
-    __shared__ unsigned s_warp[AT_WARPS];
-    __shared__ int s_seq;
-    __shared__ int64_t s_steps;
+// A segment: the steps [tile0, tile1) of one triple that lie in a piece.
+struct Segment {
+    int seq, len, n;          // the sequence, its slots and steps
+    int unit, row_begin;      // the triple of this sequence and its first step on the line
+    int head, block;          // its kv head and block of rows
+    int tile0, tile1, slot_end;
+};
+
+// Walks the segments of the piece [pos, end).  `units` triples share a
+// sequence's length, `blocks` of them a kv head.
+struct Walk {
+    int pos, end, seq_begin, units, blocks;
+    Segment s;
+    __device__ __forceinline__ void enter(const PagedKv &kv) {
+        s.len = paged_len(kv, s.seq);
+        s.n = steps_of(s.len);
+        while (pos >= seq_begin + s.n * units) {  // the next sequence with slots
+            seq_begin += s.n * units;
+            s.len = paged_len(kv, ++s.seq);
+            s.n = steps_of(s.len);
+        }
+        s.unit = (pos - seq_begin) / s.n;
+        s.head = s.unit / blocks;
+        s.block = s.unit - s.head * blocks;
+        s.row_begin = seq_begin + s.unit * s.n;
+        s.tile0 = pos - s.row_begin;
+        s.tile1 = min(s.n, end - s.row_begin);
+        s.slot_end = min(s.len, s.tile1 * STEP);
+    }
+    // the next segment, if there is one
+    __device__ __forceinline__ bool next(const PagedKv &kv) {
+        pos = s.row_begin + s.tile1;
+        if (pos >= end) return false;
+        enter(kv);
+        return true;
+    }
+};
+
+// Sums the sequences' steps and finds the one that this CTA's piece begins in
+// (w.end == w.pos: this CTA has no piece).  All threads of the block.
+__device__ __forceinline__ Line find_start(const PagedKv &kv, int blocks, Walk &w) {
+    __shared__ int s_warp[AT_WARPS], s_seq, s_steps;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = kv.a.n_seqs;
+    const int units = kv.a.n_kv_heads * blocks;
     // inclusive scan of the steps of sequences base .. base + SCAN - 1
-    unsigned own = 0, incl = 0, all = 0;
+    int own = 0, incl = 0, all = 0;
     auto scan = [&](int base) {
-        own = base + tid < n ? static_cast<unsigned>(steps_of(paged_len(kv, base + tid))) : 0u;
+        own = base + tid < n ? steps_of(paged_len(kv, base + tid)) : 0;
         incl = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const unsigned y = __shfl_up_sync(0xffffffffu, incl, d);
+            const int y = __shfl_up_sync(0xffffffffu, incl, d);
             if (lane >= d) incl += y;
         }
         __syncthreads();
@@ -154,47 +199,59 @@ __device__ __forceinline__ Line find_start(const PagedKv &kv, int units, Start &
         __syncthreads();
         all = 0;
 #pragma unroll
-        for (int w = 0; w < AT_WARPS; ++w) {
-            if (w < warp) incl += s_warp[w];
-            all += s_warp[w];
+        for (int x = 0; x < AT_WARPS; ++x) {
+            if (x < warp) incl += s_warp[x];
+            all += s_warp[x];
         }
     };
-    int64_t sum = 0;
-    int base = 0;
-    for (; base < n; base += SCAN) {
+    int sum = 0;
+    for (int base = 0; base < n; base += SCAN) {
         scan(base);
         sum += all;
     }
     Line line{sum * units, 0};
-    line.ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), line.total));
+    line.ctas = min(static_cast<int>(gridDim.x), line.total);
+    w.units = units;
+    w.blocks = blocks;
+    w.pos = w.end = 0;
     if (static_cast<int>(blockIdx.x) >= line.ctas) return line;
-    const int64_t x = line.begin(blockIdx.x) / units;
-    int64_t before = 0;
+    w.pos = line.begin(blockIdx.x);
+    w.end = line.begin(blockIdx.x + 1);
+    const int x = w.pos / units;
+    int before = 0;
     if (n <= SCAN) {
         if (incl > x && incl - own <= x) s_seq = tid, s_steps = incl - own;
     } else {
-        for (base = 0; base < n; base += SCAN) {
+        for (int base = 0; before <= x; base += SCAN) {
             scan(base);
             if (before + incl > x && before + incl - own <= x) s_seq = base + tid, s_steps = before + incl - own;
             before += all;
-            if (before > x) break;
         }
     }
     __syncthreads();
-    at = {s_seq, s_steps};
+    w.s.seq = s_seq;
+    w.seq_begin = s_steps * units;
+    w.enter(kv);
     return line;
 }
 
 // --------------------------------------------------------------- kernel ---
 template <int D, int NT> struct Shape {
-    static constexpr int NK = D / 32;           // 16-byte pieces of a K row a lane reads
-    static constexpr int NV = (D + 63) / 64;    // 16-byte pieces of a V row a lane reads
-    static constexpr int MT = NV * 4;           // 16-element tiles of the output
+    static constexpr int KS = D / 16;           // k-steps of the scores, and 16-element tiles of the output
     static constexpr int R = 8 * NT;            // rows of a block
+    static constexpr int ROW = 2 * D + 16;      // bytes of a row in the ring
+    static constexpr int CHUNKS = D / 8;        // 16-byte chunks of a row
+    static constexpr int COPIES = CHUNKS / 2;   // of a lane for a tile of 16 rows
+    static constexpr int TILE_BYTES = TILE * ROW;            // K or V of one tile
+    static constexpr int STAGE = AT_WARPS * 2 * TILE_BYTES;  // the CTA's K and V tiles
     static constexpr int PITCH = D + 4;         // floats of a row in the join buffer
-    static constexpr int MIN_CTAS = NT == 1 ? 3 : 2;
-    static constexpr int Q_BYTES = NT == 1 ? 0 : NT * NK * 32 * 16;
-    static constexpr int SMEM = Q_BYTES + AT_WARPS * R * (PITCH + 2) * 4;
+    static constexpr int Q_BYTES = NT == 1 ? 0 : NT * KS * 32 * 8;
+    static constexpr int JOIN_BYTES = R * PITCH * 4 + 2 * AT_WARPS * R * 4;
+    static constexpr int CTAS = NT == 1 ? 3 : 2;  // on a multiprocessor
+    // the ring: as many tiles as leave room for them (1 KB each is the system's)
+    static constexpr int DEPTH = (233472 / CTAS - 1024 - 128 - Q_BYTES - JOIN_BYTES) / STAGE;
+    static constexpr int SMEM = DEPTH * STAGE + Q_BYTES + JOIN_BYTES;
+    static_assert(DEPTH >= 2, "the ring needs two tiles");
 };
 
 template <typename T>
@@ -206,8 +263,8 @@ __device__ __forceinline__ void store_out(const AttendArgs &p, int64_t at, float
     }
 }
 
-// A finished row: out at elements d .. d + 3 (lanes of one warp share the
-// row), its lse by the lane of element 0.  total == 0: the row saw nothing.
+// A finished row: out at elements d .. d + 3, its lse by the lane of element 0.
+// total == 0: the row saw nothing.
 template <typename T>
 __device__ __forceinline__ void finish_row(const AttendArgs &p, int seq, int head, int r, int d, int D, float4 o, float m,
                                            float total) {
@@ -223,21 +280,20 @@ __device__ __forceinline__ void finish_row(const AttendArgs &p, int seq, int hea
             p.row_lse[(static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.rows + r] = total != 0.0f ? l2 : INFINITY;
     }
 }
+__device__ __forceinline__ float scaled(float m, float top) { return m == top ? 1.0f : exp2_fast(m - top); }
 
 template <typename T, int D, int NT, bool SCORES>
-__global__ void __launch_bounds__(AT_THREADS, Shape<D, NT>::MIN_CTAS) attend_kernel(const __grid_constant__ AttendArgs p) {
+__global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kernel(const __grid_constant__ AttendArgs p) {
     using S = Shape<D, NT>;
-    extern __shared__ __align__(16) unsigned char smem[];
-    uint4 *s_q = reinterpret_cast<uint4 *>(smem);  // [NT][NK][32 lanes] Q fragments (NT > 1)
-    float *s_o = reinterpret_cast<float *>(smem + S::Q_BYTES);  // [warp][R][PITCH]
-    float *s_m = s_o + AT_WARPS * S::R * S::PITCH, *s_l = s_m + AT_WARPS * S::R;
+    extern __shared__ __align__(16) unsigned char smem[];  // the ring: [warp][stage][K, V][row]
+    uint2 *s_q = reinterpret_cast<uint2 *>(smem + S::DEPTH * S::STAGE);  // [NT][KS][lane] Q fragments (NT > 1)
+    float *s_o = reinterpret_cast<float *>(smem + S::DEPTH * S::STAGE + S::Q_BYTES);  // [R][PITCH]
+    float *s_m = s_o + S::R * S::PITCH, *s_l = s_m + AT_WARPS * S::R;  // [warp][R]
     __shared__ bool s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
-    const int units = p.kv.a.n_kv_heads * p.row_blocks;
-    const T *kp = static_cast<const T *>(p.kv.a.k), *vp = static_cast<const T *>(p.kv.a.v);
 
-    Start at;
-    const Line line = find_start(p.kv, units, at);
+    Walk w;
+    const Line line = find_start(p.kv, p.row_blocks, w);
     // rows of empty sequences are nobody's: zeros and -infinity
     for (int s = blockIdx.x; s < p.kv.a.n_seqs; s += gridDim.x) {
         if (paged_len(p.kv, s) > 0) continue;
@@ -246,237 +302,276 @@ __global__ void __launch_bounds__(AT_THREADS, Shape<D, NT>::MIN_CTAS) attend_ker
             finish_row<T>(p, s, head, row - head * p.rows, (i - row * (D / 4)) * 4, D, make_float4(0, 0, 0, 0), 0.0f, 0.0f);
         }
     }
-    if (static_cast<int>(blockIdx.x) >= line.ctas) return;
+    if (w.pos >= w.end) return;
+    const int begin = w.pos;
 
-    int64_t pos = line.begin(blockIdx.x);
-    const int64_t begin = pos, end = line.begin(blockIdx.x + 1);
-    int seq = at.seq;
-    int64_t seq_begin = at.steps * units;
-    int len = paged_len(p.kv, seq);
-    while (pos < end) {
-        // the segment: steps [tile0, tile1) of row block u of this sequence
-        const int n = steps_of(len);
-        const int u = static_cast<int>((pos - seq_begin) / n);
-        const int64_t row_begin = seq_begin + static_cast<int64_t>(u) * n;
-        const int tile0 = static_cast<int>(pos - row_begin), tile1 = static_cast<int>(min(static_cast<int64_t>(n), end - row_begin));
-        const int head = u / p.row_blocks, r0 = (u - head * p.row_blocks) * S::R;
-        const int slot_end = min(len, tile1 * STEP);
+    // ---- the fetching side: this warp's tiles, segment after segment ----
+    // Copy i of a lane moves 16-byte chunk (32 i + lane) % CHUNKS of row (32 i +
+    // lane) / CHUNKS; the first half of the copies are rows 0-7, the second
+    // rows 8-15.  Where eight divides the page size each half lies in one page.
+    const uint32_t ring = smem_u32(smem) + warp * (S::DEPTH * 2 * S::TILE_BYTES);
+    const bool by8 = p.kv.a.page_size % 8 == 0;
+    Walk f = w;
+    int f_base = f.s.tile0 * STEP + warp * TILE, f_valid = 0;
+    int f_page0 = 0, f_page1 = 0;  // of the halves, or (by8 false) f_page0 of row lane % 16
+    uint32_t f_at = ring;
+    bool f_more = true;
+    int64_t f_v0 = 0, f_v1 = 0;  // V offsets of the halves' first rows, or f_v0 of row lane % 16
+    auto page_of = [&](int t) {
+        return t < f.s.slot_end
+                   ? __ldg(p.kv.a.table + static_cast<int64_t>(f.s.seq) * p.kv.a.table_stride + p.kv.page.div(t))
+                   : 0;
+    };
+    auto fetch_settle = [&]() {  // on to the next tile that exists, and its pages
+        while (f_base >= f.s.slot_end) {
+            f_more = f.next(p.kv);
+            if (!f_more) return;
+            f_base = f.s.tile0 * STEP + warp * TILE;
+        }
+        if (by8) {
+            f_page0 = page_of(f_base);
+            f_page1 = page_of(f_base + 8);
+        } else {
+            f_page0 = page_of(f_base + (lane & 15));
+        }
+    };
+    auto in_pool = [&](int &page) {
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.kv.a.n_pages)) {
+            report_error(ERR_BAD_INDEX);
+            page = 0;
+        }
+    };
+    auto copy_tile = [&](const T *pool, int64_t off0, int64_t off1, int64_t stride, uint32_t to) {
+        const T *src0 = pool + off0, *src1 = pool + off1;
+#pragma unroll
+        for (int i = 0; i < S::COPIES; ++i) {
+            const int x = 32 * i + lane, row = x / S::CHUNKS, chunk = x - row * S::CHUNKS;
+            const T *src;
+            if (by8)
+                src = (2 * i < S::COPIES ? src0 : src1) + (row & 7) * stride;
+            else
+                src = pool + __shfl_sync(0xffffffffu, off0, row);
+            copy_async(to + row * S::ROW + chunk * 16, src + chunk * 8, row < f_valid ? 16 : 0);
+        }
+    };
+    auto fetch_k = [&]() {
+        f_valid = 0;
+        if (f_more) {
+            f_valid = f.s.slot_end - f_base;
+            const int t0 = by8 ? f_base : f_base + (lane & 15), off0 = t0 - p.kv.page.div(t0) * p.kv.a.page_size;
+            in_pool(f_page0);
+            const int64_t k0 = paged_k_at(p.kv, f_page0, f.s.head, off0);
+            f_v0 = paged_v_at(p.kv, f_page0, f.s.head, off0);
+            int64_t k1 = 0;
+            if (by8) {
+                const int off1 = f_base + 8 - p.kv.page.div(f_base + 8) * p.kv.a.page_size;
+                in_pool(f_page1);
+                k1 = paged_k_at(p.kv, f_page1, f.s.head, off1);
+                f_v1 = paged_v_at(p.kv, f_page1, f.s.head, off1);
+            }
+            copy_tile(static_cast<const T *>(p.kv.a.k), k0, k1, p.kv.a.k_slot_stride, f_at);
+        }
+        copy_commit();
+    };
+    auto fetch_v = [&]() {
+        if (f_valid > 0) {
+            copy_tile(static_cast<const T *>(p.kv.a.v), f_v0, f_v1, p.kv.a.v_slot_stride, f_at + S::TILE_BYTES);
+            f_base += STEP;
+            fetch_settle();
+        }
+        copy_commit();
+        f_at += 2 * S::TILE_BYTES;
+        if (f_at == ring + S::DEPTH * 2 * S::TILE_BYTES) f_at = ring;
+    };
+    fetch_settle();
+#pragma unroll 1
+    for (int i = 0; i < S::DEPTH; ++i) {
+        fetch_k();
+        fetch_v();
+    }
+    // this lane's row of an ldmatrix: K's matrices are (slots 0-7, 8-15) x
+    // (elements 0-7, 8-15) in the order of an A fragment; V's are transposed, so
+    // slots and elements change places
+    const uint32_t k_lane = (lane & 15) * S::ROW + (lane >> 4) * 16;
+    const uint32_t v_lane = S::TILE_BYTES + ((lane & 7) + (lane >> 4) * 8) * S::ROW + ((lane >> 3) & 1) * 16;
+    uint32_t at = ring;
 
-        // Q fragments: row r0 + 8 nt + g, elements 32 i + 8 c ..; rows past the end are zeros
-        uint4 qf[NT == 1 ? S::NK : 1];
-        auto load_q = [&](int nt, int i) {
+    do {
+        const Segment &sg = w.s;
+        const int head = sg.head, r0 = sg.block * S::R;
+
+        // Q fragments: row r0 + 8 nt + g, elements 16 ks + 2 c and + 8; rows past the end are zeros
+        uint2 qf[NT == 1 ? S::KS : 1];
+        auto load_q = [&](int nt, int ks) {
             const int r = r0 + 8 * nt + g;
-            if (r >= p.rows) return make_uint4(0, 0, 0, 0);
+            if (r >= p.rows) return make_uint2(0, 0);
             const int j = r / p.group, h = head * p.group + r - j * p.group;
-            return __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (static_cast<int64_t>(seq) * p.n_q + j) * p.ldq +
-                                                         static_cast<int64_t>(h) * D + 32 * i + 8 * c));
+            const T *q = static_cast<const T *>(p.q) + (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldq + static_cast<int64_t>(h) * D +
+                         16 * ks + 2 * c;
+            return make_uint2(__ldg(reinterpret_cast<const unsigned *>(q)), __ldg(reinterpret_cast<const unsigned *>(q + 8)));
         };
         if (NT == 1) {
 #pragma unroll
-            for (int i = 0; i < S::NK; ++i) qf[NT == 1 ? i : 0] = load_q(0, i);
+            for (int ks = 0; ks < S::KS; ++ks) qf[NT == 1 ? ks : 0] = load_q(0, ks);
         } else {
-            for (int x = warp; x < NT * S::NK; x += AT_WARPS) s_q[x * 32 + lane] = load_q(x / S::NK, x % S::NK);
+            for (int x = warp; x < NT * S::KS; x += AT_WARPS) s_q[x * 32 + lane] = load_q(x / S::KS, x % S::KS);
             __syncthreads();
         }
-        // slots that rows 2c, 2c + 1 of each tile see
-        int seen[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) seen[nt][e] = len - (p.n_q - 1 - min((r0 + 8 * nt + 2 * c + e) / p.group, p.n_q - 1));
-        const int all_see = len - p.n_q + 1;  // slots below are seen by every row
+        // slots below are seen by every row; row 8 nt + 2 c + e sees `seen` of them
+        const int all_see = sg.len - p.n_q + 1;
+        auto seen = [&](int nt, int e) { return all_see + min((r0 + 8 * nt + 2 * c + e) / p.group, p.n_q - 1); };
 
-        float o[NT][S::MT][4], m[NT][2], l[NT][2];
+        // running maximum m of each row (and 0 in its place while it is -infinity), sum, result
+        float o[NT][S::KS][4], m[NT][2], sub[NT][2], l[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int mt = 0; mt < S::MT; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
+            for (int mt = 0; mt < S::KS; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
             m[nt][0] = m[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.0f;
+            sub[nt][0] = sub[nt][1] = l[nt][0] = l[nt][1] = 0.0f;
         }
 
-        // lane's row of a tile is slot base + lane % 16: its page, then its offsets
-        const int64_t table_row = static_cast<int64_t>(seq) * p.kv.a.table_stride;
-        auto fetch_page = [&](int base) {
-            const int t = base + (lane & 15);
-            return t < slot_end ? __ldg(p.kv.a.table + table_row + p.kv.page.div(t)) : 0;
-        };
-        int64_t k_off, v_off, meta_off;
-        auto address = [&](int base, int page) {
-            const int t = base + (lane & 15), off = t - p.kv.page.div(t) * p.kv.a.page_size;
-            if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.kv.a.n_pages)) {
-                report_error(ERR_BAD_INDEX);
-                page = 0;
-            }
-            k_off = paged_k_at(p.kv, page, head, off);
-            v_off = paged_v_at(p.kv, page, head, off);
-            if (SCORES) meta_off = paged_meta_at(p.kv, page, head, off) * (p.row_blocks * S::R) + r0;
-        };
-        uint4 kf[2][S::NK], vf[4][S::NV];
-        auto load_k = [&](int base) {
+        for (int base = sg.tile0 * STEP + warp * TILE; base < sg.slot_end; base += STEP) {
+            // scores: slots g, g + 8 of the tile by rows 2c, 2c + 1 of each block of
+            // eight; a lone block gets two sums, for two chains of half the length
+            constexpr int CH = NT == 1 ? 2 : 1;
+            float sc[NT][4], part[CH][NT][4];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int row = g + 8 * x;
-                const T *src = kp + __shfl_sync(0xffffffffu, k_off, row) + 8 * c;
-                const bool ok = base + row < slot_end;
+            for (int x = 0; x < CH; ++x)
 #pragma unroll
-                for (int i = 0; i < S::NK; ++i) kf[x][i] = ok ? ld_stream(src + 32 * i) : make_uint4(0, 0, 0, 0);
-            }
-        };
-        auto load_v = [&](int base, int64_t off) {
+                for (int nt = 0; nt < NT; ++nt) part[x][nt][0] = part[x][nt][1] = part[x][nt][2] = part[x][nt][3] = 0.0f;
+            copy_wait<2 * S::DEPTH - 1>();
+            __syncwarp();
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int row = 2 * c + (x & 1) + 8 * (x >> 1);
-                const T *src = vp + __shfl_sync(0xffffffffu, off, row) + 8 * g;
-                const bool ok = base + row < slot_end;
+            for (int ks = 0; ks < S::KS; ++ks) {
+                uint32_t a[4];
+                ldm(a, at + k_lane + ks * 32);
 #pragma unroll
-                for (int j = 0; j < S::NV; ++j)
-                    vf[x][j] = ok && 64 * j + 8 * g < D ? ld_stream(src + 64 * j) : make_uint4(0, 0, 0, 0);
-            }
-        };
-
-        int base = tile0 * STEP + warp * TILE;
-        if (base < slot_end) {
-            address(base, fetch_page(base));
-            load_k(base);
-            load_v(base, v_off);
-            int page_next = fetch_page(base + STEP);
-            for (; base < slot_end; base += STEP) {
-                // scores: rows of the tile (slots g, g + 8) by rows of the block (2c, 2c + 1)
-                float sc[NT][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < S::NK; ++i)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const uint4 q = NT == 1 ? qf[NT == 1 ? i : 0] : s_q[(nt * S::NK + i) * 32 + lane];
-                        mma_16x8x16<T>(sc[nt], kf[0][i].x, kf[1][i].x, kf[0][i].y, kf[1][i].y, q.x, q.y);
-                        mma_16x8x16<T>(sc[nt], kf[0][i].z, kf[1][i].z, kf[0][i].w, kf[1][i].w, q.z, q.w);
-                    }
-                const int64_t v_this = v_off, meta_this = meta_off;
-                const int next = base + STEP;
-                if (next < slot_end) {
-                    address(next, page_next);
-                    load_k(next);
-                    page_next = fetch_page(next + STEP);
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint2 q = NT == 1 ? qf[NT == 1 ? ks : 0] : s_q[(nt * S::KS + ks) * 32 + lane];
+                    mma_16x8x16<T>(part[ks % CH][nt], a[0], a[1], a[2], a[3], q.x, q.y);
                 }
-                // log2 units, the mask, and the rows' maxima
-                const bool edge = base + TILE > all_see;
-                bool raise = false;
+            }
+            __syncwarp();
+            fetch_k();  // into the tile just read
+            // log2 units, the mask, and the rows' maxima
+            const bool edge = base + TILE > all_see;
+            bool raise = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[nt][e] = (CH == 2 ? part[0][nt][e] + part[CH - 1][nt][e] : part[0][nt][e]) * p.scale_log2;
+                    if (edge && base + g + 8 * (e >> 1) >= seen(nt, e & 1)) sc[nt][e] = -INFINITY;
+                    raise |= sc[nt][e] > m[nt][e & 1] + RAISE;
+                }
+            if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        sc[nt][e] *= p.scale_log2;
-                        if (edge && base + g + 8 * (e >> 1) >= min(seen[nt][e & 1], slot_end)) sc[nt][e] = -INFINITY;
-                        raise |= sc[nt][e] > m[nt][e & 1] + RAISE;
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(sc[nt][e], sc[nt][e + 2]);
+#pragma unroll
+                        for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                        top = fmaxf(top, m[nt][e]);
+                        const float k = scaled(m[nt][e], top);
+                        m[nt][e] = top;
+                        sub[nt][e] = top == -INFINITY ? 0.0f : top;
+                        l[nt][e] *= k;
+#pragma unroll
+                        for (int mt = 0; mt < S::KS; ++mt) o[nt][mt][e] *= k, o[nt][mt][e + 2] *= k;
                     }
-                if (__any_sync(0xffffffffu, raise)) {
+            }
+            if (SCORES) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                for (int x = 0; x < 2; ++x) {
+                    const int t = base + g + 8 * x, e = p.kv.page.div(t);
+                    if (t < sg.slot_end) {
+                        const int page = max(0, paged_page(p.kv, sg.seq, e));
+                        float *to = p.scores + paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size) * (p.row_blocks * S::R) + r0;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float top = fmaxf(sc[nt][e], sc[nt][e + 2]);
-#pragma unroll
-                            for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                            top = fmaxf(top, m[nt][e]);
-                            const float f = top == m[nt][e] ? 1.0f : exp2_fast(m[nt][e] - top);
-                            m[nt][e] = top;
-                            l[nt][e] *= f;
-#pragma unroll
-                            for (int mt = 0; mt < S::MT; ++mt) o[nt][mt][e] *= f, o[nt][mt][e + 2] *= f;
-                        }
-                }
-                if (SCORES) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int64_t to = __shfl_sync(0xffffffffu, meta_this, g + 8 * x);
-                        if (base + g + 8 * x < slot_end)
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                *reinterpret_cast<float2 *>(p.scores + to + 8 * nt + 2 * c) = make_float2(sc[nt][2 * x], sc[nt][2 * x + 1]);
+                        for (int nt = 0; nt < NT; ++nt)
+                            *reinterpret_cast<float2 *>(to + 8 * nt + 2 * c) = make_float2(sc[nt][2 * x], sc[nt][2 * x + 1]);
                     }
                 }
-                // weights, as the sum of two 16-bit values: the tensor cores take
-                // 16-bit operands, and one rounding would cost as much precision
-                // as the result's own
-                uint32_t hi[NT][2], lo[NT][2];
+            }
+            // weights, as the sum of two 16-bit values: the tensor cores take
+            // 16-bit operands, and one rounding would cost as much precision
+            // as the result's own
+            uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[nt][e] = exp2_fast(sc[nt][e] - sub[nt][e & 1]);
+                    l[nt][e & 1] += sc[nt][e];
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const uint32_t h = pack2<T>(sc[nt][2 * x], sc[nt][2 * x + 1]);
+                    const float2 r = unpack2<T>(h);
+                    hi[nt][x] = trans8x8(h);
+                    lo[nt][x] = trans8x8(pack2<T>(sc[nt][2 * x] - r.x, sc[nt][2 * x + 1] - r.y));
+                }
+            }
+            copy_wait<2 * S::DEPTH - 1>();
+            __syncwarp();
+            // A slot that only some rows see has weight 0 in the others, and 0
+            // times an infinity or NaN in its V row would reach them: such
+            // elements count as zeros here and are added row by row below.
+            bool odd = false;
+            if (edge && p.n_q > 1) {
+#pragma unroll 1
+                for (int i = 0; i < S::COPIES; ++i) {
+                    const int x = 32 * i + lane, row = x / S::CHUNKS, chunk = x - row * S::CHUNKS;
+                    uint4 *v = reinterpret_cast<uint4 *>(smem + (at - smem_u32(smem)) + S::TILE_BYTES + row * S::ROW + chunk * 16);
+                    bool any = false;
+                    const uint4 y = make_uint4(finite_part<T>(v->x, any), finite_part<T>(v->y, any), finite_part<T>(v->z, any),
+                                               finite_part<T>(v->w, any));
+                    if (any) *v = y, odd = true;
+                }
+                odd = __any_sync(0xffffffffu, odd);
+                __syncwarp();
+            }
+#pragma unroll
+            for (int mt = 0; mt < S::KS; ++mt) {
+                uint32_t a[4];
+                ldm_trans(a, at + v_lane + mt * 32);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float mm = m[nt][e & 1];
-                        sc[nt][e] = exp2_fast(sc[nt][e] - (mm == -INFINITY ? 0.0f : mm));
-                        l[nt][e & 1] += sc[nt][e];
-                    }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t h = pack2<T>(sc[nt][2 * x], sc[nt][2 * x + 1]);
-                        const float2 f = unpack2<T>(h);
-                        hi[nt][x] = trans8x8(h);
-                        lo[nt][x] = trans8x8(pack2<T>(sc[nt][2 * x] - f.x, sc[nt][2 * x + 1] - f.y));
-                    }
+                    mma_16x8x16<T>(o[nt][mt], a[0], a[1], a[2], a[3], hi[nt][0], hi[nt][1]);
+                    mma_16x8x16<T>(o[nt][mt], a[0], a[1], a[2], a[3], lo[nt][0], lo[nt][1]);
                 }
-                // A slot that only some rows see has weight 0 in the others, and 0
-                // times an infinity or NaN in its V row would reach them: such
-                // elements are taken out here and added row by row below.
-                bool odd = false;
-                if (edge && p.n_q > 1) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-#pragma unroll
-                        for (int j = 0; j < S::NV; ++j) {
-                            vf[x][j].x = finite_part<T>(vf[x][j].x, odd);
-                            vf[x][j].y = finite_part<T>(vf[x][j].y, odd);
-                            vf[x][j].z = finite_part<T>(vf[x][j].z, odd);
-                            vf[x][j].w = finite_part<T>(vf[x][j].w, odd);
-                        }
-                    odd = __any_sync(0xffffffffu, odd);
-                }
-#pragma unroll
-                for (int mt = 0; mt < S::MT; ++mt) {
-                    const uint32_t v0 = reinterpret_cast<const uint32_t *>(&vf[0][mt / 4])[mt % 4];
-                    const uint32_t v1 = reinterpret_cast<const uint32_t *>(&vf[1][mt / 4])[mt % 4];
-                    const uint32_t v2 = reinterpret_cast<const uint32_t *>(&vf[2][mt / 4])[mt % 4];
-                    const uint32_t v3 = reinterpret_cast<const uint32_t *>(&vf[3][mt / 4])[mt % 4];
-                    const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
-                    const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
+            }
+            __syncwarp();
+            fetch_v();
+            at += 2 * S::TILE_BYTES;
+            if (at == ring + S::DEPTH * 2 * S::TILE_BYTES) at = ring;
+            if (odd) {
+                for (int t = 0; t < TILE && base + t < sg.slot_end; ++t) {
+                    const int e = p.kv.page.div(base + t), page = max(0, paged_page(p.kv, sg.seq, e));
+                    const T *src = static_cast<const T *>(p.kv.a.v) +
+                                   paged_v_at(p.kv, page, head, base + t - e * p.kv.a.page_size) + g;
+                    const int from = (t & 7) * 4 + c;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma_16x8x16<T>(o[nt][mt], a0, a1, a2, a3, hi[nt][0], hi[nt][1]);
-                        mma_16x8x16<T>(o[nt][mt], a0, a1, a2, a3, lo[nt][0], lo[nt][1]);
-                    }
-                }
-                if (odd) {
-                    for (int t = 0; t < TILE; ++t) {
-                        const T *src = vp + __shfl_sync(0xffffffffu, v_this, t) + 8 * g;
-                        const int from = (t & 7) * 4 + c;
+                        const float w0 = __shfl_sync(0xffffffffu, t < 8 ? sc[nt][0] : sc[nt][2], from);
+                        const float w1 = __shfl_sync(0xffffffffu, t < 8 ? sc[nt][1] : sc[nt][3], from);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            const float w0 = __shfl_sync(0xffffffffu, t < 8 ? sc[nt][0] : sc[nt][2], from);
-                            const float w1 = __shfl_sync(0xffffffffu, t < 8 ? sc[nt][1] : sc[nt][3], from);
-                            if (base + t >= slot_end) continue;
+                        for (int mt = 0; mt < S::KS; ++mt)
 #pragma unroll
-                            for (int mt = 0; mt < S::MT; ++mt) {
-                                if (64 * (mt / 4) + 8 * g >= D) continue;
-                                const float2 f = unpack2<T>(*reinterpret_cast<const uint32_t *>(src + 64 * (mt / 4) + 2 * (mt % 4)));
-#pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const float v = e ? f.y : f.x;
-                                    if (isfinite(v)) continue;
-                                    if (base + t < seen[nt][0]) o[nt][mt][2 * e] += w0 * v;
-                                    if (base + t < seen[nt][1]) o[nt][mt][2 * e + 1] += w1 * v;
-                                }
+                            for (int y = 0; y < 2; ++y) {
+                                const float v = Half16<T>::up(src[16 * mt + 8 * y]);
+                                if (isfinite(v)) continue;
+                                if (base + t < seen(nt, 0)) o[nt][mt][2 * y] += w0 * v;
+                                if (base + t < seen(nt, 1)) o[nt][mt][2 * y + 1] += w1 * v;
                             }
-                        }
                     }
                 }
-                if (next < slot_end) load_v(next, v_off);
             }
         }
 
-        // ---- join the warps: maximum, then scaled sums in shared memory ----
+        // ---- join the warps: maxima, then the scaled sums, one warp after another ----
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -489,43 +584,45 @@ __global__ void __launch_bounds__(AT_THREADS, Shape<D, NT>::MIN_CTAS) attend_ker
                 }
             }
         __syncthreads();
+        auto top_of = [&](int r) {
+            float top = s_m[r];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int x = 1; x < AT_WARPS; ++x) top = fmaxf(top, s_m[x * S::R + r]);
+            return top;
+        };
+#pragma unroll 1
+        for (int turn = 0; turn < AT_WARPS; ++turn) {
+            if (warp == turn) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = 8 * nt + 2 * c + e;
-                float top = s_m[r];
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int w = 1; w < AT_WARPS; ++w) top = fmaxf(top, s_m[w * S::R + r]);
-                const float f = m[nt][e] == top ? 1.0f : exp2_fast(m[nt][e] - top);
-                float *dst = s_o + (warp * S::R + r) * S::PITCH;
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = 8 * nt + 2 * c + e;
+                        const float k = scaled(m[nt][e], top_of(r));
+                        float *dst = s_o + r * S::PITCH + g;
 #pragma unroll
-                for (int mt = 0; mt < S::MT; mt += 2) {
-                    const int d = 64 * (mt / 4) + 8 * g + 2 * (mt % 4);
-                    if (d < D)
-                        *reinterpret_cast<float4 *>(dst + d) = make_float4(o[nt][mt][e] * f, o[nt][mt][e + 2] * f,
-                                                                           o[nt][mt + 1][e] * f, o[nt][mt + 1][e + 2] * f);
-                }
+                        for (int mt = 0; mt < S::KS; ++mt)
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const float x = o[nt][mt][e + 2 * y] * k;
+                                dst[16 * mt + 8 * y] = turn ? dst[16 * mt + 8 * y] + x : x;
+                            }
+                    }
             }
-        __syncthreads();
-        const bool whole = tile0 == 0 && tile1 == n;
-        const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (pos == begin ? 0 : 1);
+            __syncthreads();
+        }
+        const bool whole = sg.tile0 == 0 && sg.tile1 == sg.n;
+        const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (w.pos == begin ? 0 : 1);
         for (int i = tid; i < S::R * (D / 4); i += AT_THREADS) {
             const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
             if (r0 + r >= p.rows) break;
-            float top = s_m[r], total = 0.0f;
+            const float top = top_of(r);
+            float total = 0.0f;
 #pragma unroll
-            for (int w = 1; w < AT_WARPS; ++w) top = fmaxf(top, s_m[w * S::R + r]);
-            float4 sum = make_float4(0, 0, 0, 0);
-#pragma unroll
-            for (int w = 0; w < AT_WARPS; ++w) {
-                const float mw = s_m[w * S::R + r];
-                total += s_l[w * S::R + r] * (mw == top ? 1.0f : exp2_fast(mw - top));
-                const float4 x = *reinterpret_cast<const float4 *>(s_o + (w * S::R + r) * S::PITCH + d);
-                sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
-            }
+            for (int x = 0; x < AT_WARPS; ++x) total += s_l[x * S::R + r] * scaled(s_m[x * S::R + r], top);
+            const float4 sum = *reinterpret_cast<const float4 *>(s_o + r * S::PITCH + d);
             if (whole) {
-                finish_row<T>(p, seq, head, r0 + r, d, D, sum, top, total);
+                finish_row<T>(p, sg.seq, head, r0 + r, d, D, sum, top, total);
             } else {
                 *reinterpret_cast<float4 *>(p.part_o + (slot * S::R + r) * D + d) = sum;
                 if (d == 0) p.part_ml[slot * S::R + r] = make_float2(top, total);
@@ -533,78 +630,88 @@ __global__ void __launch_bounds__(AT_THREADS, Shape<D, NT>::MIN_CTAS) attend_ker
         }
         if (!whole) {
             // ---- the last of the row's segments to arrive joins them, in order ----
-            const int first = line.piece(row_begin), last = line.piece(row_begin + n - 1);
-            unsigned *arrived = p.arrived + first;
+            const int first = line.piece(sg.row_begin), last = line.piece(sg.row_begin + sg.n - 1);
             __threadfence();
             __syncthreads();
-            if (tid == 0) s_last = atomicAdd(arrived, 1u) == static_cast<unsigned>(last - first);
+            if (tid == 0) s_last = atomicAdd(p.arrived + first, 1u) == static_cast<unsigned>(last - first);
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                if (tid == 0) *arrived = 0;  // ready for the next call
-                for (int r = warp; r < S::R && r0 + r < p.rows; r += AT_WARPS) {
-                    // piece x holds the row's segment in its first slot unless it begins before the row
-                    auto slot_of = [&](int x) { return (static_cast<int64_t>(x) * 2 + (line.begin(x) < row_begin ? 1 : 0)) * S::R + r; };
-                    float top = -INFINITY;
-                    for (int x = first + lane; x <= last; x += 32) top = fmaxf(top, __ldcg(p.part_ml + slot_of(x)).x);
+                if (tid == 0) p.arrived[first] = 0;  // ready for the next call
+                // a piece that begins before the row has its segment in its second slot
+                const int64_t second = line.begin(first) < sg.row_begin ? 1 : 0;
+                auto slot_of = [&](int x) { return (static_cast<int64_t>(x) * 2 + (x == first ? second : 0)) * S::R; };
+                // the rows' maxima: LR lanes a row
+                constexpr int LR = AT_THREADS / S::R, CHUNK = S::PITCH;
+                const int mr = tid / LR, ml = tid % LR;
+                float top = -INFINITY, total = 0.0f;
+                for (int x = first + ml; x <= last; x += LR) top = fmaxf(top, __ldcg(p.part_ml + slot_of(x) + mr).x);
 #pragma unroll
-                    for (int x = 16; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                    float total = 0.0f;
-                    float4 sum = make_float4(0, 0, 0, 0);
+                for (int x = 1; x < LR; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                // the segments' factors, CHUNK at a time, then the sums
+                constexpr int LD = D / 4, RG = AT_THREADS / LD, RT = (S::R + RG - 1) / RG;
+                const int d = tid % LD, rg = tid / LD;
+                float4 sum[RT];
+#pragma unroll
+                for (int i = 0; i < RT; ++i) sum[i] = make_float4(0, 0, 0, 0);
+                for (int x0 = first; x0 <= last; x0 += CHUNK) {
+                    const int nx = min(CHUNK, last + 1 - x0);
+                    __syncthreads();
+                    for (int x = ml; x < nx; x += LR) {
+                        const float2 y = __ldcg(p.part_ml + slot_of(x0 + x) + mr);
+                        const float k = scaled(y.x, top);
+                        total += y.y * k;
+                        s_o[mr * CHUNK + x] = k;
+                    }
+                    __syncthreads();
 #pragma unroll 4
-                    for (int x = first; x <= last; ++x) {
-                        const int64_t from = slot_of(x);
-                        const float2 ml = __ldcg(p.part_ml + from);
-                        const float f = ml.x == top ? 1.0f : exp2_fast(ml.x - top);
-                        total += ml.y * f;
-                        if (lane < D / 4) {
-                            const float4 y = __ldcg(reinterpret_cast<const float4 *>(p.part_o + from * D + 4 * lane));
-                            sum.x += f * y.x, sum.y += f * y.y, sum.z += f * y.z, sum.w += f * y.w;
+                    for (int x = 0; x < nx; ++x) {
+                        const float *src = p.part_o + slot_of(x0 + x) * D + 4 * d;
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) {
+                            const int r = rg + i * RG;
+                            if (rg < RG && r < S::R && r0 + r < p.rows) {
+                                const float k = s_o[r * CHUNK + x];
+                                const float4 y = __ldcg(reinterpret_cast<const float4 *>(src + r * D));
+                                sum[i].x += k * y.x, sum[i].y += k * y.y, sum[i].z += k * y.z, sum[i].w += k * y.w;
+                            }
                         }
                     }
-                    if (lane < D / 4) finish_row<T>(p, seq, head, r0 + r, 4 * lane, D, sum, top, total);
+                }
+#pragma unroll
+                for (int x = 1; x < LR; x <<= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+                if (ml == 0) s_m[mr] = top, s_l[mr] = total;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    const int r = rg + i * RG;
+                    if (rg < RG && r < S::R && r0 + r < p.rows) finish_row<T>(p, sg.seq, head, r0 + r, 4 * d, D, sum[i], s_m[r], s_l[r]);
                 }
             }
         }
         __syncthreads();  // the join buffer and Q are free again
-        pos = row_begin + tile1;
-        if (pos < end && pos == seq_begin + static_cast<int64_t>(n) * units) {
-            seq_begin = pos;
-            do len = paged_len(p.kv, ++seq);
-            while (len == 0);
-        }
-    }
+    } while (w.next(p.kv));
 }
 
 // acc += the slots' weights: exp2(score - lse) summed over the rows, a thread
 // for four rows of a slot, on the same line of steps as the attention.
-template <int QUADS>  // float4s of a slot's padded rows that neighbouring lanes share
+constexpr int QUADS = 2;  // neighbouring lanes that share a slot
 __global__ void __launch_bounds__(AT_THREADS) accumulate_kernel(const __grid_constant__ AttendArgs p, int padded) {
-    const int tid = threadIdx.x, heads = p.kv.a.n_kv_heads;
-    Start at;
-    const Line line = find_start(p.kv, heads, at);
-    if (static_cast<int>(blockIdx.x) >= line.ctas) return;
-    int64_t pos = line.begin(blockIdx.x);
-    const int64_t end = line.begin(blockIdx.x + 1);
-    int seq = at.seq;
-    int64_t seq_begin = at.steps * heads;
-    int len = paged_len(p.kv, seq);
-    const int part = tid % QUADS;
-    while (pos < end) {
-        const int n = steps_of(len);
-        const int head = static_cast<int>((pos - seq_begin) / n);
-        const int64_t row_begin = seq_begin + static_cast<int64_t>(head) * n;
-        const int tile0 = static_cast<int>(pos - row_begin), tile1 = static_cast<int>(min(static_cast<int64_t>(n), end - row_begin));
-        const int slot_end = min(len, tile1 * STEP);
-        const float *lse = p.row_lse + (static_cast<int64_t>(seq) * heads + head) * p.rows;
-        for (int t0 = tile0 * STEP; t0 < slot_end; t0 += AT_THREADS / QUADS) {
+    const int tid = threadIdx.x, heads = p.kv.a.n_kv_heads, part = tid % QUADS;
+    Walk w;
+    find_start(p.kv, 1, w);
+    if (w.pos >= w.end) return;
+    do {
+        const Segment &sg = w.s;
+        const float *lse = p.row_lse + (static_cast<int64_t>(sg.seq) * heads + sg.unit) * p.rows;
+        for (int t0 = sg.tile0 * STEP; t0 < sg.slot_end; t0 += AT_THREADS / QUADS) {
             const int t = t0 + tid / QUADS;
             float sum = 0.0f;
             int64_t meta = -1;
-            if (t < slot_end) {
-                const int e = p.kv.page.div(t), page = paged_page(p.kv, seq, e);
+            if (t < sg.slot_end) {
+                const int e = p.kv.page.div(t), page = paged_page(p.kv, sg.seq, e);
                 if (page >= 0) {
-                    meta = paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size);
+                    meta = paged_meta_at(p.kv, page, sg.unit, t - e * p.kv.a.page_size);
                     for (int r = 4 * part; r < p.rows; r += 4 * QUADS) {
                         const float4 x = __ldcg(reinterpret_cast<const float4 *>(p.scores + meta * padded + r));
                         sum += exp2_fast(x.x - __ldcg(lse + r));
@@ -618,13 +725,7 @@ __global__ void __launch_bounds__(AT_THREADS) accumulate_kernel(const __grid_con
             for (int x = 1; x < QUADS; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
             if (meta >= 0 && part == 0) p.kv.a.acc[meta] += sum;
         }
-        pos = row_begin + tile1;
-        if (pos < end && pos == seq_begin + static_cast<int64_t>(n) * heads) {
-            seq_begin = pos;
-            do len = paged_len(p.kv, ++seq);
-            while (len == 0);
-        }
-    }
+    } while (w.next(p.kv));
 }
 
 // ------------------------------------------------------------------ host ---
@@ -643,11 +744,14 @@ int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumu
     const int rows = n_heads / kv->n_kv_heads * n_q;
     pl.nt = tile_count(rows);
     pl.row_blocks = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
+    const int64_t steps = (static_cast<int64_t>(kv->max_pages) * kv->page_size + STEP - 1) / STEP;
+    if (steps * kv->n_seqs * kv->n_kv_heads * pl.row_blocks > 0x7fffffff)
+        return paged_fail(ABRA_E_UNSUPPORTED, "the tables name over 2^31 steps of %d slots", STEP);
     pl.ctas = pl.sms * (pl.nt == 1 ? 3 : 2);
     const int64_t padded = static_cast<int64_t>(pl.row_blocks) * 8 * pl.nt;
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     int64_t at = 0;
-    pl.arrived = at, at = up(at + static_cast<int64_t>(pl.sms) * MAX_CTAS * 4);  // the same place for all arguments
+    pl.arrived = at, at = up(at + static_cast<int64_t>(pl.ctas) * 4);  // the same place for all arguments
     pl.part_o = at, at = up(at + static_cast<int64_t>(pl.ctas) * 2 * 8 * pl.nt * kv->head_dim * 4);
     pl.part_ml = at, at = up(at + static_cast<int64_t>(pl.ctas) * 2 * 8 * pl.nt * 8);
     pl.row_lse = pl.scores = at;
@@ -663,10 +767,8 @@ int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumu
 template <typename T, int D, int NT, bool SCORES>
 cudaError_t launch_one(const AttendArgs &p, const Plan &pl, cudaStream_t st) {
     constexpr int smem = Shape<D, NT>::SMEM;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D, NT, SCORES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return e;
-    }
+    const cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D, NT, SCORES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
     attend_kernel<T, D, NT, SCORES><<<pl.ctas, AT_THREADS, smem, st>>>(p);
     return cudaGetLastError();
 }
@@ -688,7 +790,7 @@ template <typename T> cudaError_t launch(const AttendArgs &p, const Plan &pl, bo
     const cudaError_t e = launch_dim<T, true>(p, pl, st);
     if (e != cudaSuccess) return e;
     const int padded = pl.row_blocks * 8 * pl.nt;
-    accumulate_kernel<2><<<pl.sms * 8, AT_THREADS, 0, st>>>(p, padded);
+    accumulate_kernel<<<pl.sms * 8, AT_THREADS, 0, st>>>(p, padded);
     return cudaGetLastError();
 }
 
