@@ -9,8 +9,12 @@
 // Bound: a slot of one kv head is 4 D bytes for 4 D flops a row, and a kv head
 // has few rows (group x n_q), so the kernel is bound by reading the cache once.
 // The work is cut evenly whatever the lengths are: the steps of 64 slots of all
-// (sequence, kv head, block of rows) triples form one line, and each of the
-// resident CTAs takes an equal piece of it, crossing from triple to triple.
+// (sequence, kv head, block of rows) triples form one line, cut into equal
+// pieces of one CTA each, which cross from triple to triple.  There are several
+// pieces to a resident CTA where there is enough work, because CTAs with the
+// same bytes to read finish at very different times (43 to 93 us of one
+// 131,071-slot sequence in 444 equal pieces).  A second kernel joins the rows
+// that were split and adds the weights.
 //
 // Layout: both products run on the tensor cores with the slots (16 a warp) as
 // the tall side and the rows (8 a tile) as the narrow one, S^T = K Q^T and O^T
@@ -20,6 +24,8 @@
 // ends of the rows; no warp waits for another before a row ends.  Rows in the
 // ring are padded by 16 bytes, so the eight rows of an ldmatrix lie in distinct
 // banks.
+#include <algorithm>
+
 #include "paged_kv.cuh"
 
 namespace abra {
@@ -29,9 +35,14 @@ constexpr int AT_WARPS = 4, AT_THREADS = AT_WARPS * 32;
 constexpr int TILE = 16;                  // slots of a warp's tile
 constexpr int STEP = TILE * AT_WARPS;     // slots of a CTA's step
 constexpr int SCAN = AT_THREADS;          // sequences of one block scan
+constexpr int PIECE = 8;                  // steps of a piece, where there are enough to fill the GPU
+constexpr int WAVES = 4;                  // pieces for each CTA that the GPU holds, at most
 // A row's maximum is raised only when a score passes it by 2^RAISE: weights
 // stay below 2^RAISE (well inside fp16), and most tiles need no reduction.
 constexpr float RAISE = 10.0f;
+// What beginning and ending a row costs beside its steps, in steps (its
+// queries, the join of its warps).
+constexpr int ROW_COST = 1;
 
 struct AttendArgs {
     PagedKv kv;
@@ -41,11 +52,12 @@ struct AttendArgs {
     int64_t ldq, ldo;
     float scale_log2;  // scale / ln 2: scores are kept in units of log2
     int n_heads, n_q, group, rows, row_blocks, out_f32;
+    int resident;  // CTAs of the first kernel that the GPU holds at once
     // workspace
-    unsigned *arrived;  // [cta] segments done of the split row that begins in that CTA's piece (at most one)
-    float *part_o;      // [cta][2][8 NT][D]
-    float2 *part_ml;    // [cta][2][8 NT] maximum (log2 units) and sum
-    float *row_lse;     // [seq][kv head][row] log2 of the sum, +inf for a row that sees nothing
+    float *part_o;      // [piece][2][8 NT][D]
+    float2 *part_ml;    // [piece][2][8 NT] maximum (log2 units) and sum
+    int2 *split;        // [seq][kv head][row block] the first part's place, the last part's piece
+    float *row_lse;     // [seq][kv head][row] log2 of the sum of a row that lies in one piece
     float *scores;      // [page][kv head][offset][padded rows], log2 units
 };
 
@@ -129,65 +141,70 @@ template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t x
 __device__ __forceinline__ int steps_of(int len) { return (len + STEP - 1) / STEP; }
 
 struct Line {
-    int total;  // steps of all triples
-    int ctas;   // pieces; each has at least one step
-    __device__ __forceinline__ int begin(int cta) const {
-        return static_cast<int>(static_cast<int64_t>(cta) * total / ctas);
+    int total;       // the triples' costs
+    int pieces;      // each has at least one unit of cost
+    int quot, rest;  // total / pieces and what is left
+    __device__ __forceinline__ Line(int total, int pieces) : total(total), pieces(pieces), quot(0), rest(0) {
+        if (pieces > 0) quot = total / pieces, rest = total - quot * pieces;
     }
-    // the piece that holds step x
-    __device__ __forceinline__ int piece(int x) const {
-        return static_cast<int>((static_cast<int64_t>(x + 1) * ctas - 1) / total);
+    // the first `rest` pieces are one longer
+    __device__ __forceinline__ int begin(int i) const { return i * quot + min(i, rest); }
+    __device__ __forceinline__ int piece(int x) const {  // the piece that holds x
+        const int longer = rest * (quot + 1);
+        return x < longer ? x / (quot + 1) : rest + (x - longer) / quot;
     }
 };
 
 // A segment: the steps [tile0, tile1) of one triple that lie in a piece.
 struct Segment {
     int seq, len, n;          // the sequence, its slots and steps
-    int unit, row_begin;      // the triple of this sequence and its first step on the line
+    int unit, row_begin;      // the triple of this sequence and its first place on the line
     int head, block;          // its kv head and block of rows
     int tile0, tile1, slot_end;
 };
 
 // Walks the segments of the piece [pos, end).  `units` triples share a
-// sequence's length, `blocks` of them a kv head.
+// sequence's length, `blocks` of them a kv head; a triple of n steps takes
+// ROW_COST + n places.
 struct Walk {
     int pos, end, seq_begin, units, blocks;
     Segment s;
-    __device__ __forceinline__ void enter(const PagedKv &kv) {
-        s.len = paged_len(kv, s.seq);
-        s.n = steps_of(s.len);
-        while (pos >= seq_begin + s.n * units) {  // the next sequence with slots
-            seq_begin += s.n * units;
-            s.len = paged_len(kv, ++s.seq);
-            s.n = steps_of(s.len);
+    __device__ __forceinline__ int span() const { return s.n ? (s.n + ROW_COST) * units : 0; }
+    __device__ __forceinline__ void length(int len) { s.len = len, s.n = steps_of(len); }
+    // the segment at pos; false when the piece ends before its first step
+    __device__ __forceinline__ bool enter(const PagedKv &kv) {
+        while (pos >= seq_begin + span()) {  // the next sequence with slots
+            seq_begin += span();
+            length(paged_len(kv, ++s.seq));
         }
-        s.unit = (pos - seq_begin) / s.n;
+        s.unit = (pos - seq_begin) / (s.n + ROW_COST);
         s.head = s.unit / blocks;
         s.block = s.unit - s.head * blocks;
-        s.row_begin = seq_begin + s.unit * s.n;
-        s.tile0 = pos - s.row_begin;
-        s.tile1 = min(s.n, end - s.row_begin);
+        s.row_begin = seq_begin + s.unit * (s.n + ROW_COST);
+        s.tile0 = max(0, pos - s.row_begin - ROW_COST);
+        s.tile1 = min(s.n, end - s.row_begin - ROW_COST);
         s.slot_end = min(s.len, s.tile1 * STEP);
+        return s.tile0 < s.tile1;
     }
     // the next segment, if there is one
     __device__ __forceinline__ bool next(const PagedKv &kv) {
-        pos = s.row_begin + s.tile1;
-        if (pos >= end) return false;
-        enter(kv);
-        return true;
+        pos = s.row_begin + ROW_COST + s.tile1;
+        return pos < end && enter(kv);
     }
 };
 
-// Sums the sequences' steps and finds the one that this CTA's piece begins in
-// (w.end == w.pos: this CTA has no piece).  All threads of the block.
-__device__ __forceinline__ Line find_start(const PagedKv &kv, int blocks, Walk &w) {
-    __shared__ int s_warp[AT_WARPS], s_seq, s_steps;
+// Sums the sequences' costs and finds the one in which piece `piece` of at
+// most `most` begins; false when there is nothing in it.  All threads of the
+// block.
+__device__ __forceinline__ bool find_start(const PagedKv &kv, int blocks, int piece, int most, int least, Line &line, Walk &w) {
+    __shared__ int s_warp[AT_WARPS], s_seq, s_begin, s_len;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = kv.a.n_seqs;
     const int units = kv.a.n_kv_heads * blocks;
-    // inclusive scan of the steps of sequences base .. base + SCAN - 1
-    int own = 0, incl = 0, all = 0;
+    // inclusive scan of the costs of sequences base .. base + SCAN - 1
+    int len = 0, own = 0, incl = 0, all = 0;
     auto scan = [&](int base) {
-        own = base + tid < n ? steps_of(paged_len(kv, base + tid)) : 0;
+        len = base + tid < n ? paged_len(kv, base + tid) : 0;
+        own = len ? (steps_of(len) + ROW_COST) * units : 0;
         incl = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -204,35 +221,33 @@ __device__ __forceinline__ Line find_start(const PagedKv &kv, int blocks, Walk &
             all += s_warp[x];
         }
     };
-    int sum = 0;
+    int total = 0;
     for (int base = 0; base < n; base += SCAN) {
         scan(base);
-        sum += all;
+        total += all;
     }
-    Line line{sum * units, 0};
-    line.ctas = min(static_cast<int>(gridDim.x), line.total);
+    // as many pieces as the GPU holds at once, more where they stay long
+    line = Line(total, min(min(max(least, total / PIECE), most), total));
+    if (piece >= line.pieces) return false;
+    w.pos = line.begin(piece);
+    w.end = line.begin(piece + 1);
     w.units = units;
     w.blocks = blocks;
-    w.pos = w.end = 0;
-    if (static_cast<int>(blockIdx.x) >= line.ctas) return line;
-    w.pos = line.begin(blockIdx.x);
-    w.end = line.begin(blockIdx.x + 1);
-    const int x = w.pos / units;
     int before = 0;
     if (n <= SCAN) {
-        if (incl > x && incl - own <= x) s_seq = tid, s_steps = incl - own;
+        if (incl > w.pos && incl - own <= w.pos) s_seq = tid, s_begin = incl - own, s_len = len;
     } else {
-        for (int base = 0; before <= x; base += SCAN) {
+        for (int base = 0; before <= w.pos; base += SCAN) {
             scan(base);
-            if (before + incl > x && before + incl - own <= x) s_seq = base + tid, s_steps = before + incl - own;
+            if (before + incl > w.pos && before + incl - own <= w.pos) s_seq = base + tid, s_begin = before + incl - own, s_len = len;
             before += all;
         }
     }
     __syncthreads();
     w.s.seq = s_seq;
-    w.seq_begin = s_steps * units;
-    w.enter(kv);
-    return line;
+    w.seq_begin = s_begin;
+    w.length(s_len);
+    return w.enter(kv);
 }
 
 // --------------------------------------------------------------- kernel ---
@@ -277,7 +292,7 @@ __device__ __forceinline__ void finish_row(const AttendArgs &p, int seq, int hea
         const float l2 = total != 0.0f ? m + log2f(total) : -INFINITY;
         if (p.lse) p.lse[row * p.n_heads + h] = l2 * 0.69314718055994531f;
         if (p.row_lse)
-            p.row_lse[(static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.rows + r] = total != 0.0f ? l2 : INFINITY;
+            p.row_lse[(static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.rows + r] = l2;
     }
 }
 __device__ __forceinline__ float scaled(float m, float top) { return m == top ? 1.0f : exp2_fast(m - top); }
@@ -289,20 +304,12 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
     uint2 *s_q = reinterpret_cast<uint2 *>(smem + S::DEPTH * S::STAGE);  // [NT][KS][lane] Q fragments (NT > 1)
     float *s_o = reinterpret_cast<float *>(smem + S::DEPTH * S::STAGE + S::Q_BYTES);  // [R][PITCH]
     float *s_m = s_o + S::R * S::PITCH, *s_l = s_m + AT_WARPS * S::R;  // [warp][R]
-    __shared__ bool s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
 
+    pdl_launch_dependents();  // the join may take its place; it waits for the whole grid
     Walk w;
-    const Line line = find_start(p.kv, p.row_blocks, w);
-    // rows of empty sequences are nobody's: zeros and -infinity
-    for (int s = blockIdx.x; s < p.kv.a.n_seqs; s += gridDim.x) {
-        if (paged_len(p.kv, s) > 0) continue;
-        for (int i = tid; i < p.kv.a.n_kv_heads * p.rows * (D / 4); i += AT_THREADS) {
-            const int row = i / (D / 4), head = row / p.rows;
-            finish_row<T>(p, s, head, row - head * p.rows, (i - row * (D / 4)) * 4, D, make_float4(0, 0, 0, 0), 0.0f, 0.0f);
-        }
-    }
-    if (w.pos >= w.end) return;
+    Line line(0, 0);
+    if (!find_start(p.kv, p.row_blocks, blockIdx.x, gridDim.x, p.resident, line, w)) return;
     const int begin = w.pos;
 
     // ---- the fetching side: this warp's tiles, segment after segment ----
@@ -628,110 +635,162 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
                 if (d == 0) p.part_ml[slot * S::R + r] = make_float2(top, total);
             }
         }
-        if (!whole) {
-            // ---- the last of the row's segments to arrive joins them, in order ----
-            const int first = line.piece(sg.row_begin), last = line.piece(sg.row_begin + sg.n - 1);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) s_last = atomicAdd(p.arrived + first, 1u) == static_cast<unsigned>(last - first);
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                if (tid == 0) p.arrived[first] = 0;  // ready for the next call
-                // a piece that begins before the row has its segment in its second slot
-                const int64_t second = line.begin(first) < sg.row_begin ? 1 : 0;
-                auto slot_of = [&](int x) { return (static_cast<int64_t>(x) * 2 + (x == first ? second : 0)) * S::R; };
-                // the rows' maxima: LR lanes a row
-                constexpr int LR = AT_THREADS / S::R, CHUNK = S::PITCH;
-                const int mr = tid / LR, ml = tid % LR;
-                float top = -INFINITY, total = 0.0f;
-                for (int x = first + ml; x <= last; x += LR) top = fmaxf(top, __ldcg(p.part_ml + slot_of(x) + mr).x);
-#pragma unroll
-                for (int x = 1; x < LR; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                // the segments' factors, CHUNK at a time, then the sums
-                constexpr int LD = D / 4, RG = AT_THREADS / LD, RT = (S::R + RG - 1) / RG;
-                const int d = tid % LD, rg = tid / LD;
-                float4 sum[RT];
-#pragma unroll
-                for (int i = 0; i < RT; ++i) sum[i] = make_float4(0, 0, 0, 0);
-                for (int x0 = first; x0 <= last; x0 += CHUNK) {
-                    const int nx = min(CHUNK, last + 1 - x0);
-                    __syncthreads();
-                    for (int x = ml; x < nx; x += LR) {
-                        const float2 y = __ldcg(p.part_ml + slot_of(x0 + x) + mr);
-                        const float k = scaled(y.x, top);
-                        total += y.y * k;
-                        s_o[mr * CHUNK + x] = k;
-                    }
-                    __syncthreads();
-#pragma unroll 4
-                    for (int x = 0; x < nx; ++x) {
-                        const float *src = p.part_o + slot_of(x0 + x) * D + 4 * d;
-#pragma unroll
-                        for (int i = 0; i < RT; ++i) {
-                            const int r = rg + i * RG;
-                            if (rg < RG && r < S::R && r0 + r < p.rows) {
-                                const float k = s_o[r * CHUNK + x];
-                                const float4 y = __ldcg(reinterpret_cast<const float4 *>(src + r * D));
-                                sum[i].x += k * y.x, sum[i].y += k * y.y, sum[i].z += k * y.z, sum[i].w += k * y.w;
-                            }
-                        }
-                    }
-                }
-#pragma unroll
-                for (int x = 1; x < LR; x <<= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
-                if (ml == 0) s_m[mr] = top, s_l[mr] = total;
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    const int r = rg + i * RG;
-                    if (rg < RG && r < S::R && r0 + r < p.rows) finish_row<T>(p, sg.seq, head, r0 + r, 4 * d, D, sum[i], s_m[r], s_l[r]);
-                }
-            }
-        }
+        if (sg.tile0 == 0 && tid == 0)
+            p.split[static_cast<int64_t>(sg.seq) * w.units + sg.unit] =
+                make_int2(static_cast<int>(slot), whole ? static_cast<int>(blockIdx.x) : line.piece(sg.row_begin + ROW_COST + sg.n - 1));
         __syncthreads();  // the join buffer and Q are free again
     } while (w.next(p.kv));
 }
 
-// acc += the slots' weights: exp2(score - lse) summed over the rows, a thread
-// for four rows of a slot, on the same line of steps as the attention.
-constexpr int QUADS = 2;  // neighbouring lanes that share a slot
-__global__ void __launch_bounds__(AT_THREADS) accumulate_kernel(const __grid_constant__ AttendArgs p, int padded) {
-    const int tid = threadIdx.x, heads = p.kv.a.n_kv_heads, part = tid % QUADS;
+// Parts of a row: the first at place `first` (a piece has two), then one in the
+// first place of each piece up to `last`.
+struct Parts {
+    int first, last;
+    __device__ __forceinline__ Parts(int2 x) : first(x.x), last(x.y) {}
+    __device__ __forceinline__ int count() const { return last - (first >> 1) + 1; }
+    __device__ __forceinline__ int64_t place(int i) const { return i ? 2 * (static_cast<int64_t>(first >> 1) + i) : first; }
+};
+
+constexpr int JOIN_WARPS = 8;
+
+// The second kernel: a CTA for each output row.  It writes the rows of empty
+// sequences (zeros) and joins the split ones; the parts are dealt to the warps,
+// which meet in shared memory in a fixed order.
+template <typename T, int D>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ AttendArgs p, int r_block) {
+    __shared__ float s_top[JOIN_WARPS], s_total[JOIN_WARPS];
+    __shared__ __align__(16) float s_sum[JOIN_WARPS][D];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int r = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
+    pdl_launch_dependents();
+    pdl_wait();
+    if (paged_len(p.kv, seq) == 0) {
+        if (tid < D / 4) finish_row<T>(p, seq, head, r, 4 * tid, D, make_float4(0, 0, 0, 0), 0.0f, 0.0f);
+        return;
+    }
+    const int block = r / r_block;
+    const Parts parts(__ldcg(p.split + (static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.row_blocks + block));
+    const int n = parts.count();
+    if (n == 1) return;
+    const int rr = r - block * r_block;
+    // this warp's parts: warp, warp + JOIN_WARPS, ..., 32 of them at a time
+    float top = -INFINITY, total = 0.0f;
+    float4 sum = make_float4(0, 0, 0, 0);
+    for (int base = warp; base < n; base += 32 * JOIN_WARPS) {
+        const int mine = base + lane * JOIN_WARPS;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (mine < n) ml = __ldcg(p.part_ml + parts.place(mine) * r_block + rr);
+        float t = ml.x;
+#pragma unroll
+        for (int x = 16; x >= 1; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+        t = fmaxf(t, top);
+        const float keep = scaled(top, t), k = scaled(ml.x, t);
+        top = t;
+        total = total * keep + ml.y * k;  // lane by lane, added up below
+        sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
+        const int left = min(32, (n - base + JOIN_WARPS - 1) / JOIN_WARPS);
+#pragma unroll 8
+        for (int i = 0; i < left; ++i) {
+            const float ki = __shfl_sync(0xffffffffu, k, i);
+            if (lane < D / 4) {
+                const float4 y = __ldcg(reinterpret_cast<const float4 *>(
+                    p.part_o + (parts.place(base + i * JOIN_WARPS) * r_block + rr) * D + 4 * lane));
+                sum.x += ki * y.x, sum.y += ki * y.y, sum.z += ki * y.z, sum.w += ki * y.w;
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 16; x >= 1; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    if (lane == 0) s_top[warp] = top, s_total[warp] = total;
+    if (lane < D / 4) *reinterpret_cast<float4 *>(&s_sum[warp][4 * lane]) = sum;
+    __syncthreads();
+    if (tid >= D / 4) return;
+    top = s_top[0];
+    const int used = min(n, JOIN_WARPS);
+    for (int x = 1; x < used; ++x) top = fmaxf(top, s_top[x]);
+    total = 0.0f;
+    sum = make_float4(0, 0, 0, 0);
+    for (int x = 0; x < used; ++x) {
+        const float k = scaled(s_top[x], top);
+        const float4 y = *reinterpret_cast<const float4 *>(&s_sum[x][4 * tid]);
+        total += s_total[x] * k;
+        sum.x += k * y.x, sum.y += k * y.y, sum.z += k * y.z, sum.w += k * y.w;
+    }
+    finish_row<T>(p, seq, head, r, 4 * tid, D, sum, top, total);
+}
+
+// acc += the slots' weights, exp2(score - lse) summed over the rows, on pieces
+// of the same kind of line; two neighbouring lanes share a slot.  A row's lse
+// comes from its parts, so this needs the first kernel only.
+constexpr int ACC_ROWS = 64;  // rows whose lse is held at a time
+__global__ void __launch_bounds__(AT_THREADS) accumulate_kernel(const __grid_constant__ AttendArgs p, int r_block, int padded) {
+    __shared__ float s_lse[ACC_ROWS];
+    const int tid = threadIdx.x, heads = p.kv.a.n_kv_heads, half = tid & 1;
     Walk w;
-    find_start(p.kv, 1, w);
-    if (w.pos >= w.end) return;
+    Line line(0, 0);
+    pdl_wait();
+    if (!find_start(p.kv, 1, blockIdx.x, gridDim.x, gridDim.x, line, w)) return;
     do {
         const Segment &sg = w.s;
-        const float *lse = p.row_lse + (static_cast<int64_t>(sg.seq) * heads + sg.unit) * p.rows;
-        for (int t0 = sg.tile0 * STEP; t0 < sg.slot_end; t0 += AT_THREADS / QUADS) {
-            const int t = t0 + tid / QUADS;
-            float sum = 0.0f;
-            int64_t meta = -1;
-            if (t < sg.slot_end) {
-                const int e = p.kv.page.div(t), page = paged_page(p.kv, sg.seq, e);
-                if (page >= 0) {
-                    meta = paged_meta_at(p.kv, page, sg.unit, t - e * p.kv.a.page_size);
-                    for (int r = 4 * part; r < p.rows; r += 4 * QUADS) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p.scores + meta * padded + r));
-                        sum += exp2_fast(x.x - __ldcg(lse + r));
-                        if (r + 1 < p.rows) sum += exp2_fast(x.y - __ldcg(lse + r + 1));
-                        if (r + 2 < p.rows) sum += exp2_fast(x.z - __ldcg(lse + r + 2));
-                        if (r + 3 < p.rows) sum += exp2_fast(x.w - __ldcg(lse + r + 3));
+        for (int r0 = 0; r0 < p.rows; r0 += ACC_ROWS) {
+            const int nr = min(ACC_ROWS, p.rows - r0);
+            __syncthreads();
+            for (int i = tid >> 5; i < nr; i += AT_WARPS) {  // a warp a row
+                const int r = r0 + i, block = r / r_block;
+                const int64_t triple = (static_cast<int64_t>(sg.seq) * heads + sg.head);
+                const Parts parts(__ldcg(p.split + triple * p.row_blocks + block));
+                const int n = parts.count(), lane = tid & 31;
+                float lse;
+                if (n == 1) {
+                    lse = __ldcg(p.row_lse + triple * p.rows + r);
+                } else {
+                    float top = -INFINITY, total = 0.0f;
+                    for (int x = lane; x < n; x += 32) {
+                        const float2 ml = __ldcg(p.part_ml + parts.place(x) * r_block + r - block * r_block);
+                        const float t = fmaxf(top, ml.x);
+                        total = total * scaled(top, t) + ml.y * scaled(ml.x, t);
+                        top = t;
+                    }
+#pragma unroll
+                    for (int x = 16; x >= 1; x >>= 1) {
+                        const float ot = __shfl_xor_sync(0xffffffffu, top, x), on = __shfl_xor_sync(0xffffffffu, total, x);
+                        const float t = fmaxf(top, ot);
+                        total = total * scaled(top, t) + on * scaled(ot, t);
+                        top = t;
+                    }
+                    lse = total != 0.0f ? top + log2f(total) : -INFINITY;
+                }
+                if (lane == 0) s_lse[i] = lse == -INFINITY ? INFINITY : lse;  // a row that sees nothing weighs nothing
+            }
+            __syncthreads();
+            for (int t0 = sg.tile0 * STEP; t0 < sg.slot_end; t0 += AT_THREADS / 2) {
+                const int t = t0 + (tid >> 1);
+                float sum = 0.0f;
+                int64_t meta = -1;
+                if (t < sg.slot_end) {
+                    const int e = p.kv.page.div(t), page = paged_page(p.kv, sg.seq, e);
+                    if (page >= 0) {
+                        meta = paged_meta_at(p.kv, page, sg.head, t - e * p.kv.a.page_size);
+                        for (int i = 4 * half; i < nr; i += 8) {
+                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p.scores + meta * padded + r0 + i));
+                            sum += exp2_fast(x.x - s_lse[i]);
+                            if (i + 1 < nr) sum += exp2_fast(x.y - s_lse[i + 1]);
+                            if (i + 2 < nr) sum += exp2_fast(x.z - s_lse[i + 2]);
+                            if (i + 3 < nr) sum += exp2_fast(x.w - s_lse[i + 3]);
+                        }
                     }
                 }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                if (meta >= 0 && half == 0) p.kv.a.acc[meta] += sum;
             }
-#pragma unroll
-            for (int x = 1; x < QUADS; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            if (meta >= 0 && part == 0) p.kv.a.acc[meta] += sum;
         }
     } while (w.next(p.kv));
 }
 
 // ------------------------------------------------------------------ host ---
 struct Plan {
-    int nt, row_blocks, ctas, sms;
-    int64_t arrived, part_o, part_ml, row_lse, scores, bytes;  // workspace offsets
+    int nt, row_blocks, resident, pieces, sms;
+    int64_t part_o, part_ml, split, row_lse, scores, bytes;  // workspace offsets
 };
 
 int tile_count(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
@@ -744,23 +803,23 @@ int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumu
     const int rows = n_heads / kv->n_kv_heads * n_q;
     pl.nt = tile_count(rows);
     pl.row_blocks = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
-    const int64_t steps = (static_cast<int64_t>(kv->max_pages) * kv->page_size + STEP - 1) / STEP;
-    if (steps * kv->n_seqs * kv->n_kv_heads * pl.row_blocks > 0x7fffffff)
-        return paged_fail(ABRA_E_UNSUPPORTED, "the tables name over 2^31 steps of %d slots", STEP);
-    pl.ctas = pl.sms * (pl.nt == 1 ? 3 : 2);
-    const int64_t padded = static_cast<int64_t>(pl.row_blocks) * 8 * pl.nt;
+    const int64_t triples = static_cast<int64_t>(kv->n_seqs) * kv->n_kv_heads * pl.row_blocks;
+    const int64_t steps = (static_cast<int64_t>(kv->max_pages) * kv->page_size + STEP - 1) / STEP + ROW_COST;
+    if (steps * triples > 0x7fffffff) return paged_fail(ABRA_E_UNSUPPORTED, "the tables name over 2^31 steps of %d slots", STEP);
+    pl.resident = pl.sms * (pl.nt == 1 ? 3 : 2);
+    pl.pieces = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(pl.resident) * WAVES, steps * triples));
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     int64_t at = 0;
-    pl.arrived = at, at = up(at + static_cast<int64_t>(pl.ctas) * 4);  // the same place for all arguments
-    pl.part_o = at, at = up(at + static_cast<int64_t>(pl.ctas) * 2 * 8 * pl.nt * kv->head_dim * 4);
-    pl.part_ml = at, at = up(at + static_cast<int64_t>(pl.ctas) * 2 * 8 * pl.nt * 8);
+    pl.part_o = at, at = up(at + static_cast<int64_t>(pl.pieces) * 2 * 8 * pl.nt * kv->head_dim * 4);
+    pl.part_ml = at, at = up(at + static_cast<int64_t>(pl.pieces) * 2 * 8 * pl.nt * 8);
+    pl.split = at, at = up(at + triples * 8);
     pl.row_lse = pl.scores = at;
     if (accumulate) {
         at = up(at + static_cast<int64_t>(kv->n_seqs) * kv->n_kv_heads * rows * 4);
         pl.scores = at;
-        at = up(at + static_cast<int64_t>(kv->n_pages) * kv->n_kv_heads * kv->page_size * padded * 4);
+        at = up(at + static_cast<int64_t>(kv->n_pages) * kv->n_kv_heads * kv->page_size * pl.row_blocks * 8 * pl.nt * 4);
     }
-    pl.bytes = at + 256;
+    pl.bytes = at;
     return ABRA_OK;
 }
 
@@ -769,7 +828,7 @@ cudaError_t launch_one(const AttendArgs &p, const Plan &pl, cudaStream_t st) {
     constexpr int smem = Shape<D, NT>::SMEM;
     const cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D, NT, SCORES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    attend_kernel<T, D, NT, SCORES><<<pl.ctas, AT_THREADS, smem, st>>>(p);
+    attend_kernel<T, D, NT, SCORES><<<pl.pieces, AT_THREADS, smem, st>>>(p);
     return cudaGetLastError();
 }
 template <typename T, int D, bool SCORES>
@@ -778,20 +837,34 @@ cudaError_t launch_rows(const AttendArgs &p, const Plan &pl, cudaStream_t st) {
            : pl.nt == 2 ? launch_one<T, D, 2, SCORES>(p, pl, st)
                         : launch_one<T, D, 4, SCORES>(p, pl, st);
 }
-template <typename T, bool SCORES> cudaError_t launch_dim(const AttendArgs &p, const Plan &pl, cudaStream_t st) {
-    switch (p.kv.a.head_dim) {
-        case 64: return launch_rows<T, 64, SCORES>(p, pl, st);
-        case 96: return launch_rows<T, 96, SCORES>(p, pl, st);
-        default: return launch_rows<T, 128, SCORES>(p, pl, st);
-    }
+// A launch that may begin before the kernel in front of it has ended (its
+// pdl_wait waits for that).
+template <typename... A> cudaError_t launch_after(void (*k)(A...), dim3 grid, int threads, cudaStream_t st, A... a) {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, a...);
+}
+template <typename T, int D> cudaError_t launch_all(const AttendArgs &p, const Plan &pl, bool accumulate, cudaStream_t st) {
+    cudaError_t e = accumulate ? launch_rows<T, D, true>(p, pl, st) : launch_rows<T, D, false>(p, pl, st);
+    if (e != cudaSuccess) return e;
+    const int r_block = 8 * pl.nt;
+    e = launch_after(join_kernel<T, D>, dim3(p.rows, p.kv.a.n_kv_heads, p.kv.a.n_seqs), JOIN_WARPS * 32, st, p, r_block);
+    if (e != cudaSuccess || !accumulate) return e;
+    return launch_after(accumulate_kernel, dim3(pl.sms * 8), AT_THREADS, st, p, r_block, pl.row_blocks * r_block);
 }
 template <typename T> cudaError_t launch(const AttendArgs &p, const Plan &pl, bool accumulate, cudaStream_t st) {
-    if (!accumulate) return launch_dim<T, false>(p, pl, st);
-    const cudaError_t e = launch_dim<T, true>(p, pl, st);
-    if (e != cudaSuccess) return e;
-    const int padded = pl.row_blocks * 8 * pl.nt;
-    accumulate_kernel<<<pl.sms * 8, AT_THREADS, 0, st>>>(p, padded);
-    return cudaGetLastError();
+    switch (p.kv.a.head_dim) {
+        case 64: return launch_all<T, 64>(p, pl, accumulate, st);
+        case 96: return launch_all<T, 96>(p, pl, accumulate, st);
+        default: return launch_all<T, 128>(p, pl, accumulate, st);
+    }
 }
 
 int check(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, int32_t flags) {
@@ -857,9 +930,10 @@ extern "C" int abra_paged_attention(const abra_paged_kv *kv, const void *q, int6
                  group * n_q,
                  pl.row_blocks,
                  out_type == ABRA_GGML_F32,
-                 reinterpret_cast<unsigned *>(ws + pl.arrived),
+                 pl.resident,
                  reinterpret_cast<float *>(ws + pl.part_o),
                  reinterpret_cast<float2 *>(ws + pl.part_ml),
+                 reinterpret_cast<int2 *>(ws + pl.split),
                  accumulate ? reinterpret_cast<float *>(ws + pl.row_lse) : nullptr,
                  reinterpret_cast<float *>(ws + pl.scores)};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -203,13 +203,13 @@ def _size(n: int, func: str) -> int:
 
 
 def paged_attention_workspace(kv: PagedKV, n_heads: int, n_q: int = 1, accumulate: bool = False):
-    """A workspace for :func:`paged_attention` with these arguments: zeroed
-    bytes on the cache's device.  One serves any number of calls that follow
-    one another, all layers' among them; calls on several streams need one each."""
+    """A workspace for :func:`paged_attention` with these arguments
+    (uninitialised bytes).  One serves any number of calls that follow one
+    another, all layers' among them; calls on several streams need one each."""
     import torch
 
     n = lib.abra_paged_attention_workspace(kv._ref, n_heads, n_q, ABRA_PAGED_ACCUMULATE if accumulate else 0)
-    return torch.zeros(_size(n, "abra_paged_attention_workspace"), dtype=torch.uint8, device=kv.device)
+    return torch.empty(_size(n, "abra_paged_attention_workspace"), dtype=torch.uint8, device=kv.device)
 
 
 def paged_attention(kv: PagedKV, q, scale: float, out=None, lse=None, accumulate: bool = False,

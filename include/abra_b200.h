@@ -546,9 +546,8 @@ int abra_paged_append(const abra_paged_kv *kv, const void *q, const void *k, con
  * takes log sum_t exp(scale q.k_t).  A query that sees no slot gives zeros and
  * -infinity.  With ABRA_PAGED_ACCUMULATE every slot's softmax weight, summed
  * over the n_q queries and the group's heads, is added to acc.
- * workspace (256-byte aligned, abra_paged_attention_workspace bytes) must be
- * zero before its first use; each call leaves it ready for the next one,
- * whatever its arguments.  Calls that can overlap need a workspace each.
+ * workspace (256-byte aligned, abra_paged_attention_workspace bytes) may hold
+ * anything; calls that can overlap need one each.
  * head_dim 64, 96 or 128. */
 #define ABRA_PAGED_ACCUMULATE 1
 int64_t abra_paged_attention_workspace(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q,
