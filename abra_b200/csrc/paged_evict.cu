@@ -8,6 +8,15 @@
 // slot below the budget takes the i-th kept one above it, so sources (slots >=
 // budget) and targets (< budget) never meet and the order of the copies does
 // not matter.
+//
+// Two kernels.  The first selects: a cluster of CTAs per (sequence, kv head)
+// reads weights and positions once, keeps the keys in shared memory, finds the
+// budget-th largest by four passes of 8 bits over them (histograms added up
+// through the cluster's shared memory) and writes the lists of holes and movers
+// in slot order.  The second copies, a CTA for every 128 moves of a list; it is
+// bound by the rows it reads and writes.
+#include <algorithm>
+
 #include "paged_kv.cuh"
 
 namespace abra {
@@ -15,8 +24,8 @@ namespace {
 
 struct EvictArgs {
     PagedKv kv;
-    int32_t *new_lens, *moves;
-    int budget, n_sink, n_recent, cap;  // cap: entries of a move list
+    int32_t *new_lens, *counts, *moves;  // counts: moves of a row; moves: its holes, then its movers, cap each
+    int budget, n_sink, n_recent, cap, held;  // held: keys of a CTA that fit its shared memory
 };
 
 // Unsigned order of the weights: the float's bits with the sign folded, -0 as
@@ -28,96 +37,205 @@ __device__ __forceinline__ uint32_t rank_key(float a, int pos, int n_sink, int r
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int EV_THREADS = 256;
-
-__device__ __forceinline__ int block_sum(int v, int *buf) {
-    v = __reduce_add_sync(0xffffffffu, v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-    __syncthreads();
-    int t = 0;
-    for (int w = 0; w < EV_THREADS / 32; ++w) t += buf[w];
-    return t;
+__device__ __forceinline__ int cluster_rank() {
+    int r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
 }
-// Exclusive rank of this thread's flag in the block; *total gets the count.
-__device__ __forceinline__ int block_rank(bool f, int *buf, int *total) {
-    const unsigned b = __ballot_sync(0xffffffffu, f);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    __syncthreads();
-    if (lane == 0) buf[warp] = __popc(b);
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < EV_THREADS / 32; ++w) {
-        if (w < warp) before += buf[w];
-        all += buf[w];
-    }
-    *total = all;
-    return before + __popc(b & ((1u << lane) - 1u));
+__device__ __forceinline__ int cluster_size() {
+    int n;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+    return n;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The value that CTA `rank` of the cluster has at this address of its shared memory.
+__device__ __forceinline__ int peer_value(const int *p, int rank) {
+    uint32_t at;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
 }
 
-// One CTA per (kv head, sequence): the budget-th largest key bit by bit, then
-// one walk over the slots that lists holes and movers, then the copies.
-template <int D>
-__global__ void __launch_bounds__(EV_THREADS) evict_kernel(const __grid_constant__ EvictArgs p) {
-    __shared__ int buf[EV_THREADS / 32];
-    const int g = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+constexpr int SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32;
+constexpr int BINS = 256;
+constexpr int LANE_BINS_BYTES = BINS * 32 * 4;
+
+// One cluster per (kv head, sequence), an equal run of slots for each CTA.
+__global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_constant__ EvictArgs p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    int *bins = reinterpret_cast<int *>(smem);  // [BINS][32 lanes]: a lane's own column, so equal keys do not collide
+    uint32_t *held = reinterpret_cast<uint32_t *>(smem + LANE_BINS_BYTES);  // keys of the first p.held slots
+    __shared__ int s_hist[2][BINS], s_warp[SEL_WARPS], s_digit, s_left, s_tie[SEL_WARPS], s_hole[SEL_WARPS], s_mover[SEL_WARPS],
+        s_total[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = cluster_rank(), size = cluster_size();
+    const int g = blockIdx.y, s = blockIdx.z;
+    pdl_launch_dependents();
     const int len = paged_len(p.kv, s);
-    if (g == 0 && tid == 0) p.new_lens[s] = min(len, p.budget);
-    if (len <= p.budget) return;
+    const int64_t row = static_cast<int64_t>(s) * p.kv.a.n_kv_heads + g;
+    if (rank == 0 && tid == 0) {
+        if (g == 0) p.new_lens[s] = min(len, p.budget);
+        if (len <= p.budget) p.counts[row] = 0;
+    }
+    if (len <= p.budget) return;  // the whole cluster
     const int recent_from = paged_next_pos(p.kv, s, len) - p.n_recent;
-    auto meta = [&](int t) {
+    const int per = (len + size - 1) / size, first = min(len, rank * per), n = min(len, first + per) - first;
+    auto load_key = [&](int t) {
         const int e = p.kv.page.div(t);
-        return paged_meta_at(p.kv, max(0, paged_page(p.kv, s, e)), g, t - e * p.kv.a.page_size);
+        const int64_t m = paged_meta_at(p.kv, max(0, paged_page(p.kv, s, e)), g, t - e * p.kv.a.page_size);
+        return rank_key(__ldcg(p.kv.a.acc + m), __ldcg(p.kv.a.pos + m), p.n_sink, recent_from);
     };
-    auto key = [&](int t) {
-        const int64_t m = meta(t);
-        return rank_key(p.kv.a.acc[m], p.kv.a.pos[m], p.n_sink, recent_from);
-    };
+    auto key = [&](int i) { return i < p.held ? held[i] : load_key(first + i); };
+#pragma unroll 4
+    for (int i = tid; i < min(n, p.held); i += SEL_THREADS) held[i] = load_key(first + i);
+
+    // ---- the budget-th largest key, 8 bits at a time ----
     uint32_t cut = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = cut | (1u << bit);
-        int n = 0;
-        for (int t = tid; t < len; t += EV_THREADS) n += key(t) >= c;
-        if (block_sum(n, buf) >= p.budget) cut = c;
+    int left = p.budget;  // of the keys that share cut's leading bits, so many are kept
+#pragma unroll 1
+    for (int pass = 0; pass < 4; ++pass) {
+        const int shift = 24 - 8 * pass;
+        for (int i = tid; i < BINS * 32; i += SEL_THREADS) bins[i] = 0;
+        __syncthreads();
+#pragma unroll 4
+        for (int i = tid; i < n; i += SEL_THREADS) {
+            const uint32_t k = key(i);
+            if (pass == 0 || (k >> (shift + 8)) == (cut >> (shift + 8))) atomicAdd(&bins[((k >> shift) & 255) * 32 + lane], 1);
+        }
+        __syncthreads();
+        int *hist = s_hist[pass & 1];
+        if (tid < BINS) {
+            int sum = 0;
+#pragma unroll
+            for (int x = 0; x < 32; ++x) sum += bins[tid * 32 + ((x + tid) & 31)];
+            hist[tid] = sum;
+        }
+        cluster_sync();
+        // bin b of all CTAs, b = BINS - 1 - tid: an inclusive scan from the top
+        int all = 0, incl = 0;
+        if (tid < BINS) {
+            for (int r = 0; r < size; ++r) all += peer_value(hist + BINS - 1 - tid, r);
+            incl = all;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += y;
+            }
+            if (lane == 31) s_warp[warp] = incl;
+        }
+        __syncthreads();
+        if (tid < BINS) {
+            for (int x = 0; x < warp; ++x) incl += s_warp[x];
+            if (incl >= left && incl - all < left) s_digit = BINS - 1 - tid, s_left = left - (incl - all);
+        }
+        __syncthreads();
+        cut |= static_cast<uint32_t>(s_digit) << shift;
+        left = s_left;
     }
-    int above = 0;
-    for (int t = tid; t < len; t += EV_THREADS) above += key(t) > cut;
-    const int ties = p.budget - block_sum(above, buf);  // this many slots with the key `cut` stay
-    int32_t *hole = p.moves + (static_cast<int64_t>(s) * p.kv.a.n_kv_heads + g) * 2 * p.cap, *mover = hole + p.cap;
-    int n_tie = 0, n_hole = 0, n_mover = 0;
-    for (int t0 = 0; t0 < len; t0 += EV_THREADS) {
-        const int t = t0 + tid;
-        const uint32_t k = t < len ? key(t) : 0u;
-        int total;
-        const bool tie = t < len && k == cut;
-        const int r = n_tie + block_rank(tie, buf, &total);
-        n_tie += total;
-        const bool keep = t < len && (k > cut || (tie && r < ties));
-        const bool is_hole = t < p.budget && !keep, is_mover = t >= p.budget && keep;
-        const int rh = n_hole + block_rank(is_hole, buf, &total);
-        n_hole += total;
-        const int rm = n_mover + block_rank(is_mover, buf, &total);
-        n_mover += total;
-        if (is_hole) hole[rh] = t;
-        if (is_mover) mover[rm] = t;
-    }
+    // `left` of the slots whose key is cut stay: the lowest.  The last pass
+    // counted them in each CTA.
+    int ties = 0;
+    for (int r = 0; r < rank; ++r) ties += peer_value(&s_hist[1][cut & 255], r);
+
+    // ---- holes and movers in slot order: a run of slots for each warp ----
+    const int run = ((n + SEL_WARPS - 1) / SEL_WARPS + 31) & ~31, w0 = min(n, warp * run), w1 = min(n, w0 + run);
+    int own = 0;
+    for (int i = w0; i < w1; i += 32) own += __popc(__ballot_sync(0xffffffffu, i + lane < w1 && key(i + lane) == cut));
+    if (lane == 0) s_tie[warp] = own;
     __syncthreads();
-    for (int i = tid >> 5; i < n_hole; i += EV_THREADS / 32) {
-        const int lane = tid & 31, from = mover[i], to = hole[i];
+    for (int x = 0; x < warp; ++x) ties += s_tie[x];
+    // one step of 32 slots: which are holes, which movers
+    const unsigned below = (1u << lane) - 1u;
+    auto classify = [&](int i, int &tie, unsigned &holes, unsigned &movers) {
+        const bool in = i + lane < w1;
+        const uint32_t k = in ? key(i + lane) : 0u;
+        const unsigned t = __ballot_sync(0xffffffffu, in && k == cut);
+        const bool keep = in && (k > cut || (k == cut && tie + __popc(t & below) < left));
+        tie += __popc(t);
+        const bool low = first + i + lane < p.budget;
+        holes = __ballot_sync(0xffffffffu, in && low && !keep);
+        movers = __ballot_sync(0xffffffffu, !low && keep);
+    };
+    int nh = 0, nm = 0, tie = ties;
+    for (int i = w0; i < w1; i += 32) {
+        unsigned h, m;
+        classify(i, tie, h, m);
+        nh += __popc(h), nm += __popc(m);
+    }
+    if (lane == 0) s_hole[warp] = nh, s_mover[warp] = nm;
+    __syncthreads();
+    if (tid < 2) {
+        int sum = 0;
+        for (int x = 0; x < SEL_WARPS; ++x) sum += tid ? s_mover[x] : s_hole[x];
+        s_total[tid] = sum;
+    }
+    cluster_sync();
+    int hole_at = 0, mover_at = 0;
+    for (int r = 0; r < rank; ++r) hole_at += peer_value(&s_total[0], r), mover_at += peer_value(&s_total[1], r);
+    if (rank == size - 1 && tid == 0) p.counts[row] = hole_at + s_total[0];
+    for (int x = 0; x < warp; ++x) hole_at += s_hole[x], mover_at += s_mover[x];
+    int32_t *hole = p.moves + row * 2 * p.cap, *mover = hole + p.cap;
+    tie = ties;
+    for (int i = w0; i < w1; i += 32) {
+        unsigned h, m;
+        classify(i, tie, h, m);
+        if (h >> lane & 1) hole[hole_at + __popc(h & below)] = first + i + lane;
+        if (m >> lane & 1) mover[mover_at + __popc(m & below)] = first + i + lane;
+        hole_at += __popc(h), mover_at += __popc(m);
+    }
+    cluster_sync();  // nobody leaves while its shared memory is read
+}
+
+constexpr int MOVE_THREADS = 256, MOVES = 128;
+
+// MOVES moves of one list: the addresses first, then 16-byte copies, several in
+// flight a thread.
+template <int D>
+__global__ void __launch_bounds__(MOVE_THREADS) move_kernel(const __grid_constant__ EvictArgs p) {
+    constexpr int CH = D / 8;  // 16-byte chunks of a row
+    constexpr int BATCH = 8;
+    __shared__ int64_t s_from[2][MOVES], s_to[2][MOVES];  // K, V
+    __shared__ bool s_ok[MOVES];
+    const int g = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
+    const int64_t row = static_cast<int64_t>(s) * p.kv.a.n_kv_heads + g;
+    pdl_wait();
+    const int first = blockIdx.x * MOVES, n = min(MOVES, __ldcg(p.counts + row) - first);
+    if (n <= 0) return;
+    const int32_t *hole = p.moves + row * 2 * p.cap + first, *mover = hole + p.cap;
+    if (tid < n) {
+        const int from = __ldcg(mover + tid), to = __ldcg(hole + tid);
         const int ef = p.kv.page.div(from), et = p.kv.page.div(to);
         const int pf = paged_page(p.kv, s, ef), pt = paged_page(p.kv, s, et);
-        if (pf < 0 || pt < 0) continue;
         const int of = from - ef * p.kv.a.page_size, ot = to - et * p.kv.a.page_size;
-        uint16_t *kp = static_cast<uint16_t *>(p.kv.a.k), *vp = static_cast<uint16_t *>(p.kv.a.v);
-        for (int d = lane; d < D; d += 32) {
-            kp[paged_k_at(p.kv, pt, g, ot) + d] = kp[paged_k_at(p.kv, pf, g, of) + d];
-            vp[paged_v_at(p.kv, pt, g, ot) + d] = vp[paged_v_at(p.kv, pf, g, of) + d];
-        }
-        if (lane == 0) {
+        s_ok[tid] = pf >= 0 && pt >= 0;
+        if (s_ok[tid]) {
+            s_from[0][tid] = paged_k_at(p.kv, pf, g, of), s_to[0][tid] = paged_k_at(p.kv, pt, g, ot);
+            s_from[1][tid] = paged_v_at(p.kv, pf, g, of), s_to[1][tid] = paged_v_at(p.kv, pt, g, ot);
             const int64_t a = paged_meta_at(p.kv, pt, g, ot), b = paged_meta_at(p.kv, pf, g, of);
             p.kv.a.acc[a] = p.kv.a.acc[b];
             p.kv.a.pos[a] = p.kv.a.pos[b];
         }
+    }
+    __syncthreads();
+    uint16_t *const pool[2] = {static_cast<uint16_t *>(p.kv.a.k), static_cast<uint16_t *>(p.kv.a.v)};
+    for (int x0 = tid; x0 < n * 2 * CH; x0 += BATCH * MOVE_THREADS) {
+        uint4 v[BATCH];
+        uint16_t *to[BATCH];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            const int x = x0 + b * MOVE_THREADS, m = x / (2 * CH), kv = (x / CH) & 1, chunk = x % CH;
+            to[b] = nullptr;
+            if (x < n * 2 * CH && s_ok[m]) {
+                v[b] = __ldcg(reinterpret_cast<const uint4 *>(pool[kv] + s_from[kv][m] + 8 * chunk));
+                to[b] = pool[kv] + s_to[kv][m] + 8 * chunk;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+            if (to[b]) __stcg(reinterpret_cast<uint4 *>(to[b]), v[b]);
     }
 }
 
@@ -132,8 +250,62 @@ int64_t move_cap(const abra_paged_kv *kv, int32_t budget) {
     const int64_t slots = static_cast<int64_t>(kv->max_pages) * kv->page_size;
     return slots <= budget ? 0 : slots - budget < budget ? slots - budget : budget;
 }
+int64_t rows_of(const abra_paged_kv *kv) { return static_cast<int64_t>(kv->n_seqs) * kv->n_kv_heads; }
+int64_t counts_bytes(const abra_paged_kv *kv) { return (rows_of(kv) * 4 + 15) / 16 * 16 + 16; }
 int64_t workspace_bytes_of(const abra_paged_kv *kv, int32_t budget) {
-    return 16 + static_cast<int64_t>(kv->n_seqs) * kv->n_kv_heads * 2 * move_cap(kv, budget) * 4;
+    return counts_bytes(kv) + rows_of(kv) * 2 * move_cap(kv, budget) * 4;
+}
+
+constexpr int HELD_MOST = 40960;  // keys in a CTA's shared memory
+
+// CTAs of a cluster: doubled while all clusters stay resident together and
+// every CTA keeps a few thousand slots' worth of work.
+int cluster_of(const abra_paged_kv *kv, int sms) {
+    const int64_t slots = static_cast<int64_t>(kv->max_pages) * kv->page_size;
+    int c = 1;
+    while (c < 8 && ((rows_of(kv) * c * 2 <= 4 * sms && slots / c > 2 * SEL_THREADS) || slots / c > HELD_MOST)) c *= 2;
+    return c;
+}
+
+cudaError_t launch_kernel(const void *k, dim3 grid, int threads, int smem, int cluster, cudaStream_t st, EvictArgs &p) {
+    cudaLaunchAttribute at{};
+    if (cluster) {
+        at.id = cudaLaunchAttributeClusterDimension;
+        at.val.clusterDim.x = cluster;
+        at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    } else {  // may begin before the kernel in front of it has ended; its pdl_wait waits for that
+        at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at.val.programmaticStreamSerializationAllowed = 1;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    void *args[] = {&p};
+    return cudaLaunchKernelExC(&cfg, k, args);
+}
+
+cudaError_t launch(EvictArgs &p, cudaStream_t st) {
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    const int64_t slots = static_cast<int64_t>(p.kv.a.max_pages) * p.kv.a.page_size;
+    const int cluster = cluster_of(&p.kv.a, sms);
+    p.held = static_cast<int>(std::min<int64_t>((slots + cluster - 1) / cluster, HELD_MOST));
+    const int smem = LANE_BINS_BYTES + p.held * 4;
+    e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const unsigned heads = p.kv.a.n_kv_heads, seqs = p.kv.a.n_seqs;
+    e = launch_kernel(reinterpret_cast<const void *>(select_kernel), dim3(cluster, heads, seqs), SEL_THREADS, smem, cluster, st, p);
+    if (e != cudaSuccess || p.cap == 0) return e;
+    const void *k = p.kv.a.head_dim == 64   ? reinterpret_cast<const void *>(move_kernel<64>)
+                    : p.kv.a.head_dim == 96 ? reinterpret_cast<const void *>(move_kernel<96>)
+                                            : reinterpret_cast<const void *>(move_kernel<128>);
+    return launch_kernel(k, dim3((p.cap + MOVES - 1) / MOVES, heads, seqs), MOVE_THREADS, 0, 0, st, p);
 }
 
 }  // namespace
@@ -164,14 +336,8 @@ extern "C" int abra_paged_evict(const abra_paged_kv *kv, int32_t budget, int32_t
         return paged_fail(ABRA_E_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                           (long long)workspace_bytes_of(kv, budget));
     if (kv->n_seqs == 0) return ABRA_OK;
-    EvictArgs p{paged_view(kv), new_lens, static_cast<int32_t *>(workspace), budget, n_sink, n_recent,
-                static_cast<int>(move_cap(kv, budget))};
-    const dim3 grid(kv->n_kv_heads, kv->n_seqs);
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    switch (kv->head_dim) {
-        case 64: evict_kernel<64><<<grid, EV_THREADS, 0, st>>>(p); break;
-        case 96: evict_kernel<96><<<grid, EV_THREADS, 0, st>>>(p); break;
-        default: evict_kernel<128><<<grid, EV_THREADS, 0, st>>>(p); break;
-    }
-    return paged_cuda(cudaGetLastError(), "paged evict launch");
+    char *ws = static_cast<char *>(workspace);
+    EvictArgs p{paged_view(kv), new_lens, reinterpret_cast<int32_t *>(ws), reinterpret_cast<int32_t *>(ws + counts_bytes(kv)),
+                budget, n_sink, n_recent, static_cast<int>(move_cap(kv, budget)), 0};
+    return paged_cuda(launch(p, static_cast<cudaStream_t>(stream)), "paged evict launch");
 }
