@@ -22,41 +22,63 @@ struct AppendArgs {
     int n_heads, n_tokens, rope_len;
 };
 
-// Sequence of token t: the last s with cu_new[s] <= t.
-__device__ __forceinline__ int sequence_of(const int32_t *cu, int n_seqs, int t) {
-    int lo = 0, hi = n_seqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(cu + mid) <= t) lo = mid; else hi = mid;
-    }
-    return lo;
+// Four neighbouring values.
+__device__ __forceinline__ float4 load4(const float *p) { return __ldcs(reinterpret_cast<const float4 *>(p)); }
+template <typename T> __device__ __forceinline__ float4 load4(const T *p) {
+    const uint2 x = __ldcs(reinterpret_cast<const uint2 *>(p));
+    const T *h = reinterpret_cast<const T *>(&x);
+    return make_float4(Half16<T>::up(h[0]), Half16<T>::up(h[1]), Half16<T>::up(h[2]), Half16<T>::up(h[3]));
 }
+template <typename T> __device__ __forceinline__ void store4(T *p, float4 x) {
+    const T h[4] = {Half16<T>::down(x.x), Half16<T>::down(x.y), Half16<T>::down(x.z), Half16<T>::down(x.w)};
+    *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(h);
+}
+__device__ __forceinline__ float4 ldg4(const float *p) { return __ldg(reinterpret_cast<const float4 *>(p)); }
+__device__ __forceinline__ float4 mul4(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
 
-__device__ __forceinline__ float up(float x) { return x; }
-__device__ __forceinline__ float up(__half x) { return __half2float(x); }
-__device__ __forceinline__ float up(__nv_bfloat16 x) { return __bfloat162float(x); }
+constexpr int APPEND_THREADS = 256;
 
-constexpr int APPEND_WARPS = 8;
-
-// One warp per (token, head).  Lane l holds the pairs (i, i + D/2) for i = l,
-// l + 32.
+// One CTA per token.  A group of 16 lanes (8 for heads of 64) takes a head: lane
+// j holds the pairs (4 j + u, 4 j + u + D/2), u = 0..3.  The first heads' values
+// are asked for before the token's sequence, slot and page are looked up, so
+// that the chain of small reads (offsets, length, table) runs under the large
+// ones.
 template <typename TI, typename T, int D>
-__global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(const __grid_constant__ AppendArgs p) {
-    constexpr int HALF = D / 2, NP = (HALF + 31) / 32;
-    const int lane = threadIdx.x & 31;
-    const int heads = (p.q ? p.n_heads : 0) + 2 * p.kv.a.n_kv_heads;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * APPEND_WARPS + (threadIdx.x >> 5);
-    if (item >= static_cast<int64_t>(p.n_tokens) * heads) return;
-    const int t = static_cast<int>(item / heads);
-    int h = static_cast<int>(item - static_cast<int64_t>(t) * heads);
-    int kind = 0;  // 0 query, 1 key, 2 value
-    if (!p.q) kind = 1;
-    else if (h >= p.n_heads) { kind = 1; h -= p.n_heads; }
-    if (kind && h >= p.kv.a.n_kv_heads) { kind = 2; h -= p.kv.a.n_kv_heads; }
-    // the token's sequence, slot and position
-    int s, end;
+__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_constant__ AppendArgs p) {
+    constexpr int HALF = D / 2, LANES = D == 64 ? 8 : 16, GROUPS = APPEND_THREADS / LANES, BATCH = 4;
+    const int t = blockIdx.x, group = threadIdx.x / LANES, j = threadIdx.x % LANES;
+    const unsigned lanes = ((1u << LANES) - 1u) << (threadIdx.x % 32 / LANES * LANES);  // the group's
+    const bool on = 4 * j < HALF;  // heads of 96 use 12 lanes of a group
+    const int nq = p.q ? p.n_heads : 0, nkv = p.kv.a.n_kv_heads, heads = nq + 2 * nkv;
+    float4 lo[BATCH], hi[BATCH];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            const int h = base + b * GROUPS;
+            if (h >= heads || !on) {
+                lo[b] = hi[b] = make_float4(0, 0, 0, 0);
+                continue;
+            }
+            const TI *src = h < nq         ? static_cast<const TI *>(p.q) + t * p.ldq + static_cast<int64_t>(h) * D
+                            : h < nq + nkv ? static_cast<const TI *>(p.k) + t * p.ldk + static_cast<int64_t>(h - nq) * D
+                                           : static_cast<const TI *>(p.v) + t * p.ldv + static_cast<int64_t>(h - nq - nkv) * D;
+            lo[b] = load4(src + 4 * j);
+            hi[b] = load4(src + 4 * j + HALF);
+        }
+    };
+    int base = group;
+    load(base);
+    // the token's sequence (how many end at or before it), slot, position and page
+    int s = 0, end;
     if (p.cu_new) {
-        s = sequence_of(p.cu_new, p.kv.a.n_seqs, t);
+        for (int x = 0; x < p.kv.a.n_seqs; x += APPEND_THREADS) {
+            const int y = x + threadIdx.x;
+            s += __syncthreads_count(y < p.kv.a.n_seqs && __ldg(p.cu_new + y + 1) <= t);
+        }
+        if (s >= p.kv.a.n_seqs) {  // beyond the last sequence's tokens
+            if (threadIdx.x == 0) report_error(ERR_BAD_INDEX);
+            return;
+        }
         end = __ldg(p.cu_new + s + 1);
     } else {
         const int m = p.n_tokens / p.kv.a.n_seqs;
@@ -65,88 +87,79 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) append_kernel(const __grid_
     }
     const int len = paged_len(p.kv, s);
     const int slot = len - (end - t), at = paged_next_pos(p.kv, s, len) - (end - t);
-
-    const TI *src = static_cast<const TI *>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) +
-                    t * (kind == 0 ? p.ldq : kind == 1 ? p.ldk : p.ldv) + static_cast<int64_t>(h) * D;
-    float lo[NP], hi[NP];
-#pragma unroll
-    for (int u = 0; u < NP; ++u) {
-        const int i = lane + 32 * u;
-        lo[u] = i < HALF ? up(src[i]) : 0.0f;
-        hi[u] = i < HALF ? up(src[i + HALF]) : 0.0f;
+    int page = -1, off = 0;
+    if (slot >= 0) {
+        const int e = p.kv.page.div(slot);
+        off = slot - e * p.kv.a.page_size;
+        page = paged_page(p.kv, s, e);
+    } else if (threadIdx.x == 0) {  // more new tokens than the sequence has slots
+        report_error(ERR_BAD_INDEX);
     }
-    const float *nw = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
-    if (nw) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int u = 0; u < NP; ++u) ss += lo[u] * lo[u] + hi[u] * hi[u];
-#pragma unroll
-        for (int m = 16; m >= 1; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-        const float r = rsqrtf(ss * (1.0f / D) + p.eps);
-#pragma unroll
-        for (int u = 0; u < NP; ++u) {
-            const int i = lane + 32 * u;
-            if (i < HALF) {
-                lo[u] *= r * __ldg(nw + i);
-                hi[u] *= r * __ldg(nw + i + HALF);
-            }
-        }
-    }
-    if (p.rope && kind < 2) {
+    // cos and sin of the lane's four pairs
+    float4 c01 = make_float4(1, 0, 1, 0), c23 = c01;
+    if (p.rope && on) {
         if (at >= 0 && at < p.rope_len) {
-            const float2 *row = reinterpret_cast<const float2 *>(p.rope) + static_cast<int64_t>(at) * HALF;
-#pragma unroll
-            for (int u = 0; u < NP; ++u) {
-                const int i = lane + 32 * u;
-                if (i < HALF) {
-                    const float2 cs = __ldg(row + i);
-                    const float a = lo[u], b = hi[u];
-                    lo[u] = a * cs.x - b * cs.y;
-                    hi[u] = b * cs.x + a * cs.y;
-                }
-            }
-        } else if (lane == 0) {
+            const float *row = p.rope + static_cast<int64_t>(at) * D + 8 * j;
+            c01 = ldg4(row), c23 = ldg4(row + 4);
+        } else if (threadIdx.x == 0) {
             report_error(ERR_BAD_INDEX);
         }
     }
-    T *dst;
-    if (kind == 0) {
-        dst = static_cast<T *>(p.q_out) + t * p.ldqo + static_cast<int64_t>(h) * D;
-    } else {
-        if (slot < 0) {  // more new tokens than the sequence has slots
-            if (lane == 0) report_error(ERR_BAD_INDEX);
-            return;
-        }
-        const int e = p.kv.page.div(slot), off = slot - e * p.kv.a.page_size;
-        const int page = paged_page(p.kv, s, e);
-        if (page < 0) return;
-        dst = kind == 1 ? static_cast<T *>(p.kv.a.k) + paged_k_at(p.kv, page, h, off)
-                        : static_cast<T *>(p.kv.a.v) + paged_v_at(p.kv, page, h, off);
-        if (kind == 1 && lane == 0) {
-            const int64_t m = paged_meta_at(p.kv, page, h, off);
-            if (p.kv.a.acc) p.kv.a.acc[m] = 0.0f;
-            if (p.kv.a.pos) p.kv.a.pos[m] = at;
-        }
-    }
+    for (;;) {
 #pragma unroll
-    for (int u = 0; u < NP; ++u) {
-        const int i = lane + 32 * u;
-        if (i < HALF) {
-            dst[i] = Half16<T>::down(lo[u]);
-            dst[i + HALF] = Half16<T>::down(hi[u]);
+        for (int b = 0; b < BATCH; ++b) {
+            const int h = base + b * GROUPS;
+            if (h >= heads) break;  // the whole group
+            float4 x = lo[b], y = hi[b];
+            const float *nw = h < nq ? p.q_norm : h < nq + nkv ? p.k_norm : nullptr;
+            float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + (y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w);
+#pragma unroll
+            for (int m = LANES / 2; m >= 1; m >>= 1) ss += __shfl_xor_sync(lanes, ss, m);
+            if (nw && on) {
+                const float r = rsqrtf(ss * (1.0f / D) + p.eps);
+                x = mul4(mul4(x, make_float4(r, r, r, r)), ldg4(nw + 4 * j));
+                y = mul4(mul4(y, make_float4(r, r, r, r)), ldg4(nw + 4 * j + HALF));
+            }
+            if (h < nq + nkv) {
+                const float4 u = x;
+                x = make_float4(u.x * c01.x - y.x * c01.y, u.y * c01.z - y.y * c01.w, u.z * c23.x - y.z * c23.y,
+                                u.w * c23.z - y.w * c23.w);
+                y = make_float4(y.x * c01.x + u.x * c01.y, y.y * c01.z + u.y * c01.w, y.z * c23.x + u.z * c23.y,
+                                y.w * c23.z + u.w * c23.w);
+            }
+            T *dst = nullptr;
+            if (h < nq) {
+                dst = static_cast<T *>(p.q_out) + t * p.ldqo + static_cast<int64_t>(h) * D;
+            } else if (page >= 0) {
+                if (h < nq + nkv) {
+                    dst = static_cast<T *>(p.kv.a.k) + paged_k_at(p.kv, page, h - nq, off);
+                    if (j == 0) {
+                        const int64_t m = paged_meta_at(p.kv, page, h - nq, off);
+                        if (p.kv.a.acc) p.kv.a.acc[m] = 0.0f;
+                        if (p.kv.a.pos) p.kv.a.pos[m] = at;
+                    }
+                } else {
+                    dst = static_cast<T *>(p.kv.a.v) + paged_v_at(p.kv, page, h - nq - nkv, off);
+                }
+            }
+            if (dst && on) {
+                store4(dst + 4 * j, x);
+                store4(dst + 4 * j + HALF, y);
+            }
         }
+        base += BATCH * GROUPS;
+        if (base >= heads) return;
+        load(base);
     }
 }
 
 template <typename TI, typename T>
 cudaError_t launch(const AppendArgs &p, cudaStream_t stream) {
-    const int64_t heads = (p.q ? p.n_heads : 0) + 2 * p.kv.a.n_kv_heads;
-    const int64_t items = p.n_tokens * heads;
-    const dim3 grid(static_cast<unsigned>((items + APPEND_WARPS - 1) / APPEND_WARPS));
+    const dim3 grid(p.n_tokens);
     switch (p.kv.a.head_dim) {
-        case 64: append_kernel<TI, T, 64><<<grid, APPEND_WARPS * 32, 0, stream>>>(p); break;
-        case 96: append_kernel<TI, T, 96><<<grid, APPEND_WARPS * 32, 0, stream>>>(p); break;
-        default: append_kernel<TI, T, 128><<<grid, APPEND_WARPS * 32, 0, stream>>>(p); break;
+        case 64: append_kernel<TI, T, 64><<<grid, APPEND_THREADS, 0, stream>>>(p); break;
+        case 96: append_kernel<TI, T, 96><<<grid, APPEND_THREADS, 0, stream>>>(p); break;
+        default: append_kernel<TI, T, 128><<<grid, APPEND_THREADS, 0, stream>>>(p); break;
     }
     return cudaGetLastError();
 }

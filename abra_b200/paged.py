@@ -59,9 +59,12 @@ def _need(ok: bool, what: str) -> None:
 def _rows(t, name: str, width: int, device) -> tuple[int, int]:
     """(rows, row stride) of a tensor [..., heads, head_dim] or [..., width]
     whose rows of ``width`` elements are contiguous and evenly spaced."""
-    _need(t.device == device, f"{name} must be on the cache's device")
+    if t.device != device:
+        raise ValueError(f"{name} must be on the cache's device")
     shape, stride = t.shape, t.stride()
-    n, inner, i = 1, 1, t.dim()
+    if len(shape) == 2 and shape[1] == width and stride[1] == 1:
+        return shape[0], stride[0] if shape[0] > 1 else width
+    n, inner, i = 1, 1, len(shape)
     while i > 0 and inner < width:  # the trailing dimensions that make one row
         i -= 1
         _need(shape[i] == 1 or stride[i] == inner, f"the rows of {name} must be contiguous")
