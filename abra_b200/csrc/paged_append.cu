@@ -20,6 +20,8 @@ struct AppendArgs {
     void *q_out;
     float eps;
     int n_heads, n_tokens, rope_len;
+    int tokens;     // of a CTA
+    FastDiv heads;  // heads of a token, queries, keys and values
 };
 
 // Four neighbouring values.
@@ -37,28 +39,32 @@ __device__ __forceinline__ float4 ldg4(const float *p) { return __ldg(reinterpre
 __device__ __forceinline__ float4 mul4(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
 
 constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_TOKENS = 4;  // of a CTA, where there are many
 
-// One CTA per token.  A group of 16 lanes (8 for heads of 64) takes a head: lane
-// j holds the pairs (4 j + u, 4 j + u + D/2), u = 0..3.  The first heads' values
-// are asked for before the token's sequence, slot and page are looked up, so
-// that the chain of small reads (offsets, length, table) runs under the large
-// ones.
+// A CTA takes a few neighbouring tokens, a group of 16 lanes (8 for heads of
+// 64) a head: lane j holds the pairs (4 j + u, 4 j + u + D/2), u = 0..3.  The
+// first heads' values are asked for before the tokens' sequences, slots and
+// pages are looked up, so that the chain of small reads (offsets, length,
+// table) runs under the large ones, and several tokens share it.
 template <typename TI, typename T, int D>
-__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_constant__ AppendArgs p) {
-    constexpr int HALF = D / 2, LANES = D == 64 ? 8 : 16, GROUPS = APPEND_THREADS / LANES, BATCH = 4;
-    const int t = blockIdx.x, group = threadIdx.x / LANES, j = threadIdx.x % LANES;
+__global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_constant__ AppendArgs p) {
+    constexpr int HALF = D / 2, LANES = D == 64 ? 8 : 16, GROUPS = APPEND_THREADS / LANES, BATCH = 3;
+    __shared__ int s_page[APPEND_TOKENS], s_off[APPEND_TOKENS], s_at[APPEND_TOKENS];
+    const int group = threadIdx.x / LANES, j = threadIdx.x % LANES;
     const unsigned lanes = ((1u << LANES) - 1u) << (threadIdx.x % 32 / LANES * LANES);  // the group's
     const bool on = 4 * j < HALF;  // heads of 96 use 12 lanes of a group
     const int nq = p.q ? p.n_heads : 0, nkv = p.kv.a.n_kv_heads, heads = nq + 2 * nkv;
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens;
+    const int nt = static_cast<int>(min(static_cast<int64_t>(p.tokens), p.n_tokens - t0)), items = nt * heads;
     float4 lo[BATCH], hi[BATCH];
     auto load = [&](int base) {
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
-            const int h = base + b * GROUPS;
-            if (h >= heads || !on) {
-                lo[b] = hi[b] = make_float4(0, 0, 0, 0);
-                continue;
-            }
+            const int x = base + b * GROUPS;
+            lo[b] = hi[b] = make_float4(0, 0, 0, 0);
+            if (x >= items || !on) continue;
+            const int i = p.heads.div(x), h = x - i * heads;
+            const int64_t t = t0 + i;
             const TI *src = h < nq         ? static_cast<const TI *>(p.q) + t * p.ldq + static_cast<int64_t>(h) * D
                             : h < nq + nkv ? static_cast<const TI *>(p.k) + t * p.ldk + static_cast<int64_t>(h - nq) * D
                                            : static_cast<const TI *>(p.v) + t * p.ldv + static_cast<int64_t>(h - nq - nkv) * D;
@@ -68,60 +74,61 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_con
     };
     int base = group;
     load(base);
-    // the token's sequence (how many end at or before it), slot, position and page
-    int s = 0, end;
+    // the first token's sequence: how many end at or before it
+    int s = 0;
     if (p.cu_new) {
         for (int x = 0; x < p.kv.a.n_seqs; x += APPEND_THREADS) {
             const int y = x + threadIdx.x;
-            s += __syncthreads_count(y < p.kv.a.n_seqs && __ldg(p.cu_new + y + 1) <= t);
+            s += __syncthreads_count(y < p.kv.a.n_seqs && __ldg(p.cu_new + y + 1) <= t0);
         }
-        if (s >= p.kv.a.n_seqs) {  // beyond the last sequence's tokens
-            if (threadIdx.x == 0) report_error(ERR_BAD_INDEX);
-            return;
+    }
+    if (threadIdx.x < nt) {  // each token's slot, position and page
+        const int t = static_cast<int>(t0) + threadIdx.x;
+        int end, page = -1, off = 0, at = -1;
+        if (p.cu_new) {
+            while (s < p.kv.a.n_seqs && __ldg(p.cu_new + s + 1) <= t) ++s;
+            end = s < p.kv.a.n_seqs ? __ldg(p.cu_new + s + 1) : 0;
+        } else {
+            const int m = p.n_tokens / p.kv.a.n_seqs;
+            s = t / m;
+            end = (s + 1) * m;
         }
-        end = __ldg(p.cu_new + s + 1);
-    } else {
-        const int m = p.n_tokens / p.kv.a.n_seqs;
-        s = t / m;
-        end = (s + 1) * m;
-    }
-    const int len = paged_len(p.kv, s);
-    const int slot = len - (end - t), at = paged_next_pos(p.kv, s, len) - (end - t);
-    int page = -1, off = 0;
-    if (slot >= 0) {
-        const int e = p.kv.page.div(slot);
-        off = slot - e * p.kv.a.page_size;
-        page = paged_page(p.kv, s, e);
-    } else if (threadIdx.x == 0) {  // more new tokens than the sequence has slots
-        report_error(ERR_BAD_INDEX);
-    }
-    // cos and sin of the lane's four pairs
-    float4 c01 = make_float4(1, 0, 1, 0), c23 = c01;
-    if (p.rope && on) {
-        if (at >= 0 && at < p.rope_len) {
-            const float *row = p.rope + static_cast<int64_t>(at) * D + 8 * j;
-            c01 = ldg4(row), c23 = ldg4(row + 4);
-        } else if (threadIdx.x == 0) {
+        if (s < p.kv.a.n_seqs) {
+            const int len = paged_len(p.kv, s), slot = len - (end - t);
+            at = paged_next_pos(p.kv, s, len) - (end - t);
+            if (slot >= 0) {
+                const int e = p.kv.page.div(slot);
+                off = slot - e * p.kv.a.page_size;
+                page = paged_page(p.kv, s, e);
+            }
+            if (slot < 0 || (p.rope && (at < 0 || at >= p.rope_len))) report_error(ERR_BAD_INDEX);
+        } else {  // beyond the last sequence's tokens
             report_error(ERR_BAD_INDEX);
         }
+        s_page[threadIdx.x] = page, s_off[threadIdx.x] = off, s_at[threadIdx.x] = at;
     }
+    __syncthreads();
     for (;;) {
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
-            const int h = base + b * GROUPS;
-            if (h >= heads) break;  // the whole group
+            const int item = base + b * GROUPS;
+            if (item >= items) break;  // the whole group
+            const int i = p.heads.div(item), h = item - i * heads, page = s_page[i], at = s_at[i];
             float4 x = lo[b], y = hi[b];
             const float *nw = h < nq ? p.q_norm : h < nq + nkv ? p.k_norm : nullptr;
-            float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + (y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w);
+            if (nw) {
+                float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + (y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w);
 #pragma unroll
-            for (int m = LANES / 2; m >= 1; m >>= 1) ss += __shfl_xor_sync(lanes, ss, m);
-            if (nw && on) {
+                for (int m = LANES / 2; m >= 1; m >>= 1) ss += __shfl_xor_sync(lanes, ss, m);
                 const float r = rsqrtf(ss * (1.0f / D) + p.eps);
-                x = mul4(mul4(x, make_float4(r, r, r, r)), ldg4(nw + 4 * j));
-                y = mul4(mul4(y, make_float4(r, r, r, r)), ldg4(nw + 4 * j + HALF));
+                if (on) {
+                    x = mul4(mul4(x, make_float4(r, r, r, r)), ldg4(nw + 4 * j));
+                    y = mul4(mul4(y, make_float4(r, r, r, r)), ldg4(nw + 4 * j + HALF));
+                }
             }
-            if (h < nq + nkv) {
-                const float4 u = x;
+            if (p.rope && h < nq + nkv && on && at >= 0 && at < p.rope_len) {
+                const float *row = p.rope + static_cast<int64_t>(at) * D + 8 * j;
+                const float4 c01 = ldg4(row), c23 = ldg4(row + 4), u = x;  // cos, sin of two pairs each
                 x = make_float4(u.x * c01.x - y.x * c01.y, u.y * c01.z - y.y * c01.w, u.z * c23.x - y.z * c23.y,
                                 u.w * c23.z - y.w * c23.w);
                 y = make_float4(y.x * c01.x + u.x * c01.y, y.y * c01.z + u.y * c01.w, y.z * c23.x + u.z * c23.y,
@@ -129,17 +136,17 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_con
             }
             T *dst = nullptr;
             if (h < nq) {
-                dst = static_cast<T *>(p.q_out) + t * p.ldqo + static_cast<int64_t>(h) * D;
+                dst = static_cast<T *>(p.q_out) + (t0 + i) * p.ldqo + static_cast<int64_t>(h) * D;
             } else if (page >= 0) {
                 if (h < nq + nkv) {
-                    dst = static_cast<T *>(p.kv.a.k) + paged_k_at(p.kv, page, h - nq, off);
+                    dst = static_cast<T *>(p.kv.a.k) + paged_k_at(p.kv, page, h - nq, s_off[i]);
                     if (j == 0) {
-                        const int64_t m = paged_meta_at(p.kv, page, h - nq, off);
+                        const int64_t m = paged_meta_at(p.kv, page, h - nq, s_off[i]);
                         if (p.kv.a.acc) p.kv.a.acc[m] = 0.0f;
                         if (p.kv.a.pos) p.kv.a.pos[m] = at;
                     }
                 } else {
-                    dst = static_cast<T *>(p.kv.a.v) + paged_v_at(p.kv, page, h - nq - nkv, off);
+                    dst = static_cast<T *>(p.kv.a.v) + paged_v_at(p.kv, page, h - nq - nkv, s_off[i]);
                 }
             }
             if (dst && on) {
@@ -148,14 +155,14 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_con
             }
         }
         base += BATCH * GROUPS;
-        if (base >= heads) return;
+        if (base >= items) return;
         load(base);
     }
 }
 
 template <typename TI, typename T>
 cudaError_t launch(const AppendArgs &p, cudaStream_t stream) {
-    const dim3 grid(p.n_tokens);
+    const dim3 grid((p.n_tokens + p.tokens - 1) / p.tokens);
     switch (p.kv.a.head_dim) {
         case 64: append_kernel<TI, T, 64><<<grid, APPEND_THREADS, 0, stream>>>(p); break;
         case 96: append_kernel<TI, T, 96><<<grid, APPEND_THREADS, 0, stream>>>(p); break;
@@ -189,7 +196,6 @@ extern "C" int abra_paged_append(const abra_paged_kv *kv, const void *q, const v
     if (!k || !v || (q != nullptr) != (q_out != nullptr))
         return paged_fail(ABRA_E_INVALID, "null k or v, or only one of q and q_out");
     if (q && n_heads < 1) return paged_fail(ABRA_E_INVALID, "n_heads must be positive");
-    if (n_heads > 65535) return paged_fail(ABRA_E_UNSUPPORTED, "over 65535 heads");
     const int64_t kvw = static_cast<int64_t>(kv->n_kv_heads) * kv->head_dim;
     const int64_t qw = static_cast<int64_t>(n_heads) * kv->head_dim;
     if (ldk < kvw || ldv < kvw || (q && (ldq < qw || ldqo < qw)))
@@ -201,8 +207,10 @@ extern "C" int abra_paged_append(const abra_paged_kv *kv, const void *q, const v
         return paged_fail(ABRA_E_INVALID, "norm weights and rope must be 16-byte aligned");
     if (rope && rope_len < 1) return paged_fail(ABRA_E_INVALID, "rope_len must be positive");
     const int64_t heads = (q ? n_heads : 0) + 2ll * kv->n_kv_heads;
-    if (n_tokens * heads > (1ll << 33)) return paged_fail(ABRA_E_UNSUPPORTED, "n_tokens * heads over 2^33");
-    AppendArgs p{paged_view(kv), q, k, v, ldq, ldk, ldv, ldqo, cu_new, q_norm, k_norm, rope, q_out, eps, n_heads, n_tokens, rope_len};
+    if (heads > 65535) return paged_fail(ABRA_E_UNSUPPORTED, "over 65535 heads of a token");
+    AppendArgs p{paged_view(kv), q, k, v, ldq, ldk, ldv, ldqo, cu_new, q_norm, k_norm, rope, q_out, eps, n_heads, n_tokens, rope_len,
+                 // few tokens: one a CTA, for the shortest way; many: the lookups shared
+                 n_tokens >= 8 * 148 ? APPEND_TOKENS : 1, fast_div(static_cast<uint32_t>(heads))};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
     if (kv->type == ABRA_GGML_F16)

@@ -796,10 +796,7 @@ struct Plan {
 int tile_count(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
 int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumulate, Plan &pl) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&pl.sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return paged_cuda(e, "device properties");
+    pl.sms = device_sm_count();
     const int rows = n_heads / kv->n_kv_heads * n_q;
     pl.nt = tile_count(rows);
     pl.row_blocks = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
@@ -826,7 +823,8 @@ int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumu
 template <typename T, int D, int NT, bool SCORES>
 cudaError_t launch_one(const AttendArgs &p, const Plan &pl, cudaStream_t st) {
     constexpr int smem = Shape<D, NT>::SMEM;
-    const cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D, NT, SCORES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = paged_smem(reinterpret_cast<const void *>(attend_kernel<T, D, NT, SCORES>), smem, done);
     if (e != cudaSuccess) return e;
     attend_kernel<T, D, NT, SCORES><<<pl.pieces, AT_THREADS, smem, st>>>(p);
     return cudaGetLastError();

@@ -289,15 +289,12 @@ cudaError_t launch_kernel(const void *k, dim3 grid, int threads, int smem, int c
 }
 
 cudaError_t launch(EvictArgs &p, cudaStream_t st) {
-    int dev = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e != cudaSuccess) return e;
     const int64_t slots = static_cast<int64_t>(p.kv.a.max_pages) * p.kv.a.page_size;
-    const int cluster = cluster_of(&p.kv.a, sms);
+    const int cluster = cluster_of(&p.kv.a, device_sm_count());
     p.held = static_cast<int>(std::min<int64_t>((slots + cluster - 1) / cluster, HELD_MOST));
     const int smem = LANE_BINS_BYTES + p.held * 4;
-    e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = paged_smem(reinterpret_cast<const void *>(select_kernel), LANE_BINS_BYTES + HELD_MOST * 4, done);
     if (e != cudaSuccess) return e;
     const unsigned heads = p.kv.a.n_kv_heads, seqs = p.kv.a.n_seqs;
     e = launch_kernel(reinterpret_cast<const void *>(select_kernel), dim3(cluster, heads, seqs), SEL_THREADS, smem, cluster, st, p);

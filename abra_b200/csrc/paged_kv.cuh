@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -119,6 +120,15 @@ inline int paged_check(const abra_paged_kv *kv) {
     return ABRA_OK;
 }
 inline PagedKv paged_view(const abra_paged_kv *kv) { return {*kv, fast_div(static_cast<uint32_t>(kv->page_size))}; }
+// Sets a kernel's dynamic shared memory limit once a device (bit d of `done`).
+inline cudaError_t paged_smem(const void *k, int bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (done.load(std::memory_order_relaxed) >> (dev & 63) & 1)) return e;
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return e;
+}
 inline int paged_cuda(cudaError_t e, const char *what) {
     return e == cudaSuccess ? ABRA_OK : paged_fail(ABRA_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }

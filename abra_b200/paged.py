@@ -45,25 +45,29 @@ class PagedKvDesc(C.Structure):
                 ("n_seqs", C.c_int32), ("max_pages", C.c_int32)]
 
 
-def _types() -> dict:
-    import torch
-
-    return {torch.float32: ABRA_GGML_F32, torch.float16: ABRA_GGML_F16, torch.bfloat16: ABRA_GGML_BF16}
-
-
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
 
 
-def _rows(t, name: str, width: int, device) -> tuple[int, int]:
+def _rows(t, name: str, width: int, index: int) -> tuple[int, int]:
     """(rows, row stride) of a tensor [..., heads, head_dim] or [..., width]
-    whose rows of ``width`` elements are contiguous and evenly spaced."""
-    if t.device != device:
+    whose rows of ``width`` elements are contiguous and evenly spaced, on
+    device ``index`` (-1: the CPU)."""
+    if t.get_device() != index:
         raise ValueError(f"{name} must be on the cache's device")
-    shape, stride = t.shape, t.stride()
-    if len(shape) == 2 and shape[1] == width and stride[1] == 1:
-        return shape[0], stride[0] if shape[0] > 1 else width
+    shape = t.shape
+    if len(shape) == 2 and shape[1] == width and t.stride(1) == 1:
+        return shape[0], t.stride(0) if shape[0] > 1 else width
+    n = t.numel() // width if width else 0
+    if t.is_contiguous() and n * width == t.numel() and shape[-1] <= width:
+        inner, i = 1, len(shape)
+        while i > 0 and inner < width:
+            i -= 1
+            inner *= shape[i]
+        if inner == width:
+            return n, width
+    stride = t.stride()
     n, inner, i = 1, 1, len(shape)
     while i > 0 and inner < width:  # the trailing dimensions that make one row
         i -= 1
@@ -128,22 +132,34 @@ class PagedKV:
         def at(t):
             return 0 if t is None else t.data_ptr()
 
+        self._types = {torch.float32: ABRA_GGML_F32, torch.float16: ABRA_GGML_F16,
+                       torch.bfloat16: ABRA_GGML_BF16}
         self.desc = PagedKvDesc(
             at(k), at(v), at(acc), at(pos), at(table), at(lens), at(next_pos), *k.stride()[:3],
             *v.stride()[:3], max(table.stride(0), self.max_pages) if self.n_seqs < 2 else table.stride(0),
-            _types()[k.dtype], self.n_pages, self.n_kv_heads, self.head_dim, self.page_size, self.n_seqs,
+            self._types[k.dtype], self.n_pages, self.n_kv_heads, self.head_dim, self.page_size, self.n_seqs,
             self.max_pages)
         self._ref = C.byref(self.desc)
-        self._types = _types()
+        self._index = k.get_device()
+        # the current stream's handle without building a Stream object, where torch has it
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self._current_device = torch.cuda.current_device
+
+    def _stream(self, stream) -> int:
+        """The stream of a call on this cache, whose device must be the current one."""
+        if self._current_device() != self._index:
+            raise ValueError(f"the cache is on device {self._index}, which is not the current one")
+        if stream is None and self._raw_stream is not None:
+            return self._raw_stream(self._index)
+        return stream_handle(stream)
 
 
-def _vector(t, name: str, n: int, device):
-    import torch
-
+def _vector(t, name: str, n: int, kv: PagedKV):
     if t is None:
         return 0
-    _need(t.device == device and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n,
-          f"{name} must be {n} contiguous float32 values on the cache's device")
+    if not (t.get_device() == kv._index and kv._types.get(t.dtype) == ABRA_GGML_F32 and t.numel() == n
+            and t.is_contiguous()):
+        raise ValueError(f"{name} must be {n} contiguous float32 values on the cache's device")
     return t.data_ptr()
 
 
@@ -159,44 +175,54 @@ def paged_append(kv: PagedKV, k, v, q=None, q_out=None, cu_new=None, q_norm=None
     q_norm, k_norm: float32 [head_dim] RMSNorm weights; rope: float32 [length,
     head_dim / 2, 2], cos and sin of each position.
     """
-    import torch
-
-    dev, hd = kv.device, kv.head_dim
+    dev, hd, types = kv._index, kv.head_dim, kv._types
     kvw = kv.n_kv_heads * hd
+    dtype = k.dtype
     n, ldk = _rows(k, "k", kvw, dev)
     nv, ldv = _rows(v, "v", kvw, dev)
-    _need(nv == n and v.dtype == k.dtype and k.dtype in kv._types,
-          "k and v must have the same rows and type, float32, float16 or bfloat16")
-    heads, ldq, ldqo, qp, qop = 0, 0, 0, 0, 0
+    if nv != n or v.dtype != dtype or dtype not in types:
+        raise ValueError("k and v must have the same rows and type, float32, float16 or bfloat16")
+    heads = ldq = ldqo = qp = qop = 0
     if q is not None:
         width = q.shape[-1] if q.dim() == 2 else q.shape[-2] * q.shape[-1]
-        _need(width % hd == 0, "q must be whole heads")
         heads = width // hd
         nq, ldq = _rows(q, "q", width, dev)
-        _need(nq == n and q.dtype == k.dtype, "q must have the rows and the type of k and v")
+        if heads * hd != width or nq != n or q.dtype != dtype:
+            raise ValueError("q must be whole heads with the rows and the type of k and v")
         if q_out is None:
-            q_out = torch.empty((n, heads, hd), dtype=kv.dtype, device=dev)
+            import torch
+
+            q_out = torch.empty((n, heads, hd), dtype=kv.dtype, device=kv.device)
         no, ldqo = _rows(q_out, "q_out", width, dev)
-        _need(no == n and q_out.dtype == kv.dtype, "q_out must have q's rows and the cache's type")
+        if no != n or q_out.dtype != kv.dtype:
+            raise ValueError("q_out must have q's rows and the cache's type")
         qp, qop = q.data_ptr(), q_out.data_ptr()
-    else:
-        _need(q_out is None, "q_out without q")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    cu = 0
     if cu_new is not None:
-        _need(cu_new.device == dev and cu_new.dtype == torch.int32 and cu_new.is_contiguous()
-              and cu_new.numel() == kv.n_seqs + 1, "cu_new must be contiguous int32 [n_seqs + 1]")
+        if not (cu_new.get_device() == dev and cu_new.dtype == kv.lens.dtype and cu_new.is_contiguous()
+                and cu_new.numel() == kv.n_seqs + 1):
+            raise ValueError("cu_new must be contiguous int32 [n_seqs + 1]")
+        cu = cu_new.data_ptr()
     rope_len = 0
     if rope is not None:
-        _need(rope.dim() == 3 and rope.shape[1] == hd // 2 and rope.shape[2] == 2,
-              "rope must be [length, head_dim / 2, 2]")
+        if rope.dim() != 3 or rope.shape[2] != 2:
+            raise ValueError("rope must be [length, head_dim / 2, 2]")
         rope_len = rope.shape[0]
     rc = lib.abra_paged_append(
-        kv._ref, qp, k.data_ptr(), v.data_ptr(), kv._types[k.dtype], ldq, ldk, ldv, heads,
-        0 if cu_new is None else cu_new.data_ptr(), n, _vector(q_norm, "q_norm", hd, dev),
-        _vector(k_norm, "k_norm", hd, dev), eps, _vector(rope, "rope", rope_len * hd, dev), rope_len, qop,
-        ldqo, stream_handle(stream))
+        kv._ref, qp, k.data_ptr(), v.data_ptr(), types[dtype], ldq, ldk, ldv, heads, cu, n,
+        _vector(q_norm, "q_norm", hd, kv), _vector(k_norm, "k_norm", hd, kv), eps,
+        _vector(rope, "rope", rope_len * hd, kv), rope_len, qop, ldqo, kv._stream(stream))
     if rc:
         _lib.check(rc, "abra_paged_append")
     return q_out
+
+
+def _bytes(workspace, kv: PagedKV) -> tuple[int, int]:
+    if workspace.get_device() != kv._index or not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous on the cache's device")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def _size(n: int, func: str) -> int:
@@ -224,29 +250,26 @@ def paged_attention(kv: PagedKV, q, scale: float, out=None, lse=None, accumulate
     unless a float32 ``out`` is given.  lse: float32 [n_seqs, n_q, heads], log
     of the softmax's denominator.  accumulate: add every slot's weight to
     kv.acc."""
-    import torch
-
-    dev, hd = kv.device, kv.head_dim
-    _need(q.dim() in (3, 4) and q.shape[0] == kv.n_seqs and q.shape[-1] == hd and q.dtype == kv.dtype,
-          "q must be [n_seqs, n_q, heads, head_dim] in the cache's type")
-    heads, n_q = q.shape[-2], q.shape[1] if q.dim() == 4 else 1
+    dev, hd, shape = kv._index, kv.head_dim, q.shape
+    if len(shape) not in (3, 4) or shape[0] != kv.n_seqs or shape[-1] != hd or q.dtype != kv.dtype:
+        raise ValueError("q must be [n_seqs, n_q, heads, head_dim] in the cache's type")
+    heads, n_q = shape[-2], shape[1] if len(shape) == 4 else 1
     width = heads * hd
     _, ldq = _rows(q, "q", width, dev)
     if out is None:
-        out = torch.empty(q.shape, dtype=kv.dtype, device=dev)
-    _need(out.numel() == q.numel() and (out.dtype == kv.dtype or out.dtype == torch.float32),
-          "out must be like q, in the cache's type or float32")
+        import torch
+
+        out = torch.empty(shape, dtype=kv.dtype, device=kv.device)
+    out_type = kv._types.get(out.dtype)
+    if out.numel() != q.numel() or (out.dtype != kv.dtype and out_type != ABRA_GGML_F32):
+        raise ValueError("out must be like q, in the cache's type or float32")
     _, ldo = _rows(out, "out", width, dev)
-    if lse is not None:
-        _need(lse.device == dev and lse.dtype == torch.float32 and lse.is_contiguous()
-              and lse.numel() == kv.n_seqs * n_q * heads, "lse must be contiguous float32 [n_seqs, n_q, heads]")
+    flags = ABRA_PAGED_ACCUMULATE if accumulate else 0
     if workspace is None:
         workspace = paged_attention_workspace(kv, heads, n_q, accumulate)
-    _need(workspace.device == dev and workspace.is_contiguous(), "the workspace must be contiguous on the cache's device")
     rc = lib.abra_paged_attention(
-        kv._ref, q.data_ptr(), ldq, heads, n_q, scale, out.data_ptr(), kv._types[out.dtype], ldo,
-        0 if lse is None else lse.data_ptr(), ABRA_PAGED_ACCUMULATE if accumulate else 0,
-        workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream_handle(stream))
+        kv._ref, q.data_ptr(), ldq, heads, n_q, scale, out.data_ptr(), out_type, ldo,
+        _vector(lse, "lse", kv.n_seqs * n_q * heads, kv), flags, *_bytes(workspace, kv), kv._stream(stream))
     if rc:
         _lib.check(rc, "abra_paged_attention")
     return out
@@ -268,18 +291,17 @@ def paged_evict(kv: PagedKV, budget: int, n_sink: int = 0, n_recent: int = 0, ne
     into the evicted slots below it.  Returns new_lens, int32 [n_seqs]; kv.lens
     is not changed, so that every layer's cache can be cut before
     ``kv.lens.copy_(new_lens)``."""
-    import torch
-
     if new_lens is None:
+        import torch
+
         new_lens = torch.empty(kv.n_seqs, dtype=torch.int32, device=kv.device)
-    _need(new_lens.device == kv.device and new_lens.dtype == torch.int32 and new_lens.is_contiguous()
-          and new_lens.numel() == kv.n_seqs, "new_lens must be contiguous int32 [n_seqs] on the cache's device")
+    elif not (new_lens.get_device() == kv._index and new_lens.dtype == kv.lens.dtype
+              and new_lens.is_contiguous() and new_lens.numel() == kv.n_seqs):
+        raise ValueError("new_lens must be contiguous int32 [n_seqs] on the cache's device")
     if workspace is None:
         workspace = paged_evict_workspace(kv, budget)
-    _need(workspace.device == kv.device and workspace.is_contiguous(),
-          "the workspace must be contiguous on the cache's device")
-    rc = lib.abra_paged_evict(kv._ref, budget, n_sink, n_recent, new_lens.data_ptr(), workspace.data_ptr(),
-                              workspace.numel() * workspace.element_size(), stream_handle(stream))
+    rc = lib.abra_paged_evict(kv._ref, budget, n_sink, n_recent, new_lens.data_ptr(), *_bytes(workspace, kv),
+                              kv._stream(stream))
     if rc:
         _lib.check(rc, "abra_paged_evict")
     return new_lens

@@ -148,12 +148,12 @@ def test_row_strides_of_views():
     from abra_b200.paged import _rows
 
     x = torch.zeros(6, 400)
-    assert _rows(x[:, 8:136], "x", 128, x.device) == (6, 400)
-    assert _rows(x[:, 8:136].unflatten(1, (2, 64)), "x", 128, x.device) == (6, 400)
-    assert _rows(x[:, :384].view(6, 3, 128), "x", 384, x.device) == (6, 400)
-    assert _rows(torch.zeros(2, 3, 4, 64), "x", 256, x.device) == (6, 256)
-    assert _rows(torch.zeros(1, 1, 4, 64), "x", 256, x.device) == (1, 256)
-    assert _rows(x[:0, :128], "x", 128, x.device)[0] == 0
+    assert _rows(x[:, 8:136], "x", 128, -1) == (6, 400)
+    assert _rows(x[:, 8:136].unflatten(1, (2, 64)), "x", 128, -1) == (6, 400)
+    assert _rows(x[:, :384].view(6, 3, 128), "x", 384, -1) == (6, 400)
+    assert _rows(torch.zeros(2, 3, 4, 64), "x", 256, -1) == (6, 256)
+    assert _rows(torch.zeros(1, 1, 4, 64), "x", 256, -1) == (1, 256)
+    assert _rows(x[:0, :128], "x", 128, -1)[0] == 0
     for bad in (x[:, :256:2], torch.zeros(4, 2, 300)[:, :, :128].transpose(0, 1)[:, :, :64], x[:, :100]):
         with pytest.raises(ValueError):
-            _rows(bad, "x", 128, x.device)
+            _rows(bad, "x", 128, -1)
