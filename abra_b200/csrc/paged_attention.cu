@@ -226,8 +226,9 @@ __device__ __forceinline__ bool find_start(const PagedKv &kv, int blocks, int pi
         scan(base);
         total += all;
     }
-    // as many pieces as the GPU holds at once, more where they stay long
-    line = Line(total, min(min(max(least, total / PIECE), most), total));
+    // as many pieces as the GPU holds at once, or whole multiples where they stay long
+    const int waves = max(1, total / (PIECE * least));
+    line = Line(total, min(min(waves * least, most), total));
     if (piece >= line.pieces) return false;
     w.pos = line.begin(piece);
     w.end = line.begin(piece + 1);
@@ -689,13 +690,23 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
         total = total * keep + ml.y * k;  // lane by lane, added up below
         sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
         const int left = min(32, (n - base + JOIN_WARPS - 1) / JOIN_WARPS);
-#pragma unroll 8
-        for (int i = 0; i < left; ++i) {
-            const float ki = __shfl_sync(0xffffffffu, k, i);
-            if (lane < D / 4) {
-                const float4 y = __ldcg(reinterpret_cast<const float4 *>(
-                    p.part_o + (parts.place(base + i * JOIN_WARPS) * r_block + rr) * D + 4 * lane));
-                sum.x += ki * y.x, sum.y += ki * y.y, sum.z += ki * y.z, sum.w += ki * y.w;
+        // all parts but the first lie evenly; 16 loads in flight a lane
+        const int64_t even = (2 * (static_cast<int64_t>(parts.first >> 1) + base) * r_block + rr) * D;
+        const int64_t odd = base == 0 ? (static_cast<int64_t>(parts.first & 1)) * r_block * D : 0;
+        const float *src = p.part_o + even + 4 * min(lane, D / 4 - 1);
+        for (int i0 = 0; i0 < left; i0 += 16) {
+            float4 y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                y[i] = make_float4(0, 0, 0, 0);
+                if (i0 + i < left)
+                    y[i] = __ldcg(reinterpret_cast<const float4 *>(src + (i0 + i == 0 ? odd : 0) +
+                                                                   static_cast<int64_t>(i0 + i) * (2 * JOIN_WARPS * D) * r_block));
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float ki = __shfl_sync(0xffffffffu, k, i0 + i);  // 0 beyond the last part
+                sum.x += ki * y[i].x, sum.y += ki * y[i].y, sum.z += ki * y[i].z, sum.w += ki * y[i].w;
             }
         }
     }

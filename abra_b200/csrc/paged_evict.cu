@@ -50,6 +50,7 @@ __device__ __forceinline__ int cluster_size() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+constexpr int MOST_CTAS = 8;  // of a cluster
 // The value that CTA `rank` of the cluster has at this address of its shared memory.
 __device__ __forceinline__ int peer_value(const int *p, int rank) {
     uint32_t at;
@@ -59,7 +60,7 @@ __device__ __forceinline__ int peer_value(const int *p, int rank) {
     return v;
 }
 
-constexpr int SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32;
+constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32;
 constexpr int BINS = 256;
 constexpr int LANE_BINS_BYTES = BINS * 32 * 4;
 
@@ -89,7 +90,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
         return rank_key(__ldcg(p.kv.a.acc + m), __ldcg(p.kv.a.pos + m), p.n_sink, recent_from);
     };
     auto key = [&](int i) { return i < p.held ? held[i] : load_key(first + i); };
-#pragma unroll 4
+#pragma unroll 8
     for (int i = tid; i < min(n, p.held); i += SEL_THREADS) held[i] = load_key(first + i);
 
     // ---- the budget-th largest key, 8 bits at a time ----
@@ -117,7 +118,9 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
         // bin b of all CTAs, b = BINS - 1 - tid: an inclusive scan from the top
         int all = 0, incl = 0;
         if (tid < BINS) {
-            for (int r = 0; r < size; ++r) all += peer_value(hist + BINS - 1 - tid, r);
+#pragma unroll
+            for (int r = 0; r < MOST_CTAS; ++r)
+                if (r < size) all += peer_value(hist + BINS - 1 - tid, r);
             incl = all;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -259,11 +262,12 @@ int64_t workspace_bytes_of(const abra_paged_kv *kv, int32_t budget) {
 constexpr int HELD_MOST = 40960;  // keys in a CTA's shared memory
 
 // CTAs of a cluster: doubled while all clusters stay resident together and
-// every CTA keeps a few thousand slots' worth of work.
+// every CTA keeps eight slots a thread; adding up histograms of a cluster costs
+// more than a few slots do.
 int cluster_of(const abra_paged_kv *kv, int sms) {
     const int64_t slots = static_cast<int64_t>(kv->max_pages) * kv->page_size;
     int c = 1;
-    while (c < 8 && ((rows_of(kv) * c * 2 <= 4 * sms && slots / c > 2 * SEL_THREADS) || slots / c > HELD_MOST)) c *= 2;
+    while (c < MOST_CTAS && ((rows_of(kv) * c * 2 <= 2 * sms && slots / c > 8 * SEL_THREADS) || slots / c > HELD_MOST)) c *= 2;
     return c;
 }
 
