@@ -51,7 +51,7 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 constexpr int MOST_CTAS = 8;  // of a cluster
-// The value that CTA `rank` of the cluster has at this address of its shared memory.
+// What CTA `rank` of the cluster has at this address of its shared memory.
 __device__ __forceinline__ int peer_value(const int *p, int rank) {
     uint32_t at;
     int v;
@@ -59,8 +59,19 @@ __device__ __forceinline__ int peer_value(const int *p, int rank) {
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
     return v;
 }
+__device__ __forceinline__ int4 peer_value4(const int4 *p, int rank) {
+    uint32_t at;
+    int4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(at)
+                 : "memory");
+    return v;
+}
 
 constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32;
+static_assert(SEL_WARPS == 32, "lanes stand for warps");
 constexpr int BINS = 256;
 constexpr int LANE_BINS_BYTES = BINS * 32 * 4;
 
@@ -69,8 +80,8 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
     extern __shared__ __align__(16) unsigned char smem[];
     int *bins = reinterpret_cast<int *>(smem);  // [BINS][32 lanes]: a lane's own column, so equal keys do not collide
     uint32_t *held = reinterpret_cast<uint32_t *>(smem + LANE_BINS_BYTES);  // keys of the first p.held slots
-    __shared__ int s_hist[2][BINS], s_warp[SEL_WARPS], s_digit, s_left, s_tie[SEL_WARPS], s_hole[SEL_WARPS], s_mover[SEL_WARPS],
-        s_total[2];
+    __shared__ __align__(16) int s_hist[2][BINS];
+    __shared__ int s_found[3], s_tie[SEL_WARPS], s_hole[SEL_WARPS], s_mover[SEL_WARPS], s_total[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = cluster_rank(), size = cluster_size();
     const int g = blockIdx.y, s = blockIdx.z;
@@ -90,17 +101,18 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
         return rank_key(__ldcg(p.kv.a.acc + m), __ldcg(p.kv.a.pos + m), p.n_sink, recent_from);
     };
     auto key = [&](int i) { return i < p.held ? held[i] : load_key(first + i); };
+    for (int i = tid; i < BINS * 32; i += SEL_THREADS) bins[i] = 0;
 #pragma unroll 8
     for (int i = tid; i < min(n, p.held); i += SEL_THREADS) held[i] = load_key(first + i);
+    __syncthreads();
 
-    // ---- the budget-th largest key, 8 bits at a time ----
+    // ---- the budget-th largest key, 8 bits at a time, until all keys with the
+    // leading bits found so far are kept or they are the whole key ----
     uint32_t cut = 0;
-    int left = p.budget;  // of the keys that share cut's leading bits, so many are kept
+    int left = p.budget, same = 0, pass = 0;  // of the `same` keys that share cut's leading bits, `left` are kept
 #pragma unroll 1
-    for (int pass = 0; pass < 4; ++pass) {
+    for (; pass < 4; ++pass) {
         const int shift = 24 - 8 * pass;
-        for (int i = tid; i < BINS * 32; i += SEL_THREADS) bins[i] = 0;
-        __syncthreads();
 #pragma unroll 4
         for (int i = tid; i < n; i += SEL_THREADS) {
             const uint32_t k = key(i);
@@ -114,55 +126,72 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
             for (int x = 0; x < 32; ++x) sum += bins[tid * 32 + ((x + tid) & 31)];
             hist[tid] = sum;
         }
-        cluster_sync();
-        // bin b of all CTAs, b = BINS - 1 - tid: an inclusive scan from the top
-        int all = 0, incl = 0;
-        if (tid < BINS) {
+        if (size > 1) cluster_sync();
+        else __syncthreads();
+        if (warp == 0) {  // lane l: bins 8 l .. 8 l + 7 of all CTAs; a scan from the top bin
+            int b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
             for (int r = 0; r < MOST_CTAS; ++r)
-                if (r < size) all += peer_value(hist + BINS - 1 - tid, r);
-            incl = all;
+                if (r < size) {
+                    const int4 x = peer_value4(reinterpret_cast<const int4 *>(hist) + 2 * lane, r);
+                    const int4 y = peer_value4(reinterpret_cast<const int4 *>(hist) + 2 * lane + 1, r);
+                    b[0] += x.x, b[1] += x.y, b[2] += x.z, b[3] += x.w, b[4] += y.x, b[5] += y.y, b[6] += y.z, b[7] += y.w;
+                }
+            int above = b[0] + b[1] + b[2] + b[3] + b[4] + b[5] + b[6] + b[7];
+            const int own = above;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, incl, d);
-                if (lane >= d) incl += y;
+                const int y = __shfl_down_sync(0xffffffffu, above, d);
+                if (lane + d < 32) above += y;
             }
-            if (lane == 31) s_warp[warp] = incl;
+            above -= own;  // keys in higher lanes' bins
+#pragma unroll
+            for (int x = 7; x >= 0; --x) {
+                if (above < left && above + b[x] >= left) s_found[0] = 8 * lane + x, s_found[1] = left - above, s_found[2] = b[x];
+                above += b[x];
+            }
+        } else {  // the others empty the bins for the next pass
+            for (int i = tid - 32; i < BINS * 32; i += SEL_THREADS - 32) bins[i] = 0;
         }
         __syncthreads();
-        if (tid < BINS) {
-            for (int x = 0; x < warp; ++x) incl += s_warp[x];
-            if (incl >= left && incl - all < left) s_digit = BINS - 1 - tid, s_left = left - (incl - all);
-        }
-        __syncthreads();
-        cut |= static_cast<uint32_t>(s_digit) << shift;
-        left = s_left;
+        cut |= static_cast<uint32_t>(s_found[0]) << shift;
+        left = s_found[1], same = s_found[2];
+        if (left == same) break;  // the same in every CTA
     }
-    // `left` of the slots whose key is cut stay: the lowest.  The last pass
-    // counted them in each CTA.
+    // Slots with a key above cut stay, and of those at cut the lowest `left`.
+    // Only after four passes can there be others at cut (equal keys); the last
+    // pass counted them in each CTA.
+    const bool equals = left != same;
     int ties = 0;
-    for (int r = 0; r < rank; ++r) ties += peer_value(&s_hist[1][cut & 255], r);
 
     // ---- holes and movers in slot order: a run of slots for each warp ----
     const int run = ((n + SEL_WARPS - 1) / SEL_WARPS + 31) & ~31, w0 = min(n, warp * run), w1 = min(n, w0 + run);
-    int own = 0;
-    for (int i = w0; i < w1; i += 32) own += __popc(__ballot_sync(0xffffffffu, i + lane < w1 && key(i + lane) == cut));
-    if (lane == 0) s_tie[warp] = own;
-    __syncthreads();
-    for (int x = 0; x < warp; ++x) ties += s_tie[x];
+    if (equals) {
+        for (int r = 0; r < rank; ++r) ties += peer_value(&s_hist[1][cut & 255], r);
+        int own = 0;
+#pragma unroll 4
+        for (int i = w0; i < w1; i += 32) own += __popc(__ballot_sync(0xffffffffu, i + lane < w1 && key(i + lane) == cut));
+        if (lane == 0) s_tie[warp] = own;
+        __syncthreads();
+        for (int x = 0; x < warp; ++x) ties += s_tie[x];
+    }
     // one step of 32 slots: which are holes, which movers
     const unsigned below = (1u << lane) - 1u;
     auto classify = [&](int i, int &tie, unsigned &holes, unsigned &movers) {
         const bool in = i + lane < w1;
         const uint32_t k = in ? key(i + lane) : 0u;
-        const unsigned t = __ballot_sync(0xffffffffu, in && k == cut);
-        const bool keep = in && (k > cut || (k == cut && tie + __popc(t & below) < left));
-        tie += __popc(t);
+        bool keep = in && k >= cut;
+        if (equals) {
+            const unsigned t = __ballot_sync(0xffffffffu, in && k == cut);
+            keep = in && (k > cut || (k == cut && tie + __popc(t & below) < left));
+            tie += __popc(t);
+        }
         const bool low = first + i + lane < p.budget;
         holes = __ballot_sync(0xffffffffu, in && low && !keep);
         movers = __ballot_sync(0xffffffffu, !low && keep);
     };
     int nh = 0, nm = 0, tie = ties;
+#pragma unroll 4
     for (int i = w0; i < w1; i += 32) {
         unsigned h, m;
         classify(i, tie, h, m);
@@ -170,18 +199,22 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
     }
     if (lane == 0) s_hole[warp] = nh, s_mover[warp] = nm;
     __syncthreads();
-    if (tid < 2) {
-        int sum = 0;
-        for (int x = 0; x < SEL_WARPS; ++x) sum += tid ? s_mover[x] : s_hole[x];
-        s_total[tid] = sum;
+    // lanes add up the warps, and the CTAs of the cluster
+    int hole_at = s_hole[lane], mover_at = s_mover[lane];
+    if (warp == 0) {
+        const int h = __reduce_add_sync(0xffffffffu, hole_at), m = __reduce_add_sync(0xffffffffu, mover_at);
+        if (lane == 0) s_total[0] = h, s_total[1] = m;
     }
-    cluster_sync();
-    int hole_at = 0, mover_at = 0;
-    for (int r = 0; r < rank; ++r) hole_at += peer_value(&s_total[0], r), mover_at += peer_value(&s_total[1], r);
+    hole_at = __reduce_add_sync(0xffffffffu, lane < warp ? hole_at : 0);
+    mover_at = __reduce_add_sync(0xffffffffu, lane < warp ? mover_at : 0);
+    if (size > 1) cluster_sync();
+    else __syncthreads();
+    hole_at += __reduce_add_sync(0xffffffffu, lane < rank ? peer_value(&s_total[0], lane) : 0);
+    mover_at += __reduce_add_sync(0xffffffffu, lane < rank ? peer_value(&s_total[1], lane) : 0);
     if (rank == size - 1 && tid == 0) p.counts[row] = hole_at + s_total[0];
-    for (int x = 0; x < warp; ++x) hole_at += s_hole[x], mover_at += s_mover[x];
     int32_t *hole = p.moves + row * 2 * p.cap, *mover = hole + p.cap;
     tie = ties;
+#pragma unroll 4
     for (int i = w0; i < w1; i += 32) {
         unsigned h, m;
         classify(i, tie, h, m);
@@ -189,7 +222,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
         if (m >> lane & 1) mover[mover_at + __popc(m & below)] = first + i + lane;
         hole_at += __popc(h), mover_at += __popc(m);
     }
-    cluster_sync();  // nobody leaves while its shared memory is read
+    if (size > 1) cluster_sync();  // nobody leaves while its shared memory is read
 }
 
 constexpr int MOVE_THREADS = 256, MOVES = 128;
