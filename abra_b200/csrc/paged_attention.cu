@@ -26,48 +26,17 @@
 // banks.
 #include <algorithm>
 
-#include "paged_kv.cuh"
+#include "paged_attention.cuh"
 
 namespace abra {
 namespace {
 
 constexpr int AT_WARPS = 4, AT_THREADS = AT_WARPS * 32;
-constexpr int TILE = 16;                  // slots of a warp's tile
-constexpr int STEP = TILE * AT_WARPS;     // slots of a CTA's step
-constexpr int SCAN = AT_THREADS;          // sequences of one block scan
-constexpr int PIECE = 8;                  // steps of a piece, where there are enough to fill the GPU
-constexpr int WAVES = 4;                  // pieces for each CTA that the GPU holds, at most
-// A row's maximum is raised only when a score passes it by 2^RAISE: weights
-// stay below 2^RAISE (well inside fp16), and most tiles need no reduction.
-constexpr float RAISE = 10.0f;
-// What beginning and ending a row costs beside its steps, in steps (its
-// queries, the join of its warps).
-constexpr int ROW_COST = 1;
-
-struct AttendArgs {
-    PagedKv kv;
-    const void *q;
-    void *out;
-    float *lse;
-    int64_t ldq, ldo;
-    float scale_log2;  // scale / ln 2: scores are kept in units of log2
-    int n_heads, n_q, group, rows, row_blocks, out_f32;
-    int resident;  // CTAs of the first kernel that the GPU holds at once
-    // workspace
-    float *part_o;      // [piece][2][8 NT][D]
-    float2 *part_ml;    // [piece][2][8 NT] maximum (log2 units) and sum
-    int2 *split;        // [seq][kv head][row block] the first part's place, the last part's piece
-    float *row_lse;     // [seq][kv head][row] log2 of the sum of a row that lies in one piece
-    float *scores;      // [page][kv head][offset][padded rows], log2 units
-};
+constexpr int TILE = 16;               // slots of a warp's tile
+constexpr int STEP = TILE * AT_WARPS;  // slots of a CTA's step
+constexpr int WIDE_FROM = 16;          // more rows a kv head go to the kernel of paged_attention_wide.cu
 
 // ------------------------------------------------------------------ PTX ---
-// 16 bytes into shared memory past L1; `bytes` 0 writes zeros and reads nothing.
-__device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 template <typename T>
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                             uint32_t b0, uint32_t b1);
@@ -108,149 +77,6 @@ __device__ __forceinline__ uint32_t trans8x8(uint32_t a) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x);
-template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&x));
-}
-template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&x));
-}
-// The packed pair with its infinities and NaNs as zeros; `any` collects them.
-template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t x, bool &any) {
-    constexpr uint32_t EXP = Half16<T>::type == ABRA_GGML_F16 ? 0x7c00u : 0x7f80u;
-    if ((x & EXP) == EXP) x &= 0xffff0000u, any = true;
-    if ((x & (EXP << 16)) == (EXP << 16)) x &= 0x0000ffffu, any = true;
-    return x;
-}
-
-// ------------------------------------------------------------ the line ---
-__device__ __forceinline__ int steps_of(int len) { return (len + STEP - 1) / STEP; }
-
-struct Line {
-    int total;       // the triples' costs
-    int pieces;      // each has at least one unit of cost
-    int quot, rest;  // total / pieces and what is left
-    __device__ __forceinline__ Line(int total, int pieces) : total(total), pieces(pieces), quot(0), rest(0) {
-        if (pieces > 0) quot = total / pieces, rest = total - quot * pieces;
-    }
-    // the first `rest` pieces are one longer
-    __device__ __forceinline__ int begin(int i) const { return i * quot + min(i, rest); }
-    __device__ __forceinline__ int piece(int x) const {  // the piece that holds x
-        const int longer = rest * (quot + 1);
-        return x < longer ? x / (quot + 1) : rest + (x - longer) / quot;
-    }
-};
-
-// A segment: the steps [tile0, tile1) of one triple that lie in a piece.
-struct Segment {
-    int seq, len, n;          // the sequence, its slots and steps
-    int unit, row_begin;      // the triple of this sequence and its first place on the line
-    int head, block;          // its kv head and block of rows
-    int tile0, tile1, slot_end;
-};
-
-// Walks the segments of the piece [pos, end).  `units` triples share a
-// sequence's length, `blocks` of them a kv head; a triple of n steps takes
-// ROW_COST + n places.
-struct Walk {
-    int pos, end, seq_begin, units, blocks;
-    Segment s;
-    __device__ __forceinline__ int span() const { return s.n ? (s.n + ROW_COST) * units : 0; }
-    __device__ __forceinline__ void length(int len) { s.len = len, s.n = steps_of(len); }
-    // the segment at pos; false when the piece ends before its first step
-    __device__ __forceinline__ bool enter(const PagedKv &kv) {
-        while (pos >= seq_begin + span()) {  // the next sequence with slots
-            seq_begin += span();
-            length(paged_len(kv, ++s.seq));
-        }
-        s.unit = (pos - seq_begin) / (s.n + ROW_COST);
-        s.head = s.unit / blocks;
-        s.block = s.unit - s.head * blocks;
-        s.row_begin = seq_begin + s.unit * (s.n + ROW_COST);
-        s.tile0 = max(0, pos - s.row_begin - ROW_COST);
-        s.tile1 = min(s.n, end - s.row_begin - ROW_COST);
-        s.slot_end = min(s.len, s.tile1 * STEP);
-        return s.tile0 < s.tile1;
-    }
-    // the next segment, if there is one
-    __device__ __forceinline__ bool next(const PagedKv &kv) {
-        pos = s.row_begin + ROW_COST + s.tile1;
-        return pos < end && enter(kv);
-    }
-};
-
-// Sums the sequences' costs and finds the one in which piece `piece` of at
-// most `most` begins; false when there is nothing in it.  All threads of the
-// block.
-__device__ __forceinline__ bool find_start(const PagedKv &kv, int blocks, int piece, int most, int least, Line &line, Walk &w) {
-    __shared__ int s_warp[AT_WARPS], s_seq, s_begin, s_len;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = kv.a.n_seqs;
-    const int units = kv.a.n_kv_heads * blocks;
-    // inclusive scan of the costs of sequences base .. base + SCAN - 1
-    int len = 0, own = 0, incl = 0, all = 0;
-    auto scan = [&](int base) {
-        len = base + tid < n ? paged_len(kv, base + tid) : 0;
-        own = len ? (steps_of(len) + ROW_COST) * units : 0;
-        incl = own;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += y;
-        }
-        __syncthreads();
-        if (lane == 31) s_warp[warp] = incl;
-        __syncthreads();
-        all = 0;
-#pragma unroll
-        for (int x = 0; x < AT_WARPS; ++x) {
-            if (x < warp) incl += s_warp[x];
-            all += s_warp[x];
-        }
-    };
-    int total = 0;
-    for (int base = 0; base < n; base += SCAN) {
-        scan(base);
-        total += all;
-    }
-    // as many pieces as the GPU holds at once, or whole multiples where they stay long
-    const int waves = max(1, total / (PIECE * least));
-    line = Line(total, min(min(waves * least, most), total));
-    if (piece >= line.pieces) return false;
-    w.pos = line.begin(piece);
-    w.end = line.begin(piece + 1);
-    w.units = units;
-    w.blocks = blocks;
-    int before = 0;
-    if (n <= SCAN) {
-        if (incl > w.pos && incl - own <= w.pos) s_seq = tid, s_begin = incl - own, s_len = len;
-    } else {
-        for (int base = 0; before <= w.pos; base += SCAN) {
-            scan(base);
-            if (before + incl > w.pos && before + incl - own <= w.pos) s_seq = base + tid, s_begin = before + incl - own, s_len = len;
-            before += all;
-        }
-    }
-    __syncthreads();
-    w.s.seq = s_seq;
-    w.seq_begin = s_begin;
-    w.length(s_len);
-    return w.enter(kv);
-}
-
 // --------------------------------------------------------------- kernel ---
 template <int D, int NT> struct Shape {
     static constexpr int KS = D / 16;           // k-steps of the scores, and 16-element tiles of the output
@@ -270,34 +96,6 @@ template <int D, int NT> struct Shape {
     static_assert(DEPTH >= 2, "the ring needs two tiles");
 };
 
-template <typename T>
-__device__ __forceinline__ void store_out(const AttendArgs &p, int64_t at, float4 x) {
-    if (p.out_f32) {
-        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = x;
-    } else {
-        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
-    }
-}
-
-// A finished row: out at elements d .. d + 3, its lse by the lane of element 0.
-// total == 0: the row saw nothing.
-template <typename T>
-__device__ __forceinline__ void finish_row(const AttendArgs &p, int seq, int head, int r, int d, int D, float4 o, float m,
-                                           float total) {
-    const int j = r / p.group, h = head * p.group + r - j * p.group;
-    const int64_t row = static_cast<int64_t>(seq) * p.n_q + j;
-    const float inv = total != 0.0f ? 1.0f / total : 0.0f;
-    store_out<T>(p, row * p.ldo + static_cast<int64_t>(h) * D + d,
-                 total != 0.0f ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0, 0, 0, 0));
-    if (d == 0) {
-        const float l2 = total != 0.0f ? m + log2f(total) : -INFINITY;
-        if (p.lse) p.lse[row * p.n_heads + h] = l2 * 0.69314718055994531f;
-        if (p.row_lse)
-            p.row_lse[(static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.rows + r] = l2;
-    }
-}
-__device__ __forceinline__ float scaled(float m, float top) { return m == top ? 1.0f : exp2_fast(m - top); }
-
 template <typename T, int D, int NT, bool SCORES>
 __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kernel(const __grid_constant__ AttendArgs p) {
     using S = Shape<D, NT>;
@@ -308,9 +106,9 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
 
     pdl_launch_dependents();  // the join may take its place; it waits for the whole grid
-    Walk w;
+    Walk<STEP> w;
     Line line(0, 0);
-    if (!find_start(p.kv, p.row_blocks, blockIdx.x, gridDim.x, p.resident, line, w)) return;
+    if (!find_start<AT_THREADS>(p.kv, p.row_blocks, blockIdx.x, gridDim.x, p.resident, line, w)) return;
     const int begin = w.pos;
 
     // ---- the fetching side: this warp's tiles, segment after segment ----
@@ -319,7 +117,7 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
     // rows 8-15.  Where eight divides the page size each half lies in one page.
     const uint32_t ring = smem_u32(smem) + warp * (S::DEPTH * 2 * S::TILE_BYTES);
     const bool by8 = p.kv.a.page_size % 8 == 0;
-    Walk f = w;
+    Walk<STEP> f = w;
     int f_base = f.s.tile0 * STEP + warp * TILE, f_valid = 0;
     int f_page0 = 0, f_page1 = 0;  // of the halves, or (by8 false) f_page0 of row lane % 16
     uint32_t f_at = ring;
@@ -690,21 +488,21 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
         total = total * keep + ml.y * k;  // lane by lane, added up below
         sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
         const int left = min(32, (n - base + JOIN_WARPS - 1) / JOIN_WARPS);
-        // all parts but the first lie evenly; 16 loads in flight a lane
+        // all parts but the first lie evenly; eight loads in flight a lane
         const int64_t even = (2 * (static_cast<int64_t>(parts.first >> 1) + base) * r_block + rr) * D;
         const int64_t odd = base == 0 ? (static_cast<int64_t>(parts.first & 1)) * r_block * D : 0;
         const float *src = p.part_o + even + 4 * min(lane, D / 4 - 1);
-        for (int i0 = 0; i0 < left; i0 += 16) {
-            float4 y[16];
+        for (int i0 = 0; i0 < left; i0 += 8) {
+            float4 y[8];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 8; ++i) {
                 y[i] = make_float4(0, 0, 0, 0);
                 if (i0 + i < left)
                     y[i] = __ldcg(reinterpret_cast<const float4 *>(src + (i0 + i == 0 ? odd : 0) +
                                                                    static_cast<int64_t>(i0 + i) * (2 * JOIN_WARPS * D) * r_block));
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 8; ++i) {
                 const float ki = __shfl_sync(0xffffffffu, k, i0 + i);  // 0 beyond the last part
                 sum.x += ki * y[i].x, sum.y += ki * y[i].y, sum.z += ki * y[i].z, sum.w += ki * y[i].w;
             }
@@ -737,10 +535,10 @@ constexpr int ACC_ROWS = 64;  // rows whose lse is held at a time
 __global__ void __launch_bounds__(AT_THREADS) accumulate_kernel(const __grid_constant__ AttendArgs p, int r_block, int padded) {
     __shared__ float s_lse[ACC_ROWS];
     const int tid = threadIdx.x, heads = p.kv.a.n_kv_heads, half = tid & 1;
-    Walk w;
+    Walk<STEP> w;
     Line line(0, 0);
     pdl_wait();
-    if (!find_start(p.kv, 1, blockIdx.x, gridDim.x, gridDim.x, line, w)) return;
+    if (!find_start<AT_THREADS>(p.kv, 1, blockIdx.x, gridDim.x, gridDim.x, line, w)) return;
     do {
         const Segment &sg = w.s;
         for (int r0 = 0; r0 < p.rows; r0 += ACC_ROWS) {
@@ -800,32 +598,33 @@ __global__ void __launch_bounds__(AT_THREADS) accumulate_kernel(const __grid_con
 
 // ------------------------------------------------------------------ host ---
 struct Plan {
-    int nt, row_blocks, resident, pieces, sms;
+    int wide, block, row_blocks, resident, pieces, sms;  // block: rows of a block
     int64_t part_o, part_ml, split, row_lse, scores, bytes;  // workspace offsets
 };
 
-int tile_count(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 
 int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumulate, Plan &pl) {
     pl.sms = device_sm_count();
     const int rows = n_heads / kv->n_kv_heads * n_q;
-    pl.nt = tile_count(rows);
-    pl.row_blocks = (rows + 8 * pl.nt - 1) / (8 * pl.nt);
+    pl.wide = rows > WIDE_FROM;
+    pl.block = pl.wide ? (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) : rows <= 8 ? 8 : 16;
+    pl.row_blocks = (rows + pl.block - 1) / pl.block;
     const int64_t triples = static_cast<int64_t>(kv->n_seqs) * kv->n_kv_heads * pl.row_blocks;
-    const int64_t steps = (static_cast<int64_t>(kv->max_pages) * kv->page_size + STEP - 1) / STEP + ROW_COST;
-    if (steps * triples > 0x7fffffff) return paged_fail(ABRA_E_UNSUPPORTED, "the tables name over 2^31 steps of %d slots", STEP);
-    pl.resident = pl.sms * (pl.nt == 1 ? 3 : 2);
+    const int step = pl.wide ? WIDE_STEP : STEP;
+    const int64_t steps = (static_cast<int64_t>(kv->max_pages) * kv->page_size + step - 1) / step + ROW_COST;
+    if (steps * triples > 0x7fffffff) return paged_fail(ABRA_E_UNSUPPORTED, "the tables name over 2^31 steps of %d slots", step);
+    pl.resident = pl.sms * (pl.wide ? 1 : pl.block == 8 ? 3 : 2);
     pl.pieces = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(pl.resident) * WAVES, steps * triples));
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     int64_t at = 0;
-    pl.part_o = at, at = up(at + static_cast<int64_t>(pl.pieces) * 2 * 8 * pl.nt * kv->head_dim * 4);
-    pl.part_ml = at, at = up(at + static_cast<int64_t>(pl.pieces) * 2 * 8 * pl.nt * 8);
+    pl.part_o = at, at = up(at + static_cast<int64_t>(pl.pieces) * 2 * pl.block * kv->head_dim * 4);
+    pl.part_ml = at, at = up(at + static_cast<int64_t>(pl.pieces) * 2 * pl.block * 8);
     pl.split = at, at = up(at + triples * 8);
     pl.row_lse = pl.scores = at;
     if (accumulate) {
         at = up(at + static_cast<int64_t>(kv->n_seqs) * kv->n_kv_heads * rows * 4);
         pl.scores = at;
-        at = up(at + static_cast<int64_t>(kv->n_pages) * kv->n_kv_heads * kv->page_size * pl.row_blocks * 8 * pl.nt * 4);
+        at = up(at + static_cast<int64_t>(kv->n_pages) * kv->n_kv_heads * kv->page_size * pl.row_blocks * pl.block * 4);
     }
     pl.bytes = at;
     return ABRA_OK;
@@ -842,9 +641,7 @@ cudaError_t launch_one(const AttendArgs &p, const Plan &pl, cudaStream_t st) {
 }
 template <typename T, int D, bool SCORES>
 cudaError_t launch_rows(const AttendArgs &p, const Plan &pl, cudaStream_t st) {
-    return pl.nt == 1   ? launch_one<T, D, 1, SCORES>(p, pl, st)
-           : pl.nt == 2 ? launch_one<T, D, 2, SCORES>(p, pl, st)
-                        : launch_one<T, D, 4, SCORES>(p, pl, st);
+    return pl.block == 8 ? launch_one<T, D, 1, SCORES>(p, pl, st) : launch_one<T, D, 2, SCORES>(p, pl, st);
 }
 // A launch that may begin before the kernel in front of it has ended (its
 // pdl_wait waits for that).
@@ -861,9 +658,10 @@ template <typename... A> cudaError_t launch_after(void (*k)(A...), dim3 grid, in
     return cudaLaunchKernelEx(&cfg, k, a...);
 }
 template <typename T, int D> cudaError_t launch_all(const AttendArgs &p, const Plan &pl, bool accumulate, cudaStream_t st) {
-    cudaError_t e = accumulate ? launch_rows<T, D, true>(p, pl, st) : launch_rows<T, D, false>(p, pl, st);
+    cudaError_t e = pl.wide ? launch_attend_wide(p, pl.block, pl.pieces, accumulate, st)
+                    : accumulate ? launch_rows<T, D, true>(p, pl, st) : launch_rows<T, D, false>(p, pl, st);
     if (e != cudaSuccess) return e;
-    const int r_block = 8 * pl.nt;
+    const int r_block = pl.block;
     e = launch_after(join_kernel<T, D>, dim3(p.rows, p.kv.a.n_kv_heads, p.kv.a.n_seqs), JOIN_WARPS * 32, st, p, r_block);
     if (e != cudaSuccess || !accumulate) return e;
     return launch_after(accumulate_kernel, dim3(pl.sms * 8), AT_THREADS, st, p, r_block, pl.row_blocks * r_block);

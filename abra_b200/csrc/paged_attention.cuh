@@ -1,0 +1,222 @@
+// paged_attention.cuh -- what the kernels of the paged attention share: their
+// arguments, the line of steps that their CTAs divide, and the end of a row.
+#pragma once
+
+#include "paged_kv.cuh"
+
+namespace abra {
+
+constexpr int PIECE = 8;                  // steps of a piece, where there are enough to fill the GPU
+constexpr int WAVES = 4;                  // pieces for each CTA that the GPU holds, at most
+// A row's maximum is raised only when a score passes it by 2^RAISE: weights
+// stay below 2^RAISE (well inside fp16), and most tiles need no reduction.
+constexpr float RAISE = 10.0f;
+// What beginning and ending a row costs beside its steps, in steps (its
+// queries, the join of its warps).
+constexpr int ROW_COST = 1;
+
+struct AttendArgs {
+    PagedKv kv;
+    const void *q;
+    void *out;
+    float *lse;
+    int64_t ldq, ldo;
+    float scale_log2;  // scale / ln 2: scores are kept in units of log2
+    int n_heads, n_q, group, rows, row_blocks, out_f32;
+    int resident;  // CTAs of the first kernel that the GPU holds at once
+    // workspace
+    float *part_o;      // [piece][2][rows of a block][D]
+    float2 *part_ml;    // [piece][2][rows of a block] maximum (log2 units) and sum
+    int2 *split;        // [seq][kv head][row block] the first part's place, the last part's piece
+    float *row_lse;     // [seq][kv head][row] log2 of the sum of a row that lies in one piece
+    float *scores;      // [page][kv head][offset][padded rows], log2 units
+};
+
+// ------------------------------------------------------------------ PTX ---
+// 16 bytes into shared memory past L1; `bytes` 0 writes zeros and reads nothing.
+__device__ __forceinline__ void copy_async(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// What a sum relative to the maximum m counts relative to `top`.
+__device__ __forceinline__ float scaled(float m, float top) { return m == top ? 1.0f : exp2_fast(m - top); }
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t x);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t x) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&x));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&x));
+}
+// The packed pair with its infinities and NaNs as zeros; `any` collects them.
+template <typename T> __device__ __forceinline__ uint32_t finite_part(uint32_t x, bool &any) {
+    constexpr uint32_t EXP = Half16<T>::type == ABRA_GGML_F16 ? 0x7c00u : 0x7f80u;
+    if ((x & EXP) == EXP) x &= 0xffff0000u, any = true;
+    if ((x & (EXP << 16)) == (EXP << 16)) x &= 0x0000ffffu, any = true;
+    return x;
+}
+
+// ------------------------------------------------------------ the line ---
+struct Line {
+    int total;       // the triples' costs
+    int pieces;      // each has at least one unit of cost
+    int quot, rest;  // total / pieces and what is left
+    __device__ __forceinline__ Line(int total, int pieces) : total(total), pieces(pieces), quot(0), rest(0) {
+        if (pieces > 0) quot = total / pieces, rest = total - quot * pieces;
+    }
+    // the first `rest` pieces are one longer
+    __device__ __forceinline__ int begin(int i) const { return i * quot + min(i, rest); }
+    __device__ __forceinline__ int piece(int x) const {  // the piece that holds x
+        const int longer = rest * (quot + 1);
+        return x < longer ? x / (quot + 1) : rest + (x - longer) / quot;
+    }
+};
+
+// A segment: the steps [tile0, tile1) of one triple that lie in a piece.
+struct Segment {
+    int seq, len, n;          // the sequence, its slots and steps
+    int unit, row_begin;      // the triple of this sequence and its first place on the line
+    int head, block;          // its kv head and block of rows
+    int tile0, tile1, slot_end;
+};
+
+// Walks the segments of the piece [pos, end).  `units` triples share a
+// sequence's length, `blocks` of them a kv head; a triple of n steps of STEP
+// slots takes ROW_COST + n places.
+template <int STEP> struct Walk {
+    int pos, end, seq_begin, units, blocks;
+    Segment s;
+    static __device__ __forceinline__ int steps_of(int len) { return (len + STEP - 1) / STEP; }
+    __device__ __forceinline__ int span() const { return s.n ? (s.n + ROW_COST) * units : 0; }
+    __device__ __forceinline__ void length(int len) { s.len = len, s.n = steps_of(len); }
+    // the segment at pos; false when the piece ends before its first step
+    __device__ __forceinline__ bool enter(const PagedKv &kv) {
+        while (pos >= seq_begin + span()) {  // the next sequence with slots
+            seq_begin += span();
+            length(paged_len(kv, ++s.seq));
+        }
+        s.unit = (pos - seq_begin) / (s.n + ROW_COST);
+        s.head = s.unit / blocks;
+        s.block = s.unit - s.head * blocks;
+        s.row_begin = seq_begin + s.unit * (s.n + ROW_COST);
+        s.tile0 = max(0, pos - s.row_begin - ROW_COST);
+        s.tile1 = min(s.n, end - s.row_begin - ROW_COST);
+        s.slot_end = min(s.len, s.tile1 * STEP);
+        return s.tile0 < s.tile1;
+    }
+    // the next segment, if there is one
+    __device__ __forceinline__ bool next(const PagedKv &kv) {
+        pos = s.row_begin + ROW_COST + s.tile1;
+        return pos < end && enter(kv);
+    }
+};
+
+// Sums the sequences' costs and finds the one in which piece `piece` of at
+// most `most` begins; false when there is nothing in it.  All THREADS threads
+// of the block.
+template <int THREADS, int STEP>
+__device__ __forceinline__ bool find_start(const PagedKv &kv, int blocks, int piece, int most, int least, Line &line, Walk<STEP> &w) {
+    constexpr int WARPS = THREADS / 32;
+    __shared__ int s_warp[WARPS], s_seq, s_begin, s_len;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = kv.a.n_seqs;
+    const int units = kv.a.n_kv_heads * blocks;
+    // inclusive scan of the costs of sequences base .. base + THREADS - 1
+    int len = 0, own = 0, incl = 0, all = 0;
+    auto scan = [&](int base) {
+        len = base + tid < n ? paged_len(kv, base + tid) : 0;
+        own = len ? (Walk<STEP>::steps_of(len) + ROW_COST) * units : 0;
+        incl = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += y;
+        }
+        __syncthreads();
+        if (lane == 31) s_warp[warp] = incl;
+        __syncthreads();
+        all = 0;
+#pragma unroll
+        for (int x = 0; x < WARPS; ++x) {
+            if (x < warp) incl += s_warp[x];
+            all += s_warp[x];
+        }
+    };
+    int total = 0;
+    for (int base = 0; base < n; base += THREADS) {
+        scan(base);
+        total += all;
+    }
+    // as many pieces as the GPU holds at once, or whole multiples where they stay long
+    const int waves = max(1, total / (PIECE * least));
+    line = Line(total, min(min(waves * least, most), total));
+    if (piece >= line.pieces) return false;
+    w.pos = line.begin(piece);
+    w.end = line.begin(piece + 1);
+    w.units = units;
+    w.blocks = blocks;
+    int before = 0;
+    if (n <= THREADS) {
+        if (incl > w.pos && incl - own <= w.pos) s_seq = tid, s_begin = incl - own, s_len = len;
+    } else {
+        for (int base = 0; before <= w.pos; base += THREADS) {
+            scan(base);
+            if (before + incl > w.pos && before + incl - own <= w.pos) s_seq = base + tid, s_begin = before + incl - own, s_len = len;
+            before += all;
+        }
+    }
+    __syncthreads();
+    w.s.seq = s_seq;
+    w.seq_begin = s_begin;
+    w.length(s_len);
+    return w.enter(kv);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_out(const AttendArgs &p, int64_t at, float4 x) {
+    if (p.out_f32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = x;
+    } else {
+        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
+    }
+}
+
+// A finished row's lse; total == 0: the row saw nothing.
+__device__ __forceinline__ void finish_lse(const AttendArgs &p, int seq, int head, int r, float m, float total) {
+    const int j = r / p.group, h = head * p.group + r - j * p.group;
+    const float l2 = total != 0.0f ? m + log2f(total) : -INFINITY;
+    if (p.lse) p.lse[(static_cast<int64_t>(seq) * p.n_q + j) * p.n_heads + h] = l2 * 0.69314718055994531f;
+    if (p.row_lse) p.row_lse[(static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.rows + r] = l2;
+}
+
+// A finished row: out at elements d .. d + 3, its lse by the lane of element 0.
+template <typename T>
+__device__ __forceinline__ void finish_row(const AttendArgs &p, int seq, int head, int r, int d, int D, float4 o, float m,
+                                           float total) {
+    const int j = r / p.group, h = head * p.group + r - j * p.group;
+    const int64_t row = static_cast<int64_t>(seq) * p.n_q + j;
+    const float inv = total != 0.0f ? 1.0f / total : 0.0f;
+    store_out<T>(p, row * p.ldo + static_cast<int64_t>(h) * D + d,
+                 total != 0.0f ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0, 0, 0, 0));
+    if (d == 0) finish_lse(p, seq, head, r, m, total);
+}
+
+// The kernel for blocks of 16 to 64 rows (paged_attention_wide.cu); one CTA a
+// multiprocessor.  `n`: rows of a block, 16, 32 or 64.
+constexpr int WIDE_STEP = 128;  // its slots a step
+cudaError_t launch_attend_wide(const AttendArgs &p, int n, int pieces, bool scores, cudaStream_t st);
+
+}  // namespace abra

@@ -1,0 +1,468 @@
+// paged_attention_wide.cu -- the paged attention's kernel for many rows a kv
+// head (several new tokens of a group: verification of drafts, or wide groups),
+// on the 5th-generation tensor cores.
+//
+// With R = group x n_q rows a slot of a kv head costs 8 R D flops (the weights
+// go in twice, below) for 4 D bytes.  At 64 rows that is 128 flops a byte: four
+// times what mma.sync reaches at the HBM's rate, a third of tcgen05's.
+//
+// A CTA takes steps of 128 slots.  Four loader warps copy K and V rows into a
+// ring of stages; thread t of four compute warps stands for slot t.  Per step
+//   S^T[128 slots x N] = K Q^T      (M 128, N rows, K = D)
+//   P^T = 2^(S^T - m), split into two 16-bit values, to shared memory
+//   O^T[D x N] += V^T P^T           (M 128, K = 128 slots, twice)
+// with S^T (two buffers) and O^T in tensor memory, all operands in shared
+// memory without swizzle: 16-byte chunks, chunk c of row r at c * CS + 16 r, CS
+// = 128 rows and 16 bytes more, so that neighbouring chunks of a row, which the
+// loaders write together, fall into different banks.  The same bytes are a
+// K-major operand (K: the chunk walks along D) and an M-major one (V: the chunk
+// is eight elements of D, the rows are the contracted slots).  The next step's
+// scores are issued before this step's softmax where its rows have landed.  For heads of less than 128 the
+// O^T product also takes what lies behind V in shared memory: into rows beyond D
+// of O^T that nobody reads.
+#include "paged_attention.cuh"
+#include "tc_common.cuh"
+
+namespace abra {
+namespace {
+
+constexpr int W_THREADS = 256, W_COMPUTE = 128;  // four compute and four loader warps
+
+template <int D, int N> struct Wide {
+    static constexpr int CHUNKS = D / 8;
+    static constexpr int CS = WIDE_STEP * 16 + 16;      // bytes from chunk to chunk of K, V and P
+    static constexpr int TILE = CHUNKS * CS;            // K or V of a step
+    static constexpr int QCS = N * 16 + 16;             // of Q
+    static constexpr int P_BYTES = N / 8 * CS;          // one of the two 16-bit parts
+    static constexpr int Q_BYTES = CHUNKS * QCS;
+    static constexpr int SMALL = (4 * N + 4 * N + 3 * N) * 4;  // warps' maxima and sums, m, sub, factor
+    static constexpr int FIXED = 2 * P_BYTES + Q_BYTES + SMALL;
+    static constexpr int MOST = 232448 - 1024;          // a CTA's shared memory, less the static part
+    static constexpr int FIT = (MOST - FIXED) / (2 * TILE);
+    static constexpr int STAGES = FIT < 4 ? FIT : 4;
+    static_assert(STAGES >= 2, "the ring needs two stages");
+    // the last V tile is read as 16 chunks whatever D is
+    static constexpr int BEHIND = (16 - CHUNKS) * CS;
+    static constexpr int SMEM = STAGES * 2 * TILE + (FIXED > BEHIND ? FIXED : BEHIND);
+    static_assert(SMEM <= MOST, "shared memory");
+    static constexpr int TMEM = N <= 16 ? 64 : N <= 32 ? 128 : 256;  // S, S, O of N columns each
+};
+
+// Instruction descriptor of kind::f16: fp32 accumulators, operands of type T.
+template <typename T> constexpr uint32_t idesc_f16(int M, int N, bool a_major_m, bool b_major_n) {
+    const uint32_t fmt = Half16<T>::type == ABRA_GGML_F16 ? 0u : 1u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((a_major_m ? 1u : 0u) << 15) | ((b_major_n ? 1u : 0u) << 16) |
+           (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        : "memory");
+}
+// This thread's TMEM lane, 16 columns.
+__device__ __forceinline__ void tmem_ld16(uint32_t at, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const float (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+        "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// This thread's arrival at the barrier when its copies so far have landed.
+__device__ __forceinline__ void copy_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Whether a phase has completed, without waiting for it.
+__device__ __forceinline__ bool mbar_passed(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+// Barrier of the compute warps; true for all if `x` is for one of them.
+__device__ __forceinline__ bool compute_any(bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.aligned.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(x ? 1u : 0u)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void compute_sync() { named_bar_sync(1, W_COMPUTE); }
+
+// Folds v[0 .. N) over the warp's lanes with op; lane l ends with elements l *
+// N / 32 .. (N >= 32), or element l / 2 (N = 16), in v[0 .. max(1, N / 32)).
+template <int N, typename Op> __device__ __forceinline__ void fold_lanes(float (&v)[N], Op op) {
+    const int lane = threadIdx.x & 31;
+    int width = N;
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) {
+        if (width > 1) {
+            width >>= 1;
+            const bool up = lane & d;
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i)
+                if (i < width) {
+                    const float give = up ? v[i] : v[i + width], keep = up ? v[i + width] : v[i];
+                    v[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, d));
+                }
+        } else {
+            v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], d));
+        }
+    }
+}
+// Where fold_lanes leaves element e of lane l.
+template <int N> __device__ __forceinline__ int folded(int lane, int e) { return N >= 32 ? lane * (N / 32) + e : lane >> 1; }
+
+template <typename T, int D, int N, bool SCORES>
+__global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_constant__ AttendArgs p) {
+    using S = Wide<D, N>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES], s_done[2], o_done;
+    __shared__ uint32_t s_tmem;
+    unsigned char *ring = smem;  // [stage][K, V]
+    unsigned char *s_p = smem + S::STAGES * 2 * S::TILE, *s_q = s_p + 2 * S::P_BYTES;
+    float *w_max = reinterpret_cast<float *>(s_q + S::Q_BYTES), *w_sum = w_max + 4 * N;  // [warp][N]
+    float *s_m = w_sum + 4 * N, *s_sub = s_m + N, *s_k = s_sub + N;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+    pdl_launch_dependents();  // the join may take its place; it waits for the whole grid
+    Walk<WIDE_STEP> w;
+    Line line(0, 0);
+    if (!find_start<W_THREADS>(p.kv, p.row_blocks, blockIdx.x, gridDim.x, p.resident, line, w)) return;
+    const int begin = w.pos;
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; ++i) {
+            mbar_init(&full[i], W_COMPUTE);
+            mbar_init(&empty[i], 1);
+        }
+        mbar_init(&s_done[0], 1);
+        mbar_init(&s_done[1], 1);
+        mbar_init(&o_done, 1);
+        fence_mbar_init();
+    }
+    if (warp == 0) {
+        tmem_alloc(&s_tmem, S::TMEM);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    // after a wait that gave up (its error bit is set) nothing waits any more and
+    // every loop runs to its end
+    bool lost = false;
+    auto wait = [&](uint64_t *bar, int parity) {
+        if (!lost && !mbar_wait(bar, parity)) lost = true;
+    };
+
+    if (warp >= 4) {
+        // ---- loaders: 32 rows of a step a warp, a lane answering for one of them ----
+        const int lw = warp - 4;
+        int j = 0;
+        do {
+            for (int t0 = w.s.tile0 * WIDE_STEP; t0 < w.s.slot_end; t0 += WIDE_STEP, ++j) {
+                const int st = j % S::STAGES;
+                const int t = t0 + 32 * lw + lane;
+                int page = 0, off = 0;
+                if (t < w.s.slot_end) {
+                    const int e = p.kv.page.div(t);
+                    off = t - e * p.kv.a.page_size;
+                    page = max(0, paged_page(p.kv, w.s.seq, e));
+                }
+                const int64_t k_off = paged_k_at(p.kv, page, w.s.head, off), v_off = paged_v_at(p.kv, page, w.s.head, off);
+                if (j >= S::STAGES) wait(&empty[st], (j / S::STAGES - 1) & 1);
+                const uint32_t to = smem_u32(ring) + st * 2 * S::TILE;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    const T *pool = static_cast<const T *>(kv ? p.kv.a.v : p.kv.a.k);
+#pragma unroll 8
+                    for (int i = 0; i < S::CHUNKS; ++i) {
+                        const int x = 32 * i + lane, row = x / S::CHUNKS, chunk = x - row * S::CHUNKS;
+                        const T *src = pool + __shfl_sync(0xffffffffu, kv ? v_off : k_off, row) + 8 * chunk;
+                        copy_async(to + kv * S::TILE + chunk * S::CS + (32 * lw + row) * 16, src,
+                                   t0 + 32 * lw + row < w.s.slot_end ? 16 : 0);
+                    }
+                }
+                copy_arrive(&full[st]);
+            }
+        } while (w.next(p.kv));
+        copy_commit();
+        copy_wait<0>();
+    } else {
+        // ---- compute warps: thread t is slot t of a step, and element t of the results ----
+        const uint32_t tmem = s_tmem, mine = tmem + (static_cast<uint32_t>(32 * warp) << 16), t_o = 2 * N;
+        auto desc = [&](const unsigned char *at, uint32_t lbo, uint32_t sbo) { return tc_smem_desc(at, lbo, sbo); };
+        auto issue_scores = [&](int it) {  // thread 0
+            wait(&full[it % S::STAGES], (it / S::STAGES) & 1);
+            fence_proxy_async_smem();  // the loaders' copies, seen through the barrier, before the tensor core's reads
+            tc_fence_after();
+            const unsigned char *k = ring + (it % S::STAGES) * 2 * S::TILE;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+                tc_mma_f16(tmem + (it & 1) * N, desc(k + 2 * ks * S::CS, S::CS, 128), desc(s_q + 2 * ks * S::QCS, S::QCS, 128),
+                           idesc_f16<T>(128, N, false, false), ks > 0);
+            tc_commit(&s_done[it & 1]);
+        };
+        auto issue_sum = [&](int it, bool first) {  // thread 0
+            tc_fence_after();
+            const unsigned char *v = ring + (it % S::STAGES) * 2 * S::TILE + S::TILE;
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+                for (int ks = 0; ks < WIDE_STEP / 16; ++ks)
+                    tc_mma_f16(tmem + t_o, desc(v + ks * 256, 128, S::CS), desc(s_p + part * S::P_BYTES + ks * 256, 128, S::CS),
+                               idesc_f16<T>(128, N, true, true), !first || part > 0 || ks > 0);
+            tc_commit(&empty[it % S::STAGES]);
+            tc_commit(&o_done);
+        };
+        int it = 0;  // steps of this CTA so far
+        do {
+            const Segment &sg = w.s;
+            const int r0 = sg.block * N, head = sg.head;
+            // Q as an operand: rows past the end are zeros
+            for (int x = tid; x < N * S::CHUNKS; x += W_COMPUTE) {
+                const int r = x / S::CHUNKS, chunk = x - r * S::CHUNKS, row = r0 + r;
+                uint4 q = make_uint4(0, 0, 0, 0);
+                if (row < p.rows) {
+                    const int j = row / p.group, h = head * p.group + row - j * p.group;
+                    q = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldq +
+                                                              static_cast<int64_t>(h) * D + 8 * chunk));
+                }
+                *reinterpret_cast<uint4 *>(s_q + chunk * S::QCS + r * 16) = q;
+            }
+            if (tid < N) s_m[tid] = -INFINITY, s_sub[tid] = 0.0f;
+            fence_proxy_async_smem();
+            compute_sync();
+            const int all_see = sg.len - p.n_q + 1;  // slots below are seen by every row
+            float l[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) l[n] = 0.0f;
+            bool odd = false;  // an infinity or NaN among the values of a step that not all rows see
+            if (tid == 0) issue_scores(it);
+            for (int t0 = sg.tile0 * WIDE_STEP; t0 < sg.slot_end; t0 += WIDE_STEP, ++it) {
+                const bool first = t0 == sg.tile0 * WIDE_STEP, edge = t0 + WIDE_STEP > all_see;
+                const int t = t0 + tid;
+                // the next step's scores, if its rows are here; if not, after this step
+                const bool more = t0 + WIDE_STEP < sg.slot_end;
+                bool ahead = false;
+                if (tid == 0 && more && mbar_passed(&full[(it + 1) % S::STAGES], ((it + 1) / S::STAGES) & 1)) {
+                    issue_scores(it + 1);
+                    ahead = true;
+                }
+                // ---- scores in log2 units, masked; is a maximum to be raised? ----
+                wait(&s_done[it & 1], (it >> 1) & 1);
+                tc_fence_after();
+                float s[N];
+                bool raise = false;
+#pragma unroll
+                for (int n0 = 0; n0 < N; n0 += 16) tmem_ld16(mine + (it & 1) * N + n0, *reinterpret_cast<float (*)[16]>(s + n0));
+                tmem_wait_ld();
+#pragma unroll
+                for (int n0 = 0; n0 < N; n0 += 4) {
+                    const float4 m = *reinterpret_cast<const float4 *>(s_m + n0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int n = n0 + i;
+                        s[n] *= p.scale_log2;
+                        if (edge) {
+                            const int see = min(sg.slot_end, all_see + min((r0 + n) / p.group, p.n_q - 1));
+                            if (t >= see) s[n] = -INFINITY;
+                        }
+                        raise |= s[n] > (i == 0 ? m.x : i == 1 ? m.y : i == 2 ? m.z : m.w) + RAISE;
+                    }
+                }
+                if (SCORES && t < sg.slot_end) {
+                    const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, sg.seq, e));
+                    float *to = p.scores + paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size) * (p.row_blocks * N) + r0;
+#pragma unroll
+                    for (int n = 0; n < N; n += 4) *reinterpret_cast<float4 *>(to + n) = make_float4(s[n], s[n + 1], s[n + 2], s[n + 3]);
+                }
+                raise = compute_any(raise);
+                if (it > 0) wait(&o_done, (it - 1) & 1);  // the weights' buffer and the results are at rest
+                tc_fence_after();
+                if (raise) {
+                    float top[N];
+#pragma unroll
+                    for (int n = 0; n < N; ++n) top[n] = s[n];
+                    fold_lanes<N>(top, [](float a, float b) { return fmaxf(a, b); });
+#pragma unroll
+                    for (int e = 0; e < (N >= 32 ? N / 32 : 1); ++e) w_max[warp * N + folded<N>(lane, e)] = top[e];
+                    compute_sync();
+                    if (tid < N) {
+                        const float m = s_m[tid];
+                        const float now = fmaxf(fmaxf(fmaxf(w_max[tid], w_max[N + tid]), fmaxf(w_max[2 * N + tid], w_max[3 * N + tid])), m);
+                        s_k[tid] = scaled(m, now);
+                        s_m[tid] = now;
+                        s_sub[tid] = now == -INFINITY ? 0.0f : now;
+                    }
+                    compute_sync();
+                    if (!first) {
+#pragma unroll
+                        for (int n0 = 0; n0 < N; n0 += 16) {
+                            float o[16];
+                            tmem_ld16(mine + t_o + n0, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                o[i] *= s_k[n0 + i];
+                                l[n0 + i] *= s_k[n0 + i];
+                            }
+                            tmem_st16(mine + t_o + n0, o);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                // A slot that only some rows see has weight 0 in the others, and 0
+                // times an infinity or NaN in its V row would reach them: such
+                // elements count as zeros here and are added at the row's end.
+                if (edge && p.n_q > 1) {
+                    for (int c = 0; c < S::CHUNKS; ++c) {
+                        uint4 *v = reinterpret_cast<uint4 *>(ring + (it % S::STAGES) * 2 * S::TILE + S::TILE + c * S::CS + tid * 16);
+                        bool any = false;
+                        const uint4 x = make_uint4(finite_part<T>(v->x, any), finite_part<T>(v->y, any), finite_part<T>(v->z, any),
+                                                   finite_part<T>(v->w, any));
+                        if (any) *v = x, odd = true;
+                    }
+                }
+                // ---- weights, as the sum of two 16-bit values (one rounding would
+                // cost as much precision as the result's own) ----
+#pragma unroll
+                for (int n0 = 0; n0 < N; n0 += 8) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const int n = n0 + i;
+                        const float2 sub = *reinterpret_cast<const float2 *>(s_sub + n);
+                        const float a = exp2_fast(s[n] - sub.x), b = exp2_fast(s[n + 1] - sub.y);
+                        l[n] += a;
+                        l[n + 1] += b;
+                        hi[i / 2] = pack2<T>(a, b);
+                        const float2 h = unpack2<T>(hi[i / 2]);
+                        lo[i / 2] = pack2<T>(a - h.x, b - h.y);
+                    }
+                    unsigned char *to = s_p + n0 / 8 * S::CS + tid * 16;
+                    *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4 *>(to + S::P_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                tc_fence_before();
+                fence_proxy_async_smem();
+                compute_sync();
+                if (tid == 0) {
+                    issue_sum(it, first);
+                    if (more && !ahead) issue_scores(it + 1);
+                }
+            }
+
+            // ---- the row's end ----
+            fold_lanes<N>(l, [](float a, float b) { return a + b; });
+#pragma unroll
+            for (int e = 0; e < (N >= 32 ? N / 32 : 1); ++e) w_sum[warp * N + folded<N>(lane, e)] = l[e];
+            odd = compute_any(odd);
+            wait(&o_done, (it - 1) & 1);
+            tc_fence_after();
+            const bool whole = sg.tile0 == 0 && sg.tile1 == sg.n;
+            const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (w.pos == begin ? 0 : 1);
+            const int odd_from = max(sg.tile0 * WIDE_STEP, all_see / WIDE_STEP * WIDE_STEP);  // the first step with an edge
+#pragma unroll 1
+            for (int n0 = 0; n0 < N && r0 + n0 < p.rows; n0 += 16) {
+                float o[16];
+                tmem_ld16(mine + t_o + n0, o);
+                tmem_wait_ld();
+                if (odd && tid < D) {
+                    for (int t = odd_from; t < sg.slot_end; ++t) {
+                        const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, sg.seq, e));
+                        const float v = Half16<T>::up(static_cast<const T *>(p.kv.a.v)[paged_v_at(p.kv, page, head, t - e * p.kv.a.page_size) + tid]);
+                        if (isfinite(v)) continue;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (t < all_see + min((r0 + n0 + i) / p.group, p.n_q - 1)) o[i] += v;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int n = n0 + i, r = r0 + n;
+                    if (r >= p.rows) break;
+                    const float total = w_sum[n] + w_sum[N + n] + w_sum[2 * N + n] + w_sum[3 * N + n];
+                    if (!whole) {
+                        if (tid < D) p.part_o[(slot * N + n) * D + tid] = o[i];
+                        if (tid == 0) p.part_ml[slot * N + n] = make_float2(s_m[n], total);
+                    } else {
+                        const int j = r / p.group, h = head * p.group + r - j * p.group;
+                        const int64_t row = static_cast<int64_t>(sg.seq) * p.n_q + j;
+                        if (tid < D) {
+                            const float x = total != 0.0f ? o[i] / total : 0.0f;
+                            const int64_t to = row * p.ldo + static_cast<int64_t>(h) * D + tid;
+                            if (p.out_f32) static_cast<float *>(p.out)[to] = x;
+                            else static_cast<T *>(p.out)[to] = Half16<T>::down(x);
+                        }
+                        if (tid == 0) finish_lse(p, sg.seq, head, r, s_m[n], total);
+                    }
+                }
+            }
+            if (sg.tile0 == 0 && tid == 0)
+                p.split[static_cast<int64_t>(sg.seq) * w.units + sg.unit] =
+                    make_int2(static_cast<int>(slot), whole ? static_cast<int>(blockIdx.x) : line.piece(sg.row_begin + ROW_COST + sg.n - 1));
+            tc_fence_before();
+            compute_sync();  // Q, the sums and the results are free again
+        } while (w.next(p.kv));
+    }
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(s_tmem, S::TMEM);
+}
+
+template <typename T, int D, int N, bool SCORES> cudaError_t launch_one(const AttendArgs &p, int pieces, cudaStream_t st) {
+    constexpr int smem = Wide<D, N>::SMEM;
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = paged_smem(reinterpret_cast<const void *>(attend_wide_kernel<T, D, N, SCORES>), smem, done);
+    if (e != cudaSuccess) return e;
+    attend_wide_kernel<T, D, N, SCORES><<<pieces, W_THREADS, smem, st>>>(p);
+    return cudaGetLastError();
+}
+template <typename T, int D, int N> cudaError_t launch_scores(const AttendArgs &p, int pieces, bool scores, cudaStream_t st) {
+    return scores ? launch_one<T, D, N, true>(p, pieces, st) : launch_one<T, D, N, false>(p, pieces, st);
+}
+template <typename T, int D> cudaError_t launch_rows(const AttendArgs &p, int n, int pieces, bool scores, cudaStream_t st) {
+    return n == 16   ? launch_scores<T, D, 16>(p, pieces, scores, st)
+           : n == 32 ? launch_scores<T, D, 32>(p, pieces, scores, st)
+                     : launch_scores<T, D, 64>(p, pieces, scores, st);
+}
+template <typename T> cudaError_t launch_dim(const AttendArgs &p, int n, int pieces, bool scores, cudaStream_t st) {
+    switch (p.kv.a.head_dim) {
+        case 64: return launch_rows<T, 64>(p, n, pieces, scores, st);
+        case 96: return launch_rows<T, 96>(p, n, pieces, scores, st);
+        default: return launch_rows<T, 128>(p, n, pieces, scores, st);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_attend_wide(const AttendArgs &p, int n, int pieces, bool scores, cudaStream_t st) {
+    return p.kv.a.type == ABRA_GGML_F16 ? launch_dim<__half>(p, n, pieces, scores, st)
+                                        : launch_dim<__nv_bfloat16>(p, n, pieces, scores, st);
+}
+
+}  // namespace abra
+
+ABRA_ERROR_WORD_ACCESSOR(paged_attention_wide_error_word)
