@@ -11,12 +11,11 @@
 //   S^T[128 slots x N] = K Q^T      (M 128, N rows, K = D)
 //   P^T = 2^(S^T - m), split into two 16-bit values, to shared memory
 //   O^T[D x N] += V^T P^T           (M 128, K = 128 slots, twice)
-// with S^T (two buffers) and O^T in tensor memory, all operands in shared
-// memory without swizzle: 16-byte chunks, chunk c of row r at c * CS + 16 r, CS
-// = 128 rows and 16 bytes more, so that neighbouring chunks of a row, which the
-// loaders write together, fall into different banks.  The same bytes are a
-// K-major operand (K: the chunk walks along D) and an M-major one (V: the chunk
-// is eight elements of D, the rows are the contracted slots).  The next step's
+// with S^T (two buffers) and O^T in tensor memory, all operands in shared memory
+// in rows of 128 bytes (64 elements; wider rows in planes) with the 128-byte
+// swizzle: 16-byte chunk c of row r at r * 128 + (c ^ r % 8) * 16.  The same
+// bytes are a K-major operand (K and Q: the chunks walk along D) and an M-major
+// one (V and P: the rows are the contracted slots).  The next step's
 // scores are issued before this step's softmax where its rows have landed.  For heads of less than 128 the
 // O^T product also takes what lies behind V in shared memory: into rows beyond D
 // of O^T that nobody reads.
@@ -26,28 +25,38 @@
 namespace abra {
 namespace {
 
-constexpr int W_THREADS = 256, W_COMPUTE = 128;  // four compute and four loader warps
+constexpr int W_THREADS = 256, W_COMPUTE = 128, W_LOAD = 96;  // four compute warps, three loaders, one for the tensor core
 
 template <int D, int N> struct Wide {
-    static constexpr int CHUNKS = D / 8;
-    static constexpr int CS = WIDE_STEP * 16 + 16;      // bytes from chunk to chunk of K, V and P
-    static constexpr int TILE = CHUNKS * CS;            // K or V of a step
-    static constexpr int QCS = N * 16 + 16;             // of Q
-    static constexpr int P_BYTES = N / 8 * CS;          // one of the two 16-bit parts
-    static constexpr int Q_BYTES = CHUNKS * QCS;
+    static constexpr int CHUNKS = D / 8;                // of 16 bytes in a row
+    static constexpr int PLANES = (D + 63) / 64;
+    static constexpr int PLANE = WIDE_STEP * 128;       // bytes of 64 elements of every slot
+    static constexpr int TILE = PLANES * PLANE;         // K or V of a step
+    static constexpr int P_BYTES = PLANE;               // one of the two 16-bit parts
+    static constexpr int Q_PLANE = N * 128, Q_BYTES = PLANES * Q_PLANE;
     static constexpr int SMALL = (4 * N + 4 * N + 3 * N) * 4;  // warps' maxima and sums, m, sub, factor
     static constexpr int FIXED = 2 * P_BYTES + Q_BYTES + SMALL;
-    static constexpr int MOST = 232448 - 1024;          // a CTA's shared memory, less the static part
-    static constexpr int FIT = (MOST - FIXED) / (2 * TILE);
-    static constexpr int STAGES = FIT < 4 ? FIT : 4;
-    static_assert(STAGES >= 2, "the ring needs two stages");
-    // the last V tile is read as 16 chunks whatever D is
-    static constexpr int BEHIND = (16 - CHUNKS) * CS;
-    static constexpr int SMEM = STAGES * 2 * TILE + (FIXED > BEHIND ? FIXED : BEHIND);
-    static_assert(SMEM <= MOST, "shared memory");
+    static constexpr int MOST = 232448 - 2048;          // a CTA's shared memory, less the static part and the alignment
+    static constexpr int FIT = (MOST - FIXED) / TILE;   // tiles; K's ring gets the odd one
+    static constexpr int VS = FIT / 2 < 4 ? FIT / 2 : 4, KS = FIT - VS < 4 ? FIT - VS : 4;
+    static_assert(VS >= 2, "the rings need two tiles each");
+    // V is read as two planes whatever D is: behind the last one lies P
+    static constexpr int SMEM = 1024 + (KS + VS) * TILE + FIXED;
     static constexpr int TMEM = N <= 16 ? 64 : N <= 32 ? 128 : 256;  // S, S, O of N columns each
 };
 
+// Byte of chunk c of row r in a plane.
+__device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+// Descriptor of an operand with the 128-byte swizzle (layout 2): `lbo` bytes
+// from plane to plane (M-major), 1024 from eight rows to the next eight.
+__device__ __forceinline__ uint64_t desc_swizzled(uint32_t at, uint32_t lbo) {
+    return ((at >> 4) & 0x3FFFull) | (static_cast<uint64_t>(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 // Instruction descriptor of kind::f16: fp32 accumulators, operands of type T.
 template <typename T> constexpr uint32_t idesc_f16(int M, int N, bool a_major_m, bool b_major_n) {
     const uint32_t fmt = Half16<T>::type == ABRA_GGML_F16 ? 0u : 1u;
@@ -139,13 +148,14 @@ template <int N> __device__ __forceinline__ int folded(int lane, int e) { return
 template <typename T, int D, int N, bool SCORES>
 __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_constant__ AttendArgs p) {
     using S = Wide<D, N>;
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES], s_done[2], o_done;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
+    __shared__ __align__(8) uint64_t k_full[S::KS], k_empty[S::KS], v_full[S::VS], v_empty[S::VS], s_done[2], o_done, q_ready, p_ready;
     __shared__ uint32_t s_tmem;
-    unsigned char *ring = smem;  // [stage][K, V]
-    unsigned char *s_p = smem + S::STAGES * 2 * S::TILE, *s_q = s_p + 2 * S::P_BYTES;
+    unsigned char *s_k = smem, *s_v = smem + S::KS * S::TILE;  // rings
+    unsigned char *s_p = s_v + S::VS * S::TILE, *s_q = s_p + 2 * S::P_BYTES;
     float *w_max = reinterpret_cast<float *>(s_q + S::Q_BYTES), *w_sum = w_max + 4 * N;  // [warp][N]
-    float *s_m = w_sum + 4 * N, *s_sub = s_m + N, *s_k = s_sub + N;
+    float *s_m = w_sum + 4 * N, *s_sub = s_m + N, *s_fac = s_sub + N;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     pdl_launch_dependents();  // the join may take its place; it waits for the whole grid
@@ -154,10 +164,10 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
     if (!find_start<W_THREADS>(p.kv, p.row_blocks, blockIdx.x, gridDim.x, p.resident, line, w)) return;
     const int begin = w.pos;
     if (tid == 0) {
-        for (int i = 0; i < S::STAGES; ++i) {
-            mbar_init(&full[i], W_COMPUTE);
-            mbar_init(&empty[i], 1);
-        }
+        for (int i = 0; i < S::KS; ++i) mbar_init(&k_full[i], W_LOAD), mbar_init(&k_empty[i], 1);
+        for (int i = 0; i < S::VS; ++i) mbar_init(&v_full[i], W_LOAD), mbar_init(&v_empty[i], 1);
+        mbar_init(&q_ready, W_COMPUTE);
+        mbar_init(&p_ready, W_COMPUTE);
         mbar_init(&s_done[0], 1);
         mbar_init(&s_done[1], 1);
         mbar_init(&o_done, 1);
@@ -177,66 +187,121 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
         if (!lost && !mbar_wait(bar, parity)) lost = true;
     };
 
-    if (warp >= 4) {
-        // ---- loaders: 32 rows of a step a warp, a lane answering for one of them ----
+    if (warp >= 4 && warp < 7) {
+        // ---- loaders: eight rows of a step at a time, dealt to the three warps; a
+        // lane answers for rows 8 (lw + 3 (l / 8)) + l % 8 and, l < 16, those of
+        // the two groups after the warp's fourth ----
+        constexpr int GROUPS = WIDE_STEP / 8, COPIES = S::CHUNKS / 4;  // of a lane for a group
         const int lw = warp - 4;
         int j = 0;
         do {
             for (int t0 = w.s.tile0 * WIDE_STEP; t0 < w.s.slot_end; t0 += WIDE_STEP, ++j) {
-                const int st = j % S::STAGES;
-                const int t = t0 + 32 * lw + lane;
-                int page = 0, off = 0;
-                if (t < w.s.slot_end) {
-                    const int e = p.kv.page.div(t);
-                    off = t - e * p.kv.a.page_size;
-                    page = max(0, paged_page(p.kv, w.s.seq, e));
+                int64_t off[2][2];  // K, V
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const int t = t0 + 8 * (lw + 3 * (4 * y + (lane >> 3))) + (lane & 7);
+                    int page = 0, in = 0;
+                    if (t < min(w.s.slot_end, t0 + WIDE_STEP)) {
+                        const int e = p.kv.page.div(t);
+                        in = t - e * p.kv.a.page_size;
+                        page = max(0, paged_page(p.kv, w.s.seq, e));
+                    }
+                    off[0][y] = paged_k_at(p.kv, page, w.s.head, in);
+                    off[1][y] = paged_v_at(p.kv, page, w.s.head, in);
                 }
-                const int64_t k_off = paged_k_at(p.kv, page, w.s.head, off), v_off = paged_v_at(p.kv, page, w.s.head, off);
-                if (j >= S::STAGES) wait(&empty[st], (j / S::STAGES - 1) & 1);
-                const uint32_t to = smem_u32(ring) + st * 2 * S::TILE;
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
+                    const int stages = kv ? S::VS : S::KS, st = j % stages;
+                    if (j >= stages) wait(kv ? &v_empty[st] : &k_empty[st], (j / stages - 1) & 1);
+                    const uint32_t to = smem_u32(kv ? s_v : s_k) + st * S::TILE;
                     const T *pool = static_cast<const T *>(kv ? p.kv.a.v : p.kv.a.k);
-#pragma unroll 8
-                    for (int i = 0; i < S::CHUNKS; ++i) {
-                        const int x = 32 * i + lane, row = x / S::CHUNKS, chunk = x - row * S::CHUNKS;
-                        const T *src = pool + __shfl_sync(0xffffffffu, kv ? v_off : k_off, row) + 8 * chunk;
-                        copy_async(to + kv * S::TILE + chunk * S::CS + (32 * lw + row) * 16, src,
-                                   t0 + 32 * lw + row < w.s.slot_end ? 16 : 0);
+#pragma unroll
+                    for (int q = 0; q < (GROUPS + 2) / 3; ++q) {
+                        const int group = lw + 3 * q;
+                        if (group >= GROUPS) break;
+#pragma unroll
+                        for (int i = 0; i < COPIES; ++i) {
+                            const int x = 32 * i + lane, r = x / S::CHUNKS, chunk = x - r * S::CHUNKS, row = 8 * group + r;
+                            const T *src = pool + __shfl_sync(0xffffffffu, off[kv][q / 4], 8 * (q % 4) + r) + 8 * chunk;
+                            copy_async(to + (chunk >> 3) * S::PLANE + swizzled(row, chunk & 7), src, t0 + row < w.s.slot_end ? 16 : 0);
+                        }
                     }
+                    copy_arrive(kv ? &v_full[st] : &k_full[st]);
                 }
-                copy_arrive(&full[st]);
             }
         } while (w.next(p.kv));
         copy_commit();
         copy_wait<0>();
-    } else {
-        // ---- compute warps: thread t is slot t of a step, and element t of the results ----
-        const uint32_t tmem = s_tmem, mine = tmem + (static_cast<uint32_t>(32 * warp) << 16), t_o = 2 * N;
-        auto desc = [&](const unsigned char *at, uint32_t lbo, uint32_t sbo) { return tc_smem_desc(at, lbo, sbo); };
-        auto issue_scores = [&](int it) {  // thread 0
-            wait(&full[it % S::STAGES], (it / S::STAGES) & 1);
+    } else if (warp == 7) {
+        // ---- the tensor core's warp: all lanes run, one issues ----
+        const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0), u_o = tmem + 2 * N;
+        const uint32_t u_k = __shfl_sync(0xffffffffu, smem_u32(s_k), 0), u_v = __shfl_sync(0xffffffffu, smem_u32(s_v), 0);
+        const uint32_t u_p = __shfl_sync(0xffffffffu, smem_u32(s_p), 0), u_q = __shfl_sync(0xffffffffu, smem_u32(s_q), 0);
+        const bool leader = elect_one();
+        auto issue_scores = [&](int it) {
             fence_proxy_async_smem();  // the loaders' copies, seen through the barrier, before the tensor core's reads
             tc_fence_after();
-            const unsigned char *k = ring + (it % S::STAGES) * 2 * S::TILE;
+            const uint32_t k = __shfl_sync(0xffffffffu, u_k + it % S::KS * S::TILE, 0);
+            const uint32_t d = __shfl_sync(0xffffffffu, tmem + (it & 1) * N, 0);
+            if (leader) {
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-                tc_mma_f16(tmem + (it & 1) * N, desc(k + 2 * ks * S::CS, S::CS, 128), desc(s_q + 2 * ks * S::QCS, S::QCS, 128),
-                           idesc_f16<T>(128, N, false, false), ks > 0);
-            tc_commit(&s_done[it & 1]);
+                for (int ks = 0; ks < D / 16; ++ks)
+                    tc_mma_f16(d, desc_swizzled(k + ks / 4 * S::PLANE + ks % 4 * 32, 16),
+                               desc_swizzled(u_q + ks / 4 * S::Q_PLANE + ks % 4 * 32, 16), idesc_f16<T>(128, N, false, false), ks > 0);
+                tc_commit(&k_empty[it % S::KS]);
+                tc_commit(&s_done[it & 1]);
+            }
+            __syncwarp();
         };
-        auto issue_sum = [&](int it, bool first) {  // thread 0
+        auto issue_sum = [&](int it, bool first) {
+            wait(&v_full[it % S::VS], (it / S::VS) & 1);
+            fence_proxy_async_smem();
             tc_fence_after();
-            const unsigned char *v = ring + (it % S::STAGES) * 2 * S::TILE + S::TILE;
+            const uint32_t v = __shfl_sync(0xffffffffu, u_v + it % S::VS * S::TILE, 0);
+            if (leader) {
 #pragma unroll
-            for (int part = 0; part < 2; ++part)
+                for (int part = 0; part < 2; ++part)
 #pragma unroll
-                for (int ks = 0; ks < WIDE_STEP / 16; ++ks)
-                    tc_mma_f16(tmem + t_o, desc(v + ks * 256, 128, S::CS), desc(s_p + part * S::P_BYTES + ks * 256, 128, S::CS),
-                               idesc_f16<T>(128, N, true, true), !first || part > 0 || ks > 0);
-            tc_commit(&empty[it % S::STAGES]);
-            tc_commit(&o_done);
+                    for (int ks = 0; ks < WIDE_STEP / 16; ++ks)
+                        tc_mma_f16(u_o, desc_swizzled(v + ks * 2048, S::PLANE), desc_swizzled(u_p + part * S::P_BYTES + ks * 2048, S::PLANE),
+                                   idesc_f16<T>(128, N, true, true), part > 0 || ks > 0 ? 1u : !first);
+                tc_commit(&v_empty[it % S::VS]);
+                tc_commit(&o_done);
+            }
+            __syncwarp();
         };
+        int it = 0, row = 0;
+        do {
+            const int n = (w.s.slot_end - w.s.tile0 * WIDE_STEP + WIDE_STEP - 1) / WIDE_STEP;
+            wait(&q_ready, row++ & 1);
+            wait(&k_full[it % S::KS], (it / S::KS) & 1);
+            issue_scores(it);
+            for (int k = 0; k < n; ++k, ++it) {
+                // the next step's scores as soon as its keys have landed, this step's
+                // sum as soon as its weights are there
+                bool ahead = k + 1 == n;
+                const uint64_t began = globaltimer_ns();
+                while (!__all_sync(0xffffffffu, lost || mbar_passed(&p_ready, it & 1))) {
+                    if (!ahead && __all_sync(0xffffffffu, lost || mbar_passed(&k_full[(it + 1) % S::KS], ((it + 1) / S::KS) & 1))) {
+                        issue_scores(it + 1);
+                        ahead = true;
+                    }
+                    if (globaltimer_ns() - began > WAIT_LIMIT_NS) {
+                        report_error(ERR_WAIT_TIMEOUT);
+                        lost = true;
+                    }
+                    lost = __any_sync(0xffffffffu, lost);
+                }
+                issue_sum(it, k == 0);
+                if (!ahead) {
+                    wait(&k_full[(it + 1) % S::KS], ((it + 1) / S::KS) & 1);
+                    issue_scores(it + 1);
+                }
+            }
+        } while (w.next(p.kv));
+    } else {
+        // ---- compute warps: thread t is slot t of a step, and element t of the results ----
+        const uint32_t mine = s_tmem + (static_cast<uint32_t>(32 * warp) << 16), t_o = 2 * N;
         int it = 0;  // steps of this CTA so far
         do {
             const Segment &sg = w.s;
@@ -250,27 +315,21 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                     q = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldq +
                                                               static_cast<int64_t>(h) * D + 8 * chunk));
                 }
-                *reinterpret_cast<uint4 *>(s_q + chunk * S::QCS + r * 16) = q;
+                *reinterpret_cast<uint4 *>(s_q + (chunk >> 3) * S::Q_PLANE + swizzled(r, chunk & 7)) = q;
             }
             if (tid < N) s_m[tid] = -INFINITY, s_sub[tid] = 0.0f;
             fence_proxy_async_smem();
+            mbar_arrive(&q_ready);
             compute_sync();
             const int all_see = sg.len - p.n_q + 1;  // slots below are seen by every row
             float l[N];
 #pragma unroll
             for (int n = 0; n < N; ++n) l[n] = 0.0f;
             bool odd = false;  // an infinity or NaN among the values of a step that not all rows see
-            if (tid == 0) issue_scores(it);
+            const int j0 = r0 / p.group, rem0 = r0 - j0 * p.group;  // the query of the block's first row, its head in the group
             for (int t0 = sg.tile0 * WIDE_STEP; t0 < sg.slot_end; t0 += WIDE_STEP, ++it) {
                 const bool first = t0 == sg.tile0 * WIDE_STEP, edge = t0 + WIDE_STEP > all_see;
                 const int t = t0 + tid;
-                // the next step's scores, if its rows are here; if not, after this step
-                const bool more = t0 + WIDE_STEP < sg.slot_end;
-                bool ahead = false;
-                if (tid == 0 && more && mbar_passed(&full[(it + 1) % S::STAGES], ((it + 1) / S::STAGES) & 1)) {
-                    issue_scores(it + 1);
-                    ahead = true;
-                }
                 // ---- scores in log2 units, masked; is a maximum to be raised? ----
                 wait(&s_done[it & 1], (it >> 1) & 1);
                 tc_fence_after();
@@ -279,19 +338,19 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
 #pragma unroll
                 for (int n0 = 0; n0 < N; n0 += 16) tmem_ld16(mine + (it & 1) * N + n0, *reinterpret_cast<float (*)[16]>(s + n0));
                 tmem_wait_ld();
+                if (edge) {
+                    int j = j0, rem = rem0;
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        if (t >= min(sg.slot_end, all_see + min(j, p.n_q - 1))) s[n] = p.scale_log2 < 0.0f ? INFINITY : -INFINITY;
+                        if (++rem == p.group) rem = 0, ++j;
+                    }
+                }
 #pragma unroll
                 for (int n0 = 0; n0 < N; n0 += 4) {
                     const float4 m = *reinterpret_cast<const float4 *>(s_m + n0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int n = n0 + i;
-                        s[n] *= p.scale_log2;
-                        if (edge) {
-                            const int see = min(sg.slot_end, all_see + min((r0 + n) / p.group, p.n_q - 1));
-                            if (t >= see) s[n] = -INFINITY;
-                        }
-                        raise |= s[n] > (i == 0 ? m.x : i == 1 ? m.y : i == 2 ? m.z : m.w) + RAISE;
-                    }
+                    s[n0] *= p.scale_log2, s[n0 + 1] *= p.scale_log2, s[n0 + 2] *= p.scale_log2, s[n0 + 3] *= p.scale_log2;
+                    raise |= s[n0] > m.x + RAISE || s[n0 + 1] > m.y + RAISE || s[n0 + 2] > m.z + RAISE || s[n0 + 3] > m.w + RAISE;
                 }
                 if (SCORES && t < sg.slot_end) {
                     const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, sg.seq, e));
@@ -313,7 +372,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                     if (tid < N) {
                         const float m = s_m[tid];
                         const float now = fmaxf(fmaxf(fmaxf(w_max[tid], w_max[N + tid]), fmaxf(w_max[2 * N + tid], w_max[3 * N + tid])), m);
-                        s_k[tid] = scaled(m, now);
+                        s_fac[tid] = scaled(m, now);
                         s_m[tid] = now;
                         s_sub[tid] = now == -INFINITY ? 0.0f : now;
                     }
@@ -326,8 +385,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                             tmem_wait_ld();
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
-                                o[i] *= s_k[n0 + i];
-                                l[n0 + i] *= s_k[n0 + i];
+                                o[i] *= s_fac[n0 + i];
+                                l[n0 + i] *= s_fac[n0 + i];
                             }
                             tmem_st16(mine + t_o + n0, o);
                         }
@@ -338,8 +397,10 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                 // times an infinity or NaN in its V row would reach them: such
                 // elements count as zeros here and are added at the row's end.
                 if (edge && p.n_q > 1) {
+                    wait(&v_full[it % S::VS], (it / S::VS) & 1);
                     for (int c = 0; c < S::CHUNKS; ++c) {
-                        uint4 *v = reinterpret_cast<uint4 *>(ring + (it % S::STAGES) * 2 * S::TILE + S::TILE + c * S::CS + tid * 16);
+                        uint4 *v = reinterpret_cast<uint4 *>(s_v + it % S::VS * S::TILE + (c >> 3) * S::PLANE +
+                                                             swizzled(tid, c & 7));
                         bool any = false;
                         const uint4 x = make_uint4(finite_part<T>(v->x, any), finite_part<T>(v->y, any), finite_part<T>(v->z, any),
                                                    finite_part<T>(v->w, any));
@@ -362,17 +423,13 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                         const float2 h = unpack2<T>(hi[i / 2]);
                         lo[i / 2] = pack2<T>(a - h.x, b - h.y);
                     }
-                    unsigned char *to = s_p + n0 / 8 * S::CS + tid * 16;
+                    unsigned char *to = s_p + swizzled(tid, n0 / 8);
                     *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *reinterpret_cast<uint4 *>(to + S::P_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 tc_fence_before();
                 fence_proxy_async_smem();
-                compute_sync();
-                if (tid == 0) {
-                    issue_sum(it, first);
-                    if (more && !ahead) issue_scores(it + 1);
-                }
+                mbar_arrive(&p_ready);
             }
 
             // ---- the row's end ----
@@ -380,44 +437,55 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
 #pragma unroll
             for (int e = 0; e < (N >= 32 ? N / 32 : 1); ++e) w_sum[warp * N + folded<N>(lane, e)] = l[e];
             odd = compute_any(odd);
-            wait(&o_done, (it - 1) & 1);
-            tc_fence_after();
             const bool whole = sg.tile0 == 0 && sg.tile1 == sg.n;
             const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (w.pos == begin ? 0 : 1);
+            if (tid < N && r0 + tid < p.rows) {
+                const float total = w_sum[tid] + w_sum[N + tid] + w_sum[2 * N + tid] + w_sum[3 * N + tid];
+                if (whole) finish_lse(p, sg.seq, head, r0 + tid, s_m[tid], total);
+                else p.part_ml[slot * N + tid] = make_float2(s_m[tid], total);
+                s_fac[tid] = total != 0.0f ? 1.0f / total : 0.0f;
+            }
+            compute_sync();
+            wait(&o_done, (it - 1) & 1);
+            tc_fence_after();
             const int odd_from = max(sg.tile0 * WIDE_STEP, all_see / WIDE_STEP * WIDE_STEP);  // the first step with an edge
 #pragma unroll 1
             for (int n0 = 0; n0 < N && r0 + n0 < p.rows; n0 += 16) {
                 float o[16];
                 tmem_ld16(mine + t_o + n0, o);
                 tmem_wait_ld();
-                if (odd && tid < D) {
+                if (tid >= D) continue;
+                if (odd) {
+#pragma unroll 1
                     for (int t = odd_from; t < sg.slot_end; ++t) {
                         const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, sg.seq, e));
                         const float v = Half16<T>::up(static_cast<const T *>(p.kv.a.v)[paged_v_at(p.kv, page, head, t - e * p.kv.a.page_size) + tid]);
                         if (isfinite(v)) continue;
+                        int j = (r0 + n0) / p.group, rem = r0 + n0 - j * p.group;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (t < all_see + min((r0 + n0 + i) / p.group, p.n_q - 1)) o[i] += v;
+                        for (int i = 0; i < 16; ++i) {
+                            if (t < all_see + min(j, p.n_q - 1)) o[i] += v;
+                            if (++rem == p.group) rem = 0, ++j;
+                        }
                     }
                 }
+                const int nr = min(16, p.rows - r0 - n0);
+                if (!whole) {
+                    float *to = p.part_o + (slot * N + n0) * D + tid;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int n = n0 + i, r = r0 + n;
-                    if (r >= p.rows) break;
-                    const float total = w_sum[n] + w_sum[N + n] + w_sum[2 * N + n] + w_sum[3 * N + n];
-                    if (!whole) {
-                        if (tid < D) p.part_o[(slot * N + n) * D + tid] = o[i];
-                        if (tid == 0) p.part_ml[slot * N + n] = make_float2(s_m[n], total);
-                    } else {
-                        const int j = r / p.group, h = head * p.group + r - j * p.group;
-                        const int64_t row = static_cast<int64_t>(sg.seq) * p.n_q + j;
-                        if (tid < D) {
-                            const float x = total != 0.0f ? o[i] / total : 0.0f;
-                            const int64_t to = row * p.ldo + static_cast<int64_t>(h) * D + tid;
+                    for (int i = 0; i < 16; ++i)
+                        if (i < nr) to[i * D] = o[i];
+                } else {
+                    int j = (r0 + n0) / p.group, rem = r0 + n0 - j * p.group;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int64_t to = (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldo + static_cast<int64_t>(head * p.group + rem) * D + tid;
+                        const float x = s_fac[n0 + i] != 0.0f ? o[i] * s_fac[n0 + i] : 0.0f;
+                        if (i < nr) {
                             if (p.out_f32) static_cast<float *>(p.out)[to] = x;
                             else static_cast<T *>(p.out)[to] = Half16<T>::down(x);
                         }
-                        if (tid == 0) finish_lse(p, sg.seq, head, r, s_m[n], total);
+                        if (++rem == p.group) rem = 0, ++j;
                     }
                 }
             }
