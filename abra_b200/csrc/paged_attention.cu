@@ -34,7 +34,7 @@ namespace {
 constexpr int AT_WARPS = 4, AT_THREADS = AT_WARPS * 32;
 constexpr int TILE = 16;               // slots of a warp's tile
 constexpr int STEP = TILE * AT_WARPS;  // slots of a CTA's step
-constexpr int WIDE_FROM = 16;          // more rows a kv head go to the kernel of paged_attention_wide.cu
+constexpr int WIDE_FROM = 8;           // more rows a kv head go to the kernel of paged_attention_wide.cu
 
 // ------------------------------------------------------------------ PTX ---
 template <typename T>
@@ -119,10 +119,11 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
     const bool by8 = p.kv.a.page_size % 8 == 0;
     Walk<STEP> f = w;
     int f_base = f.s.tile0 * STEP + warp * TILE, f_valid = 0;
-    int f_page0 = 0, f_page1 = 0;  // of the halves, or (by8 false) f_page0 of row lane % 16
+    int f_page = 0;  // of half l % 2 of tile f_first + l / 2 (16 tiles at a time), or (by8 false) of row l % 16 of this tile
+    int f_tile = 16;
     uint32_t f_at = ring;
     bool f_more = true;
-    int64_t f_v0 = 0, f_v1 = 0;  // V offsets of the halves' first rows, or f_v0 of row lane % 16
+    int64_t f_v0 = 0, f_v1 = 0;  // V offsets of the halves' first rows, or (by8 false) f_v0 of row lane % 16
     auto page_of = [&](int t) {
         return t < f.s.slot_end
                    ? __ldg(p.kv.a.table + static_cast<int64_t>(f.s.seq) * p.kv.a.table_stride + p.kv.page.div(t))
@@ -133,12 +134,13 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
             f_more = f.next(p.kv);
             if (!f_more) return;
             f_base = f.s.tile0 * STEP + warp * TILE;
+            f_tile = 16;
         }
-        if (by8) {
-            f_page0 = page_of(f_base);
-            f_page1 = page_of(f_base + 8);
-        } else {
-            f_page0 = page_of(f_base + (lane & 15));
+        if (!by8) {
+            f_page = page_of(f_base + (lane & 15));
+        } else if (f_tile == 16) {
+            f_page = page_of(f_base + (lane >> 1) * STEP + 8 * (lane & 1));
+            f_tile = 0;
         }
     };
     auto in_pool = [&](int &page) {
@@ -165,15 +167,18 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
         if (f_more) {
             f_valid = f.s.slot_end - f_base;
             const int t0 = by8 ? f_base : f_base + (lane & 15), off0 = t0 - p.kv.page.div(t0) * p.kv.a.page_size;
-            in_pool(f_page0);
-            const int64_t k0 = paged_k_at(p.kv, f_page0, f.s.head, off0);
-            f_v0 = paged_v_at(p.kv, f_page0, f.s.head, off0);
+            int page0 = by8 ? __shfl_sync(0xffffffffu, f_page, 2 * f_tile) : f_page;
+            in_pool(page0);
+            const int64_t k0 = paged_k_at(p.kv, page0, f.s.head, off0);
+            f_v0 = paged_v_at(p.kv, page0, f.s.head, off0);
             int64_t k1 = 0;
             if (by8) {
                 const int off1 = f_base + 8 - p.kv.page.div(f_base + 8) * p.kv.a.page_size;
-                in_pool(f_page1);
-                k1 = paged_k_at(p.kv, f_page1, f.s.head, off1);
-                f_v1 = paged_v_at(p.kv, f_page1, f.s.head, off1);
+                int page1 = __shfl_sync(0xffffffffu, f_page, 2 * f_tile + 1);
+                in_pool(page1);
+                k1 = paged_k_at(p.kv, page1, f.s.head, off1);
+                f_v1 = paged_v_at(p.kv, page1, f.s.head, off1);
+                ++f_tile;
             }
             copy_tile(static_cast<const T *>(p.kv.a.k), k0, k1, p.kv.a.k_slot_stride, f_at);
         }
@@ -450,48 +455,46 @@ struct Parts {
     __device__ __forceinline__ int64_t place(int i) const { return i ? 2 * (static_cast<int64_t>(first >> 1) + i) : first; }
 };
 
-constexpr int JOIN_WARPS = 8;
+constexpr int JOIN_WARPS = 8, JOIN_THREADS = JOIN_WARPS * 32;
+constexpr int ACC_ROWS = 64;  // rows whose lse is held at a time
 
-// The second kernel: a CTA for each output row.  It writes the rows of empty
-// sequences (zeros) and joins the split ones; the parts are dealt to the warps,
-// which meet in shared memory in a fixed order.
-template <typename T, int D>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ AttendArgs p, int r_block) {
+struct JoinArgs {
+    AttendArgs a;
+    int block;         // rows of a block
+    int warps;         // of an output row: 1, 2, 4 or 8
+    int row_ctas;      // CTAs for the rows of one kv head of a sequence
+    int joins;         // CTAs that join; the others accumulate
+};
+
+// CTA `cta`: JOIN_WARPS / warps output rows.  The parts of a row are dealt to
+// its warps, which meet in shared memory in a fixed order.
+template <typename T, int D> __device__ __forceinline__ void join_rows(const JoinArgs &ja, int cta) {
+    const AttendArgs &p = ja.a;
     __shared__ float s_top[JOIN_WARPS], s_total[JOIN_WARPS];
     __shared__ __align__(16) float s_sum[JOIN_WARPS][D];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int r = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
-    pdl_launch_dependents();
-    pdl_wait();
-    if (paged_len(p.kv, seq) == 0) {
-        if (tid < D / 4) finish_row<T>(p, seq, head, r, 4 * tid, D, make_float4(0, 0, 0, 0), 0.0f, 0.0f);
-        return;
-    }
-    const int block = r / r_block;
-    const Parts parts(__ldcg(p.split + (static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.row_blocks + block));
-    const int n = parts.count();
-    if (n == 1) return;
-    const int rr = r - block * r_block;
-    // this warp's parts: warp, warp + JOIN_WARPS, ..., 32 of them at a time
+    const int group = cta / ja.row_ctas, head = group % p.kv.a.n_kv_heads, seq = group / p.kv.a.n_kv_heads;
+    const int row = warp / ja.warps, part = warp - row * ja.warps;
+    const int r = (cta - group * ja.row_ctas) * (JOIN_WARPS / ja.warps) + row;
+    const bool in = r < p.rows;
+    const int len = paged_len(p.kv, seq), block = in ? r / ja.block : 0, rr = r - block * ja.block;
+    int2 split = make_int2(0, 0);
+    if (len > 0) split = __ldcg(p.split + (static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.row_blocks + block);
+    const Parts parts(split);
+    const int n = in && len > 0 ? parts.count() : 1;  // one part: the row is done
     float top = -INFINITY, total = 0.0f;
     float4 sum = make_float4(0, 0, 0, 0);
-    for (int base = warp; base < n; base += 32 * JOIN_WARPS) {
-        const int mine = base + lane * JOIN_WARPS;
+    // this warp's parts: part, part + warps, ..., 32 of them at a time
+    for (int base = part; n > 1 && base < n; base += 32 * ja.warps) {
+        const int mine = base + lane * ja.warps;
         float2 ml = make_float2(-INFINITY, 0.0f);
-        if (mine < n) ml = __ldcg(p.part_ml + parts.place(mine) * r_block + rr);
-        float t = ml.x;
-#pragma unroll
-        for (int x = 16; x >= 1; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
-        t = fmaxf(t, top);
-        const float keep = scaled(top, t), k = scaled(ml.x, t);
-        top = t;
-        total = total * keep + ml.y * k;  // lane by lane, added up below
-        sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
-        const int left = min(32, (n - base + JOIN_WARPS - 1) / JOIN_WARPS);
+        if (mine < n) ml = __ldcg(p.part_ml + parts.place(mine) * ja.block + rr);
+        const int left = min(32, (n - base + ja.warps - 1) / ja.warps);
         // all parts but the first lie evenly; eight loads in flight a lane
-        const int64_t even = (2 * (static_cast<int64_t>(parts.first >> 1) + base) * r_block + rr) * D;
-        const int64_t odd = base == 0 ? (static_cast<int64_t>(parts.first & 1)) * r_block * D : 0;
+        const int64_t even = (2 * (static_cast<int64_t>(parts.first >> 1) + base) * ja.block + rr) * D;
+        const int64_t odd = base == 0 ? (static_cast<int64_t>(parts.first & 1)) * ja.block * D : 0;
         const float *src = p.part_o + even + 4 * min(lane, D / 4 - 1);
+        float k = 0.0f;
         for (int i0 = 0; i0 < left; i0 += 8) {
             float4 y[8];
 #pragma unroll
@@ -499,53 +502,65 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_cons
                 y[i] = make_float4(0, 0, 0, 0);
                 if (i0 + i < left)
                     y[i] = __ldcg(reinterpret_cast<const float4 *>(src + (i0 + i == 0 ? odd : 0) +
-                                                                   static_cast<int64_t>(i0 + i) * (2 * JOIN_WARPS * D) * r_block));
+                                                                   static_cast<int64_t>(i0 + i) * (2 * D) * ja.warps * ja.block));
+            }
+            if (i0 == 0) {
+                float t = ml.x;
+#pragma unroll
+                for (int x = 16; x >= 1; x >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+                t = fmaxf(t, top);
+                const float keep = scaled(top, t);
+                k = scaled(ml.x, t);
+                top = t;
+                total = total * keep + ml.y * k;  // lane by lane, added up below
+                sum.x *= keep, sum.y *= keep, sum.z *= keep, sum.w *= keep;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float ki = __shfl_sync(0xffffffffu, k, i0 + i);  // 0 beyond the last part
+                const float ki = __shfl_sync(0xffffffffu, k, i0 + i);  // meets zeros beyond the last part
                 sum.x += ki * y[i].x, sum.y += ki * y[i].y, sum.z += ki * y[i].z, sum.w += ki * y[i].w;
             }
         }
     }
 #pragma unroll
     for (int x = 16; x >= 1; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
-    if (lane == 0) s_top[warp] = top, s_total[warp] = total;
-    if (lane < D / 4) *reinterpret_cast<float4 *>(&s_sum[warp][4 * lane]) = sum;
-    __syncthreads();
-    if (tid >= D / 4) return;
-    top = s_top[0];
-    const int used = min(n, JOIN_WARPS);
-    for (int x = 1; x < used; ++x) top = fmaxf(top, s_top[x]);
-    total = 0.0f;
-    sum = make_float4(0, 0, 0, 0);
-    for (int x = 0; x < used; ++x) {
-        const float k = scaled(s_top[x], top);
-        const float4 y = *reinterpret_cast<const float4 *>(&s_sum[x][4 * tid]);
-        total += s_total[x] * k;
-        sum.x += k * y.x, sum.y += k * y.y, sum.z += k * y.z, sum.w += k * y.w;
+    if (ja.warps > 1) {
+        if (lane == 0) s_top[warp] = top, s_total[warp] = total;
+        if (lane < D / 4) *reinterpret_cast<float4 *>(&s_sum[warp][4 * lane]) = sum;
+        __syncthreads();
+        if (part) return;
+        top = s_top[warp];
+        const int used = min(n, ja.warps);
+        for (int x = 1; x < used; ++x) top = fmaxf(top, s_top[warp + x]);
+        total = 0.0f;
+        sum = make_float4(0, 0, 0, 0);
+        for (int x = 0; x < used; ++x) {
+            const float k = scaled(s_top[warp + x], top);
+            const float4 y = *reinterpret_cast<const float4 *>(&s_sum[warp + x][4 * min(lane, D / 4 - 1)]);
+            total += s_total[warp + x] * k;
+            sum.x += k * y.x, sum.y += k * y.y, sum.z += k * y.z, sum.w += k * y.w;
+        }
     }
-    finish_row<T>(p, seq, head, r, 4 * tid, D, sum, top, total);
+    if (in && (n > 1 || len == 0) && lane < D / 4) finish_row<T>(p, seq, head, r, 4 * lane, D, sum, top, total);
 }
 
 // acc += the slots' weights, exp2(score - lse) summed over the rows, on pieces
 // of the same kind of line; two neighbouring lanes share a slot.  A row's lse
 // comes from its parts, so this needs the first kernel only.
-constexpr int ACC_ROWS = 64;  // rows whose lse is held at a time
-__global__ void __launch_bounds__(AT_THREADS) accumulate_kernel(const __grid_constant__ AttendArgs p, int r_block, int padded) {
+__device__ __forceinline__ void accumulate(const JoinArgs &ja, int cta, int ctas) {
+    const AttendArgs &p = ja.a;
     __shared__ float s_lse[ACC_ROWS];
-    const int tid = threadIdx.x, heads = p.kv.a.n_kv_heads, half = tid & 1;
+    const int tid = threadIdx.x, heads = p.kv.a.n_kv_heads, half = tid & 1, padded = p.row_blocks * ja.block;
     Walk<STEP> w;
     Line line(0, 0);
-    pdl_wait();
-    if (!find_start<AT_THREADS>(p.kv, 1, blockIdx.x, gridDim.x, gridDim.x, line, w)) return;
+    if (!find_start<JOIN_THREADS>(p.kv, 1, cta, ctas, ctas, line, w)) return;
     do {
         const Segment &sg = w.s;
         for (int r0 = 0; r0 < p.rows; r0 += ACC_ROWS) {
             const int nr = min(ACC_ROWS, p.rows - r0);
             __syncthreads();
-            for (int i = tid >> 5; i < nr; i += AT_WARPS) {  // a warp a row
-                const int r = r0 + i, block = r / r_block;
+            for (int i = tid >> 5; i < nr; i += JOIN_WARPS) {  // a warp a row
+                const int r = r0 + i, block = r / ja.block;
                 const int64_t triple = (static_cast<int64_t>(sg.seq) * heads + sg.head);
                 const Parts parts(__ldcg(p.split + triple * p.row_blocks + block));
                 const int n = parts.count(), lane = tid & 31;
@@ -555,7 +570,7 @@ __global__ void __launch_bounds__(AT_THREADS) accumulate_kernel(const __grid_con
                 } else {
                     float top = -INFINITY, total = 0.0f;
                     for (int x = lane; x < n; x += 32) {
-                        const float2 ml = __ldcg(p.part_ml + parts.place(x) * r_block + r - block * r_block);
+                        const float2 ml = __ldcg(p.part_ml + parts.place(x) * ja.block + r - block * ja.block);
                         const float t = fmaxf(top, ml.x);
                         total = total * scaled(top, t) + ml.y * scaled(ml.x, t);
                         top = t;
@@ -572,7 +587,7 @@ __global__ void __launch_bounds__(AT_THREADS) accumulate_kernel(const __grid_con
                 if (lane == 0) s_lse[i] = lse == -INFINITY ? INFINITY : lse;  // a row that sees nothing weighs nothing
             }
             __syncthreads();
-            for (int t0 = sg.tile0 * STEP; t0 < sg.slot_end; t0 += AT_THREADS / 2) {
+            for (int t0 = sg.tile0 * STEP; t0 < sg.slot_end; t0 += JOIN_THREADS / 2) {
                 const int t = t0 + (tid >> 1);
                 float sum = 0.0f;
                 int64_t meta = -1;
@@ -596,6 +611,15 @@ __global__ void __launch_bounds__(AT_THREADS) accumulate_kernel(const __grid_con
     } while (w.next(p.kv));
 }
 
+// The second kernel: it writes the rows of empty sequences (zeros), joins the
+// rows that were split, and adds the slots' weights, side by side.
+template <typename T, int D> __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ JoinArgs ja) {
+    pdl_wait();
+    const int cta = blockIdx.x;
+    if (cta < ja.joins) join_rows<T, D>(ja, cta);
+    else accumulate(ja, cta - ja.joins, gridDim.x - ja.joins);
+}
+
 // ------------------------------------------------------------------ host ---
 struct Plan {
     int wide, block, row_blocks, resident, pieces, sms;  // block: rows of a block
@@ -612,7 +636,7 @@ int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumu
     const int64_t triples = static_cast<int64_t>(kv->n_seqs) * kv->n_kv_heads * pl.row_blocks;
     const int step = pl.wide ? WIDE_STEP : STEP;
     const int64_t steps = (static_cast<int64_t>(kv->max_pages) * kv->page_size + step - 1) / step + ROW_COST;
-    if (steps * triples > 0x7fffffff) return paged_fail(ABRA_E_UNSUPPORTED, "the tables name over 2^31 steps of %d slots", step);
+    if (steps * triples > 0x7fffffff || static_cast<int64_t>(kv->n_seqs) * n_heads * n_q > 0x3fffffff) return paged_fail(ABRA_E_UNSUPPORTED, "the tables name over 2^31 steps of %d slots", step);
     pl.resident = pl.sms * (pl.wide ? 1 : pl.block == 8 ? 3 : 2);
     pl.pieces = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(pl.resident) * WAVES, steps * triples));
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
@@ -661,10 +685,13 @@ template <typename T, int D> cudaError_t launch_all(const AttendArgs &p, const P
     cudaError_t e = pl.wide ? launch_attend_wide(p, pl.block, pl.pieces, accumulate, st)
                     : accumulate ? launch_rows<T, D, true>(p, pl, st) : launch_rows<T, D, false>(p, pl, st);
     if (e != cudaSuccess) return e;
-    const int r_block = pl.block;
-    e = launch_after(join_kernel<T, D>, dim3(p.rows, p.kv.a.n_kv_heads, p.kv.a.n_seqs), JOIN_WARPS * 32, st, p, r_block);
-    if (e != cudaSuccess || !accumulate) return e;
-    return launch_after(accumulate_kernel, dim3(pl.sms * 8), AT_THREADS, st, p, r_block, pl.row_blocks * r_block);
+    // as many warps a row as keep four CTAs' worth on every multiprocessor
+    const int64_t groups = static_cast<int64_t>(p.kv.a.n_seqs) * p.kv.a.n_kv_heads;
+    int warps = JOIN_WARPS;
+    while (warps > 1 && groups * p.rows * warps > pl.sms * 4 * JOIN_WARPS) warps /= 2;
+    const int per = JOIN_WARPS / warps, row_ctas = (p.rows + per - 1) / per;
+    const JoinArgs ja{p, pl.block, warps, row_ctas, static_cast<int>(groups * row_ctas)};
+    return launch_after(join_kernel<T, D>, dim3(ja.joins + (accumulate ? pl.sms * 4 : 0)), JOIN_THREADS, st, ja);
 }
 template <typename T> cudaError_t launch(const AttendArgs &p, const Plan &pl, bool accumulate, cudaStream_t st) {
     switch (p.kv.a.head_dim) {
