@@ -21,9 +21,7 @@
 // = V^T P^T, so that a group of four heads wastes half a tile and not three
 // quarters.  Each warp has a ring of tiles of its own in shared memory, filled
 // by asynchronous 16-byte copies (zeros past the end) that run ahead across the
-// ends of the rows; no warp waits for another before a row ends.  Rows in the
-// ring are padded by 16 bytes, so the eight rows of an ldmatrix lie in distinct
-// banks.
+// ends of the rows; no warp waits for another before a row ends.
 #include <algorithm>
 
 #include "paged_attention.cuh"
@@ -34,7 +32,6 @@ namespace {
 constexpr int AT_WARPS = 4, AT_THREADS = AT_WARPS * 32;
 constexpr int TILE = 16;               // slots of a warp's tile
 constexpr int STEP = TILE * AT_WARPS;  // slots of a CTA's step
-constexpr int WIDE_FROM = 8;           // more rows a kv head go to the kernel of paged_attention_wide.cu
 
 // ------------------------------------------------------------------ PTX ---
 template <typename T>
@@ -78,31 +75,36 @@ __device__ __forceinline__ uint32_t trans8x8(uint32_t a) {
     return d;
 }
 // --------------------------------------------------------------- kernel ---
-template <int D, int NT> struct Shape {
+constexpr int ROWS = 8;   // of a block
+constexpr int CTAS = 3;   // on a multiprocessor
+template <int D> struct Shape {
     static constexpr int KS = D / 16;           // k-steps of the scores, and 16-element tiles of the output
-    static constexpr int R = 8 * NT;            // rows of a block
-    static constexpr int ROW = 2 * D + 16;      // bytes of a row in the ring
     static constexpr int CHUNKS = D / 8;        // 16-byte chunks of a row
     static constexpr int COPIES = CHUNKS / 2;   // of a lane for a tile of 16 rows
-    static constexpr int TILE_BYTES = TILE * ROW;            // K or V of one tile
-    static constexpr int STAGE = AT_WARPS * 2 * TILE_BYTES;  // the CTA's K and V tiles
-    static constexpr int PITCH = D + 4;         // floats of a row in the join buffer
-    static constexpr int Q_BYTES = NT == 1 ? 0 : NT * KS * 32 * 8;
-    static constexpr int JOIN_BYTES = R * PITCH * 4 + 2 * AT_WARPS * R * 4;
-    static constexpr int CTAS = NT == 1 ? 3 : 2;  // on a multiprocessor
-    // the ring: as many tiles as leave room for them (1 KB each is the system's)
-    static constexpr int DEPTH = (233472 / CTAS - 1024 - 128 - Q_BYTES - JOIN_BYTES) / STAGE;
-    static constexpr int SMEM = DEPTH * STAGE + Q_BYTES + JOIN_BYTES;
+    // A row's chunk c lies at c ^ (row % 8), where the chunks are 8 or 16; rows
+    // of 12 are padded by one instead.  Either way the eight rows of an ldmatrix
+    // lie in distinct banks.
+    static constexpr bool SWIZZLE = D != 96;
+    static constexpr int ROW = SWIZZLE ? 2 * D : 2 * D + 16;  // bytes of a row in the ring
+    static constexpr int TILE_BYTES = TILE * ROW;             // K or V of one tile
+    static constexpr int STAGE = AT_WARPS * 2 * TILE_BYTES;   // the CTA's K and V tiles
+    static constexpr int PITCH = D + 4;                       // floats of a row in a join buffer
+    static constexpr int JOIN_BYTES = 2 * ROWS * PITCH * 4 + 2 * AT_WARPS * ROWS * 4;
+    // the ring: as many tiles as leave room for the CTAs (1 KB each is the system's)
+    static constexpr int DEPTH = (233472 / CTAS - 1024 - 256 - JOIN_BYTES) / STAGE;
+    static constexpr int SMEM = DEPTH * STAGE + JOIN_BYTES;
     static_assert(DEPTH >= 2, "the ring needs two tiles");
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * ROW + ((SWIZZLE ? chunk ^ (row & 7) : chunk) << 4); }
+    // `bytes` (a multiple of 32) along a row from the chunk at `a`, an even chunk or the one behind it
+    static __device__ __forceinline__ uint32_t along(uint32_t a, int bytes) { return SWIZZLE ? a ^ bytes : a + bytes; }
 };
 
-template <typename T, int D, int NT, bool SCORES>
-__global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kernel(const __grid_constant__ AttendArgs p) {
-    using S = Shape<D, NT>;
-    extern __shared__ __align__(16) unsigned char smem[];  // the ring: [warp][stage][K, V][row]
-    uint2 *s_q = reinterpret_cast<uint2 *>(smem + S::DEPTH * S::STAGE);  // [NT][KS][lane] Q fragments (NT > 1)
-    float *s_o = reinterpret_cast<float *>(smem + S::DEPTH * S::STAGE + S::Q_BYTES);  // [R][PITCH]
-    float *s_m = s_o + S::R * S::PITCH, *s_l = s_m + AT_WARPS * S::R;  // [warp][R]
+template <typename T, int D, bool SCORES>
+__global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_constant__ AttendArgs p) {
+    using S = Shape<D>;
+    extern __shared__ __align__(256) unsigned char smem[];  // the ring: [warp][stage][K, V][row]
+    float *s_o = reinterpret_cast<float *>(smem + S::DEPTH * S::STAGE);  // [2][ROWS][PITCH]
+    float *s_m = s_o + 2 * ROWS * S::PITCH, *s_l = s_m + AT_WARPS * ROWS;  // [warp][ROWS]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
 
     pdl_launch_dependents();  // the join may take its place; it waits for the whole grid
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
                 src = (2 * i < S::COPIES ? src0 : src1) + (row & 7) * stride;
             else
                 src = pool + __shfl_sync(0xffffffffu, off0, row);
-            copy_async(to + row * S::ROW + chunk * 16, src + chunk * 8, row < f_valid ? 16 : 0);
+            copy_async(to + S::at(row, chunk), src + chunk * 8, row < f_valid ? 16 : 0);
         }
     };
     auto fetch_k = [&]() {
@@ -203,65 +205,49 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
     // this lane's row of an ldmatrix: K's matrices are (slots 0-7, 8-15) x
     // (elements 0-7, 8-15) in the order of an A fragment; V's are transposed, so
     // slots and elements change places
-    const uint32_t k_lane = (lane & 15) * S::ROW + (lane >> 4) * 16;
-    const uint32_t v_lane = S::TILE_BYTES + ((lane & 7) + (lane >> 4) * 8) * S::ROW + ((lane >> 3) & 1) * 16;
+    const uint32_t k_lane = S::at(lane & 15, lane >> 4);
+    const uint32_t v_lane = S::TILE_BYTES + S::at((lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1);
     uint32_t at = ring;
 
     do {
         const Segment &sg = w.s;
-        const int head = sg.head, r0 = sg.block * S::R;
+        const int head = sg.head;
 
-        // Q fragments: row r0 + 8 nt + g, elements 16 ks + 2 c and + 8; rows past the end are zeros
-        uint2 qf[NT == 1 ? S::KS : 1];
-        auto load_q = [&](int nt, int ks) {
-            const int r = r0 + 8 * nt + g;
-            if (r >= p.rows) return make_uint2(0, 0);
-            const int j = r / p.group, h = head * p.group + r - j * p.group;
-            const T *q = static_cast<const T *>(p.q) + (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldq + static_cast<int64_t>(h) * D +
-                         16 * ks + 2 * c;
-            return make_uint2(__ldg(reinterpret_cast<const unsigned *>(q)), __ldg(reinterpret_cast<const unsigned *>(q + 8)));
-        };
-        if (NT == 1) {
+        // Q fragments: row g, elements 16 ks + 2 c and + 8; rows past the end are zeros
+        uint2 qf[S::KS];
+        {
+            const int j = min(g, p.rows - 1) / p.group, h = head * p.group + g - j * p.group;
+            const T *q = static_cast<const T *>(p.q) + (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldq + static_cast<int64_t>(h) * D + 2 * c;
 #pragma unroll
-            for (int ks = 0; ks < S::KS; ++ks) qf[NT == 1 ? ks : 0] = load_q(0, ks);
-        } else {
-            for (int x = warp; x < NT * S::KS; x += AT_WARPS) s_q[x * 32 + lane] = load_q(x / S::KS, x % S::KS);
-            __syncthreads();
+            for (int ks = 0; ks < S::KS; ++ks)
+                qf[ks] = g < p.rows ? make_uint2(__ldg(reinterpret_cast<const unsigned *>(q + 16 * ks)),
+                                                 __ldg(reinterpret_cast<const unsigned *>(q + 16 * ks + 8)))
+                                    : make_uint2(0, 0);
         }
-        // slots below are seen by every row; row 8 nt + 2 c + e sees `seen` of them
+        // slots below are seen by every row; row 2 c + e sees `seen` of them
         const int all_see = sg.len - p.n_q + 1;
-        auto seen = [&](int nt, int e) { return all_see + min((r0 + 8 * nt + 2 * c + e) / p.group, p.n_q - 1); };
+        auto seen = [&](int e) { return all_see + min((2 * c + e) / p.group, p.n_q - 1); };
 
         // running maximum m of each row (and 0 in its place while it is -infinity), sum, result
-        float o[NT][S::KS][4], m[NT][2], sub[NT][2], l[NT][2];
+        float o[S::KS][4], m[2], sub[2], l[2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int mt = 0; mt < S::KS; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
-            m[nt][0] = m[nt][1] = -INFINITY;
-            sub[nt][0] = sub[nt][1] = l[nt][0] = l[nt][1] = 0.0f;
-        }
+        for (int mt = 0; mt < S::KS; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.0f;
+        m[0] = m[1] = -INFINITY;
+        sub[0] = sub[1] = l[0] = l[1] = 0.0f;
 
         for (int base = sg.tile0 * STEP + warp * TILE; base < sg.slot_end; base += STEP) {
-            // scores: slots g, g + 8 of the tile by rows 2c, 2c + 1 of each block of
-            // eight; a lone block gets two sums, for two chains of half the length
-            constexpr int CH = NT == 1 ? 2 : 1;
-            float sc[NT][4], part[CH][NT][4];
+            // scores: slots g, g + 8 of the tile by rows 2c, 2c + 1; two sums, for
+            // two chains of half the length
+            float sc[4], part[2][4];
 #pragma unroll
-            for (int x = 0; x < CH; ++x)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) part[x][nt][0] = part[x][nt][1] = part[x][nt][2] = part[x][nt][3] = 0.0f;
+            for (int x = 0; x < 2; ++x) part[x][0] = part[x][1] = part[x][2] = part[x][3] = 0.0f;
             copy_wait<2 * S::DEPTH - 1>();
             __syncwarp();
 #pragma unroll
             for (int ks = 0; ks < S::KS; ++ks) {
                 uint32_t a[4];
-                ldm(a, at + k_lane + ks * 32);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const uint2 q = NT == 1 ? qf[NT == 1 ? ks : 0] : s_q[(nt * S::KS + ks) * 32 + lane];
-                    mma_16x8x16<T>(part[ks % CH][nt], a[0], a[1], a[2], a[3], q.x, q.y);
-                }
+                ldm(a, S::along(at + k_lane, ks * 32));
+                mma_16x8x16<T>(part[ks & 1], a[0], a[1], a[2], a[3], qf[ks].x, qf[ks].y);
             }
             __syncwarp();
             fetch_k();  // into the tile just read
@@ -269,29 +255,25 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
             const bool edge = base + TILE > all_see;
             bool raise = false;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sc[nt][e] = (CH == 2 ? part[0][nt][e] + part[CH - 1][nt][e] : part[0][nt][e]) * p.scale_log2;
-                    if (edge && base + g + 8 * (e >> 1) >= seen(nt, e & 1)) sc[nt][e] = -INFINITY;
-                    raise |= sc[nt][e] > m[nt][e & 1] + RAISE;
-                }
+            for (int e = 0; e < 4; ++e) {
+                sc[e] = (part[0][e] + part[1][e]) * p.scale_log2;
+                if (edge && base + g + 8 * (e >> 1) >= seen(e & 1)) sc[e] = -INFINITY;
+                raise |= sc[e] > m[e & 1] + RAISE;
+            }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int e = 0; e < 2; ++e) {
+                    float top = fmaxf(sc[e], sc[e + 2]);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(sc[nt][e], sc[nt][e + 2]);
+                    for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    top = fmaxf(top, m[e]);
+                    const float k = scaled(m[e], top);
+                    m[e] = top;
+                    sub[e] = top == -INFINITY ? 0.0f : top;
+                    l[e] *= k;
 #pragma unroll
-                        for (int x = 4; x <= 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                        top = fmaxf(top, m[nt][e]);
-                        const float k = scaled(m[nt][e], top);
-                        m[nt][e] = top;
-                        sub[nt][e] = top == -INFINITY ? 0.0f : top;
-                        l[nt][e] *= k;
-#pragma unroll
-                        for (int mt = 0; mt < S::KS; ++mt) o[nt][mt][e] *= k, o[nt][mt][e + 2] *= k;
-                    }
+                    for (int mt = 0; mt < S::KS; ++mt) o[mt][e] *= k, o[mt][e + 2] *= k;
+                }
             }
             if (SCORES) {
 #pragma unroll
@@ -299,31 +281,26 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
                     const int t = base + g + 8 * x, e = p.kv.page.div(t);
                     if (t < sg.slot_end) {
                         const int page = max(0, paged_page(p.kv, sg.seq, e));
-                        float *to = p.scores + paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size) * (p.row_blocks * S::R) + r0;
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            *reinterpret_cast<float2 *>(to + 8 * nt + 2 * c) = make_float2(sc[nt][2 * x], sc[nt][2 * x + 1]);
+                        float *to = p.scores + paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size) * ROWS;
+                        *reinterpret_cast<float2 *>(to + 2 * c) = make_float2(sc[2 * x], sc[2 * x + 1]);
                     }
                 }
             }
             // weights, as the sum of two 16-bit values: the tensor cores take
             // 16-bit operands, and one rounding would cost as much precision
             // as the result's own
-            uint32_t hi[NT][2], lo[NT][2];
+            uint32_t hi[2], lo[2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int e = 0; e < 4; ++e) {
+                sc[e] = exp2_fast(sc[e] - sub[e & 1]);
+                l[e & 1] += sc[e];
+            }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sc[nt][e] = exp2_fast(sc[nt][e] - sub[nt][e & 1]);
-                    l[nt][e & 1] += sc[nt][e];
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const uint32_t h = pack2<T>(sc[nt][2 * x], sc[nt][2 * x + 1]);
-                    const float2 r = unpack2<T>(h);
-                    hi[nt][x] = trans8x8(h);
-                    lo[nt][x] = trans8x8(pack2<T>(sc[nt][2 * x] - r.x, sc[nt][2 * x + 1] - r.y));
-                }
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t h = pack2<T>(sc[2 * x], sc[2 * x + 1]);
+                const float2 r = unpack2<T>(h);
+                hi[x] = trans8x8(h);
+                lo[x] = trans8x8(pack2<T>(sc[2 * x] - r.x, sc[2 * x + 1] - r.y));
             }
             copy_wait<2 * S::DEPTH - 1>();
             __syncwarp();
@@ -335,7 +312,7 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
 #pragma unroll 1
                 for (int i = 0; i < S::COPIES; ++i) {
                     const int x = 32 * i + lane, row = x / S::CHUNKS, chunk = x - row * S::CHUNKS;
-                    uint4 *v = reinterpret_cast<uint4 *>(smem + (at - smem_u32(smem)) + S::TILE_BYTES + row * S::ROW + chunk * 16);
+                    uint4 *v = reinterpret_cast<uint4 *>(smem + (at - smem_u32(smem)) + S::TILE_BYTES + S::at(row, chunk));
                     bool any = false;
                     const uint4 y = make_uint4(finite_part<T>(v->x, any), finite_part<T>(v->y, any), finite_part<T>(v->z, any),
                                                finite_part<T>(v->w, any));
@@ -347,12 +324,9 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
 #pragma unroll
             for (int mt = 0; mt < S::KS; ++mt) {
                 uint32_t a[4];
-                ldm_trans(a, at + v_lane + mt * 32);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    mma_16x8x16<T>(o[nt][mt], a[0], a[1], a[2], a[3], hi[nt][0], hi[nt][1]);
-                    mma_16x8x16<T>(o[nt][mt], a[0], a[1], a[2], a[3], lo[nt][0], lo[nt][1]);
-                }
+                ldm_trans(a, S::along(at + v_lane, mt * 32));
+                mma_16x8x16<T>(o[mt], a[0], a[1], a[2], a[3], hi[0], hi[1]);
+                mma_16x8x16<T>(o[mt], a[0], a[1], a[2], a[3], lo[0], lo[1]);
             }
             __syncwarp();
             fetch_v();
@@ -364,85 +338,77 @@ __global__ void __launch_bounds__(AT_THREADS, (Shape<D, NT>::CTAS)) attend_kerne
                     const T *src = static_cast<const T *>(p.kv.a.v) +
                                    paged_v_at(p.kv, page, head, base + t - e * p.kv.a.page_size) + g;
                     const int from = (t & 7) * 4 + c;
+                    const float w0 = __shfl_sync(0xffffffffu, t < 8 ? sc[0] : sc[2], from);
+                    const float w1 = __shfl_sync(0xffffffffu, t < 8 ? sc[1] : sc[3], from);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const float w0 = __shfl_sync(0xffffffffu, t < 8 ? sc[nt][0] : sc[nt][2], from);
-                        const float w1 = __shfl_sync(0xffffffffu, t < 8 ? sc[nt][1] : sc[nt][3], from);
+                    for (int mt = 0; mt < S::KS; ++mt)
 #pragma unroll
-                        for (int mt = 0; mt < S::KS; ++mt)
-#pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                const float v = Half16<T>::up(src[16 * mt + 8 * y]);
-                                if (isfinite(v)) continue;
-                                if (base + t < seen(nt, 0)) o[nt][mt][2 * y] += w0 * v;
-                                if (base + t < seen(nt, 1)) o[nt][mt][2 * y + 1] += w1 * v;
-                            }
-                    }
+                        for (int y = 0; y < 2; ++y) {
+                            const float v = Half16<T>::up(src[16 * mt + 8 * y]);
+                            if (isfinite(v)) continue;
+                            if (base + t < seen(0)) o[mt][2 * y] += w0 * v;
+                            if (base + t < seen(1)) o[mt][2 * y + 1] += w1 * v;
+                        }
                 }
             }
         }
 
-        // ---- join the warps: maxima, then the scaled sums, one warp after another ----
+        // ---- join the warps: maxima, then the scaled sums, two warps after two ----
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                for (int x = 4; x <= 16; x <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], x);
-                if (g == 0) {
-                    s_m[warp * S::R + 8 * nt + 2 * c + e] = m[nt][e];
-                    s_l[warp * S::R + 8 * nt + 2 * c + e] = l[nt][e];
-                }
-            }
+            for (int x = 4; x <= 16; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+            if (g == 0) s_m[warp * ROWS + 2 * c + e] = m[e], s_l[warp * ROWS + 2 * c + e] = l[e];
+        }
         __syncthreads();
         auto top_of = [&](int r) {
             float top = s_m[r];
 #pragma unroll
-            for (int x = 1; x < AT_WARPS; ++x) top = fmaxf(top, s_m[x * S::R + r]);
+            for (int x = 1; x < AT_WARPS; ++x) top = fmaxf(top, s_m[x * ROWS + r]);
             return top;
         };
 #pragma unroll 1
-        for (int turn = 0; turn < AT_WARPS; ++turn) {
-            if (warp == turn) {
+        for (int turn = 0; turn < AT_WARPS / 2; ++turn) {
+            if (warp >> 1 == turn) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int e = 0; e < 2; ++e) {
+                    const int r = 2 * c + e;
+                    const float k = scaled(m[e], top_of(r));
+                    float *dst = s_o + ((warp & 1) * ROWS + r) * S::PITCH + g;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int r = 8 * nt + 2 * c + e;
-                        const float k = scaled(m[nt][e], top_of(r));
-                        float *dst = s_o + r * S::PITCH + g;
+                    for (int mt = 0; mt < S::KS; ++mt)
 #pragma unroll
-                        for (int mt = 0; mt < S::KS; ++mt)
-#pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                const float x = o[nt][mt][e + 2 * y] * k;
-                                dst[16 * mt + 8 * y] = turn ? dst[16 * mt + 8 * y] + x : x;
-                            }
-                    }
+                        for (int y = 0; y < 2; ++y) {
+                            const float x = o[mt][e + 2 * y] * k;
+                            dst[16 * mt + 8 * y] = turn ? dst[16 * mt + 8 * y] + x : x;
+                        }
+                }
             }
             __syncthreads();
         }
         const bool whole = sg.tile0 == 0 && sg.tile1 == sg.n;
         const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (w.pos == begin ? 0 : 1);
-        for (int i = tid; i < S::R * (D / 4); i += AT_THREADS) {
+        for (int i = tid; i < ROWS * (D / 4); i += AT_THREADS) {
             const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-            if (r0 + r >= p.rows) break;
+            if (r >= p.rows) break;
             const float top = top_of(r);
             float total = 0.0f;
 #pragma unroll
-            for (int x = 0; x < AT_WARPS; ++x) total += s_l[x * S::R + r] * scaled(s_m[x * S::R + r], top);
-            const float4 sum = *reinterpret_cast<const float4 *>(s_o + r * S::PITCH + d);
+            for (int x = 0; x < AT_WARPS; ++x) total += s_l[x * ROWS + r] * scaled(s_m[x * ROWS + r], top);
+            float4 sum = *reinterpret_cast<const float4 *>(s_o + r * S::PITCH + d);
+            const float4 y = *reinterpret_cast<const float4 *>(s_o + (ROWS + r) * S::PITCH + d);
+            sum.x += y.x, sum.y += y.y, sum.z += y.z, sum.w += y.w;
             if (whole) {
-                finish_row<T>(p, sg.seq, head, r0 + r, d, D, sum, top, total);
+                finish_row<T>(p, sg.seq, head, r, d, D, sum, top, total);
             } else {
-                *reinterpret_cast<float4 *>(p.part_o + (slot * S::R + r) * D + d) = sum;
-                if (d == 0) p.part_ml[slot * S::R + r] = make_float2(top, total);
+                *reinterpret_cast<float4 *>(p.part_o + (slot * ROWS + r) * D + d) = sum;
+                if (d == 0) p.part_ml[slot * ROWS + r] = make_float2(top, total);
             }
         }
         if (sg.tile0 == 0 && tid == 0)
             p.split[static_cast<int64_t>(sg.seq) * w.units + sg.unit] =
                 make_int2(static_cast<int>(slot), whole ? static_cast<int>(blockIdx.x) : line.piece(sg.row_begin + ROW_COST + sg.n - 1));
-        __syncthreads();  // the join buffer and Q are free again
+        __syncthreads();  // the join buffers are free again
     } while (w.next(p.kv));
 }
 
@@ -630,14 +596,14 @@ struct Plan {
 int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumulate, Plan &pl) {
     pl.sms = device_sm_count();
     const int rows = n_heads / kv->n_kv_heads * n_q;
-    pl.wide = rows > WIDE_FROM;
-    pl.block = pl.wide ? (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) : rows <= 8 ? 8 : 16;
+    pl.wide = rows > ROWS;
+    pl.block = !pl.wide ? ROWS : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     pl.row_blocks = (rows + pl.block - 1) / pl.block;
     const int64_t triples = static_cast<int64_t>(kv->n_seqs) * kv->n_kv_heads * pl.row_blocks;
     const int step = pl.wide ? WIDE_STEP : STEP;
     const int64_t steps = (static_cast<int64_t>(kv->max_pages) * kv->page_size + step - 1) / step + ROW_COST;
     if (steps * triples > 0x7fffffff || static_cast<int64_t>(kv->n_seqs) * n_heads * n_q > 0x3fffffff) return paged_fail(ABRA_E_UNSUPPORTED, "the tables name over 2^31 steps of %d slots", step);
-    pl.resident = pl.sms * (pl.wide ? 1 : pl.block == 8 ? 3 : 2);
+    pl.resident = pl.sms * (pl.wide ? 1 : CTAS);
     pl.pieces = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(pl.resident) * WAVES, steps * triples));
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     int64_t at = 0;
@@ -654,18 +620,13 @@ int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumu
     return ABRA_OK;
 }
 
-template <typename T, int D, int NT, bool SCORES>
-cudaError_t launch_one(const AttendArgs &p, const Plan &pl, cudaStream_t st) {
-    constexpr int smem = Shape<D, NT>::SMEM;
+template <typename T, int D, bool SCORES> cudaError_t launch_narrow(const AttendArgs &p, const Plan &pl, cudaStream_t st) {
+    constexpr int smem = Shape<D>::SMEM;
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = paged_smem(reinterpret_cast<const void *>(attend_kernel<T, D, NT, SCORES>), smem, done);
+    const cudaError_t e = paged_smem(reinterpret_cast<const void *>(attend_kernel<T, D, SCORES>), smem, done);
     if (e != cudaSuccess) return e;
-    attend_kernel<T, D, NT, SCORES><<<pl.pieces, AT_THREADS, smem, st>>>(p);
+    attend_kernel<T, D, SCORES><<<pl.pieces, AT_THREADS, smem, st>>>(p);
     return cudaGetLastError();
-}
-template <typename T, int D, bool SCORES>
-cudaError_t launch_rows(const AttendArgs &p, const Plan &pl, cudaStream_t st) {
-    return pl.block == 8 ? launch_one<T, D, 1, SCORES>(p, pl, st) : launch_one<T, D, 2, SCORES>(p, pl, st);
 }
 // A launch that may begin before the kernel in front of it has ended (its
 // pdl_wait waits for that).
@@ -683,7 +644,8 @@ template <typename... A> cudaError_t launch_after(void (*k)(A...), dim3 grid, in
 }
 template <typename T, int D> cudaError_t launch_all(const AttendArgs &p, const Plan &pl, bool accumulate, cudaStream_t st) {
     cudaError_t e = pl.wide ? launch_attend_wide(p, pl.block, pl.pieces, accumulate, st)
-                    : accumulate ? launch_rows<T, D, true>(p, pl, st) : launch_rows<T, D, false>(p, pl, st);
+                    : accumulate ? launch_narrow<T, D, true>(p, pl, st)
+                                 : launch_narrow<T, D, false>(p, pl, st);
     if (e != cudaSuccess) return e;
     // as many warps a row as keep four CTAs' worth on every multiprocessor
     const int64_t groups = static_cast<int64_t>(p.kv.a.n_seqs) * p.kv.a.n_kv_heads;

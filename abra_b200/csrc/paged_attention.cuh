@@ -6,14 +6,14 @@
 
 namespace abra {
 
-constexpr int PIECE = 8;                  // steps of a piece, where there are enough to fill the GPU
+constexpr int PIECE = 16;                 // steps of a piece, where there are enough to fill the GPU
 constexpr int WAVES = 4;                  // pieces for each CTA that the GPU holds, at most
 // A row's maximum is raised only when a score passes it by 2^RAISE: weights
 // stay below 2^RAISE (well inside fp16), and most tiles need no reduction.
 constexpr float RAISE = 10.0f;
 // What beginning and ending a row costs beside its steps, in steps (its
 // queries, the join of its warps).
-constexpr int ROW_COST = 1;
+constexpr int ROW_COST = 2;
 
 struct AttendArgs {
     PagedKv kv;
