@@ -444,9 +444,8 @@ template <typename T, int D> __device__ __forceinline__ void join_rows(const Joi
     const int r = (cta - group * ja.row_ctas) * (JOIN_WARPS / ja.warps) + row;
     const bool in = r < p.rows;
     const int len = paged_len(p.kv, seq), block = in ? r / ja.block : 0, rr = r - block * ja.block;
-    int2 split = make_int2(0, 0);
-    if (len > 0) split = __ldcg(p.split + (static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.row_blocks + block);
-    const Parts parts(split);
+    // (of an empty sequence nobody wrote this, and nobody looks at it)
+    const Parts parts(__ldcg(p.split + (static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.row_blocks + block));
     const int n = in && len > 0 ? parts.count() : 1;  // one part: the row is done
     float top = -INFINITY, total = 0.0f;
     float4 sum = make_float4(0, 0, 0, 0);

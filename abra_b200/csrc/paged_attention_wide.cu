@@ -6,8 +6,9 @@
 // go in twice, below) for 4 D bytes.  At 64 rows that is 128 flops a byte: four
 // times what mma.sync reaches at the HBM's rate, a third of tcgen05's.
 //
-// A CTA takes steps of 128 slots.  Four loader warps copy K and V rows into a
-// ring of stages; thread t of four compute warps stands for slot t.  Per step
+// A CTA takes steps of 128 slots.  Three loader warps copy K and V rows into
+// rings of tiles, one warp issues the tensor core's work, and a thread of the
+// four or eight compute warps stands for a slot.  Per step
 //   S^T[128 slots x N] = K Q^T      (M 128, N rows, K = D)
 //   P^T = 2^(S^T - m), split into two 16-bit values, to shared memory
 //   O^T[D x N] += V^T P^T           (M 128, K = 128 slots, twice)
@@ -25,9 +26,13 @@
 namespace abra {
 namespace {
 
-constexpr int W_THREADS = 256, W_COMPUTE = 128, W_LOAD = 96;  // four compute warps, three loaders, one for the tensor core
+constexpr int W_LOAD = 96;  // three loader warps
 
 template <int D, int N> struct Wide {
+    // compute warps: four, or eight that share the rows of a slot where these
+    // are so many that four take longer than the copies (2.0 us a step of 64)
+    static constexpr int CW = N >= 64 ? 8 : 4, COMPUTE = 32 * CW, THREADS = COMPUTE + W_LOAD + 32;
+    static constexpr int NH = N / (CW / 4);             // rows of a compute thread
     static constexpr int CHUNKS = D / 8;                // of 16 bytes in a row
     static constexpr int PLANES = (D + 63) / 64;
     static constexpr int PLANE = WIDE_STEP * 128;       // bytes of 64 elements of every slot
@@ -109,17 +114,16 @@ __device__ __forceinline__ bool mbar_passed(uint64_t *bar, uint32_t parity) {
 }
 
 // Barrier of the compute warps; true for all if `x` is for one of them.
-__device__ __forceinline__ bool compute_any(bool x) {
+template <int THREADS> __device__ __forceinline__ bool compute_any(bool x) {
     uint32_t r;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-        "barrier.cta.red.or.aligned.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        "barrier.cta.red.or.aligned.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r)
-        : "r"(x ? 1u : 0u)
+        : "r"(x ? 1u : 0u), "n"(THREADS)
         : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void compute_sync() { named_bar_sync(1, W_COMPUTE); }
 
 // Folds v[0 .. N) over the warp's lanes with op; lane l ends with elements l *
 // N / 32 .. (N >= 32), or element l / 2 (N = 16), in v[0 .. max(1, N / 32)).
@@ -146,7 +150,7 @@ template <int N, typename Op> __device__ __forceinline__ void fold_lanes(float (
 template <int N> __device__ __forceinline__ int folded(int lane, int e) { return N >= 32 ? lane * (N / 32) + e : lane >> 1; }
 
 template <typename T, int D, int N, bool SCORES>
-__global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_constant__ AttendArgs p) {
+__global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(const __grid_constant__ AttendArgs p) {
     using S = Wide<D, N>;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
@@ -161,13 +165,13 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
     pdl_launch_dependents();  // the join may take its place; it waits for the whole grid
     Walk<WIDE_STEP> w;
     Line line(0, 0);
-    if (!find_start<W_THREADS>(p.kv, p.row_blocks, blockIdx.x, gridDim.x, p.resident, line, w)) return;
+    if (!find_start<S::THREADS>(p.kv, p.row_blocks, blockIdx.x, gridDim.x, p.resident, line, w)) return;
     const int begin = w.pos;
     if (tid == 0) {
         for (int i = 0; i < S::KS; ++i) mbar_init(&k_full[i], W_LOAD), mbar_init(&k_empty[i], 1);
         for (int i = 0; i < S::VS; ++i) mbar_init(&v_full[i], W_LOAD), mbar_init(&v_empty[i], 1);
-        mbar_init(&q_ready, W_COMPUTE);
-        mbar_init(&p_ready, W_COMPUTE);
+        mbar_init(&q_ready, S::COMPUTE);
+        mbar_init(&p_ready, S::COMPUTE);
         mbar_init(&s_done[0], 1);
         mbar_init(&s_done[1], 1);
         mbar_init(&o_done, 1);
@@ -187,12 +191,12 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
         if (!lost && !mbar_wait(bar, parity)) lost = true;
     };
 
-    if (warp >= 4 && warp < 7) {
+    if (warp >= S::CW && warp < S::CW + 3) {
         // ---- loaders: eight rows of a step at a time, dealt to the three warps; a
         // lane answers for rows 8 (lw + 3 (l / 8)) + l % 8 and, l < 16, those of
         // the two groups after the warp's fourth ----
         constexpr int GROUPS = WIDE_STEP / 8, COPIES = S::CHUNKS / 4;  // of a lane for a group
-        const int lw = warp - 4;
+        const int lw = warp - S::CW;
         int j = 0;
         do {
             for (int t0 = w.s.tile0 * WIDE_STEP; t0 < w.s.slot_end; t0 += WIDE_STEP, ++j) {
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
         } while (w.next(p.kv));
         copy_commit();
         copy_wait<0>();
-    } else if (warp == 7) {
+    } else if (warp == S::CW + 3) {
         // ---- the tensor core's warp: all lanes run, one issues ----
         const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0), u_o = tmem + 2 * N;
         const uint32_t u_k = __shfl_sync(0xffffffffu, smem_u32(s_k), 0), u_v = __shfl_sync(0xffffffffu, smem_u32(s_v), 0);
@@ -300,75 +304,85 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
             }
         } while (w.next(p.kv));
     } else {
-        // ---- compute warps: thread t is slot t of a step, and element t of the results ----
-        const uint32_t mine = s_tmem + (static_cast<uint32_t>(32 * warp) << 16), t_o = 2 * N;
+        // ---- compute warps: thread t is slot t % 128 of a step and element t %
+        // 128 of the results, for rows n_first .. n_first + NH - 1 ----
+        constexpr int NH = S::NH;
+        const int quarter = warp & 3, st = tid & 127, n_first = (tid >> 7) * NH;
+        const uint32_t mine = s_tmem + (static_cast<uint32_t>(32 * quarter) << 16) + n_first, t_o = 2 * N;
         int it = 0;  // steps of this CTA so far
         do {
             const Segment &sg = w.s;
             const int r0 = sg.block * N, head = sg.head;
             // Q as an operand: rows past the end are zeros
-            for (int x = tid; x < N * S::CHUNKS; x += W_COMPUTE) {
-                const int r = x / S::CHUNKS, chunk = x - r * S::CHUNKS, row = r0 + r;
-                uint4 q = make_uint4(0, 0, 0, 0);
-                if (row < p.rows) {
+            constexpr int QX = (N * S::CHUNKS + S::COMPUTE - 1) / S::COMPUTE;
+            uint4 q[QX];
+#pragma unroll
+            for (int i = 0; i < QX; ++i) {
+                const int x = i * S::COMPUTE + tid, r = x / S::CHUNKS, chunk = x - r * S::CHUNKS, row = r0 + r;
+                q[i] = make_uint4(0, 0, 0, 0);
+                if (r < N && row < p.rows) {
                     const int j = row / p.group, h = head * p.group + row - j * p.group;
-                    q = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldq +
-                                                              static_cast<int64_t>(h) * D + 8 * chunk));
+                    q[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldq +
+                                                                 static_cast<int64_t>(h) * D + 8 * chunk));
                 }
-                *reinterpret_cast<uint4 *>(s_q + (chunk >> 3) * S::Q_PLANE + swizzled(r, chunk & 7)) = q;
+            }
+#pragma unroll
+            for (int i = 0; i < QX; ++i) {
+                const int x = i * S::COMPUTE + tid, r = x / S::CHUNKS, chunk = x - r * S::CHUNKS;
+                if (r < N) *reinterpret_cast<uint4 *>(s_q + (chunk >> 3) * S::Q_PLANE + swizzled(r, chunk & 7)) = q[i];
             }
             if (tid < N) s_m[tid] = -INFINITY, s_sub[tid] = 0.0f;
             fence_proxy_async_smem();
             mbar_arrive(&q_ready);
-            compute_sync();
+            named_bar_sync(1, S::COMPUTE);
             const int all_see = sg.len - p.n_q + 1;  // slots below are seen by every row
-            float l[N];
+            float l[NH];
 #pragma unroll
-            for (int n = 0; n < N; ++n) l[n] = 0.0f;
+            for (int n = 0; n < NH; ++n) l[n] = 0.0f;
             bool odd = false;  // an infinity or NaN among the values of a step that not all rows see
-            const int j0 = r0 / p.group, rem0 = r0 - j0 * p.group;  // the query of the block's first row, its head in the group
+            const int j0 = (r0 + n_first) / p.group, rem0 = r0 + n_first - j0 * p.group;  // query of this thread's first row, head in the group
             for (int t0 = sg.tile0 * WIDE_STEP; t0 < sg.slot_end; t0 += WIDE_STEP, ++it) {
                 const bool first = t0 == sg.tile0 * WIDE_STEP, edge = t0 + WIDE_STEP > all_see;
-                const int t = t0 + tid;
+                const int t = t0 + st;
                 // ---- scores in log2 units, masked; is a maximum to be raised? ----
                 wait(&s_done[it & 1], (it >> 1) & 1);
                 tc_fence_after();
-                float s[N];
+                float s[NH];
                 bool raise = false;
 #pragma unroll
-                for (int n0 = 0; n0 < N; n0 += 16) tmem_ld16(mine + (it & 1) * N + n0, *reinterpret_cast<float (*)[16]>(s + n0));
+                for (int n0 = 0; n0 < NH; n0 += 16) tmem_ld16(mine + (it & 1) * N + n0, *reinterpret_cast<float (*)[16]>(s + n0));
                 tmem_wait_ld();
                 if (edge) {
                     int j = j0, rem = rem0;
 #pragma unroll
-                    for (int n = 0; n < N; ++n) {
+                    for (int n = 0; n < NH; ++n) {
                         if (t >= min(sg.slot_end, all_see + min(j, p.n_q - 1))) s[n] = p.scale_log2 < 0.0f ? INFINITY : -INFINITY;
                         if (++rem == p.group) rem = 0, ++j;
                     }
                 }
 #pragma unroll
-                for (int n0 = 0; n0 < N; n0 += 4) {
-                    const float4 m = *reinterpret_cast<const float4 *>(s_m + n0);
+                for (int n0 = 0; n0 < NH; n0 += 4) {
+                    const float4 m = *reinterpret_cast<const float4 *>(s_m + n_first + n0);
                     s[n0] *= p.scale_log2, s[n0 + 1] *= p.scale_log2, s[n0 + 2] *= p.scale_log2, s[n0 + 3] *= p.scale_log2;
                     raise |= s[n0] > m.x + RAISE || s[n0 + 1] > m.y + RAISE || s[n0 + 2] > m.z + RAISE || s[n0 + 3] > m.w + RAISE;
                 }
                 if (SCORES && t < sg.slot_end) {
                     const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, sg.seq, e));
-                    float *to = p.scores + paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size) * (p.row_blocks * N) + r0;
+                    float *to = p.scores + paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size) * (p.row_blocks * N) + r0 + n_first;
 #pragma unroll
-                    for (int n = 0; n < N; n += 4) *reinterpret_cast<float4 *>(to + n) = make_float4(s[n], s[n + 1], s[n + 2], s[n + 3]);
+                    for (int n = 0; n < NH; n += 4) *reinterpret_cast<float4 *>(to + n) = make_float4(s[n], s[n + 1], s[n + 2], s[n + 3]);
                 }
-                raise = compute_any(raise);
+                raise = compute_any<S::COMPUTE>(raise);
                 if (it > 0) wait(&o_done, (it - 1) & 1);  // the weights' buffer and the results are at rest
                 tc_fence_after();
                 if (raise) {
-                    float top[N];
+                    float top[NH];
 #pragma unroll
-                    for (int n = 0; n < N; ++n) top[n] = s[n];
-                    fold_lanes<N>(top, [](float a, float b) { return fmaxf(a, b); });
+                    for (int n = 0; n < NH; ++n) top[n] = s[n];
+                    fold_lanes<NH>(top, [](float a, float b) { return fmaxf(a, b); });
 #pragma unroll
-                    for (int e = 0; e < (N >= 32 ? N / 32 : 1); ++e) w_max[warp * N + folded<N>(lane, e)] = top[e];
-                    compute_sync();
+                    for (int e = 0; e < (NH >= 32 ? NH / 32 : 1); ++e) w_max[quarter * N + n_first + folded<NH>(lane, e)] = top[e];
+                    named_bar_sync(1, S::COMPUTE);
                     if (tid < N) {
                         const float m = s_m[tid];
                         const float now = fmaxf(fmaxf(fmaxf(w_max[tid], w_max[N + tid]), fmaxf(w_max[2 * N + tid], w_max[3 * N + tid])), m);
@@ -376,17 +390,17 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                         s_m[tid] = now;
                         s_sub[tid] = now == -INFINITY ? 0.0f : now;
                     }
-                    compute_sync();
+                    named_bar_sync(1, S::COMPUTE);
                     if (!first) {
 #pragma unroll
-                        for (int n0 = 0; n0 < N; n0 += 16) {
+                        for (int n0 = 0; n0 < NH; n0 += 16) {
                             float o[16];
                             tmem_ld16(mine + t_o + n0, o);
                             tmem_wait_ld();
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
-                                o[i] *= s_fac[n0 + i];
-                                l[n0 + i] *= s_fac[n0 + i];
+                                o[i] *= s_fac[n_first + n0 + i];
+                                l[n0 + i] *= s_fac[n_first + n0 + i];
                             }
                             tmem_st16(mine + t_o + n0, o);
                         }
@@ -396,11 +410,11 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                 // A slot that only some rows see has weight 0 in the others, and 0
                 // times an infinity or NaN in its V row would reach them: such
                 // elements count as zeros here and are added at the row's end.
-                if (edge && p.n_q > 1) {
+                if (edge && p.n_q > 1 && n_first == 0) {
                     wait(&v_full[it % S::VS], (it / S::VS) & 1);
                     for (int c = 0; c < S::CHUNKS; ++c) {
                         uint4 *v = reinterpret_cast<uint4 *>(s_v + it % S::VS * S::TILE + (c >> 3) * S::PLANE +
-                                                             swizzled(tid, c & 7));
+                                                             swizzled(st, c & 7));
                         bool any = false;
                         const uint4 x = make_uint4(finite_part<T>(v->x, any), finite_part<T>(v->y, any), finite_part<T>(v->z, any),
                                                    finite_part<T>(v->w, any));
@@ -410,12 +424,12 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                 // ---- weights, as the sum of two 16-bit values (one rounding would
                 // cost as much precision as the result's own) ----
 #pragma unroll
-                for (int n0 = 0; n0 < N; n0 += 8) {
+                for (int n0 = 0; n0 < NH; n0 += 8) {
                     uint32_t hi[4], lo[4];
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) {
                         const int n = n0 + i;
-                        const float2 sub = *reinterpret_cast<const float2 *>(s_sub + n);
+                        const float2 sub = *reinterpret_cast<const float2 *>(s_sub + n_first + n);
                         const float a = exp2_fast(s[n] - sub.x), b = exp2_fast(s[n + 1] - sub.y);
                         l[n] += a;
                         l[n + 1] += b;
@@ -423,7 +437,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                         const float2 h = unpack2<T>(hi[i / 2]);
                         lo[i / 2] = pack2<T>(a - h.x, b - h.y);
                     }
-                    unsigned char *to = s_p + swizzled(tid, n0 / 8);
+                    unsigned char *to = s_p + swizzled(st, (n_first + n0) / 8);
                     *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *reinterpret_cast<uint4 *>(to + S::P_BYTES) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
@@ -433,10 +447,10 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
             }
 
             // ---- the row's end ----
-            fold_lanes<N>(l, [](float a, float b) { return a + b; });
+            fold_lanes<NH>(l, [](float a, float b) { return a + b; });
 #pragma unroll
-            for (int e = 0; e < (N >= 32 ? N / 32 : 1); ++e) w_sum[warp * N + folded<N>(lane, e)] = l[e];
-            odd = compute_any(odd);
+            for (int e = 0; e < (NH >= 32 ? NH / 32 : 1); ++e) w_sum[quarter * N + n_first + folded<NH>(lane, e)] = l[e];
+            odd = compute_any<S::COMPUTE>(odd);
             const bool whole = sg.tile0 == 0 && sg.tile1 == sg.n;
             const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (w.pos == begin ? 0 : 1);
             if (tid < N && r0 + tid < p.rows) {
@@ -445,23 +459,24 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                 else p.part_ml[slot * N + tid] = make_float2(s_m[tid], total);
                 s_fac[tid] = total != 0.0f ? 1.0f / total : 0.0f;
             }
-            compute_sync();
+            named_bar_sync(1, S::COMPUTE);
             wait(&o_done, (it - 1) & 1);
             tc_fence_after();
             const int odd_from = max(sg.tile0 * WIDE_STEP, all_see / WIDE_STEP * WIDE_STEP);  // the first step with an edge
 #pragma unroll 1
-            for (int n0 = 0; n0 < N && r0 + n0 < p.rows; n0 += 16) {
+            for (int n0 = 0; n0 < NH; n0 += 16) {
+                const int n = n_first + n0, nr = min(16, p.rows - r0 - n);
                 float o[16];
                 tmem_ld16(mine + t_o + n0, o);
                 tmem_wait_ld();
-                if (tid >= D) continue;
+                if (st >= D || nr <= 0) continue;
                 if (odd) {
 #pragma unroll 1
                     for (int t = odd_from; t < sg.slot_end; ++t) {
                         const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, sg.seq, e));
-                        const float v = Half16<T>::up(static_cast<const T *>(p.kv.a.v)[paged_v_at(p.kv, page, head, t - e * p.kv.a.page_size) + tid]);
+                        const float v = Half16<T>::up(static_cast<const T *>(p.kv.a.v)[paged_v_at(p.kv, page, head, t - e * p.kv.a.page_size) + st]);
                         if (isfinite(v)) continue;
-                        int j = (r0 + n0) / p.group, rem = r0 + n0 - j * p.group;
+                        int j = (r0 + n) / p.group, rem = r0 + n - j * p.group;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             if (t < all_see + min(j, p.n_q - 1)) o[i] += v;
@@ -469,18 +484,17 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                         }
                     }
                 }
-                const int nr = min(16, p.rows - r0 - n0);
                 if (!whole) {
-                    float *to = p.part_o + (slot * N + n0) * D + tid;
+                    float *to = p.part_o + (slot * N + n) * D + st;
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if (i < nr) to[i * D] = o[i];
                 } else {
-                    int j = (r0 + n0) / p.group, rem = r0 + n0 - j * p.group;
+                    int j = (r0 + n) / p.group, rem = r0 + n - j * p.group;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int64_t to = (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldo + static_cast<int64_t>(head * p.group + rem) * D + tid;
-                        const float x = s_fac[n0 + i] != 0.0f ? o[i] * s_fac[n0 + i] : 0.0f;
+                        const int64_t to = (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldo + static_cast<int64_t>(head * p.group + rem) * D + st;
+                        const float x = s_fac[n + i] != 0.0f ? o[i] * s_fac[n + i] : 0.0f;
                         if (i < nr) {
                             if (p.out_f32) static_cast<float *>(p.out)[to] = x;
                             else static_cast<T *>(p.out)[to] = Half16<T>::down(x);
@@ -493,7 +507,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) attend_wide_kernel(const __grid_
                 p.split[static_cast<int64_t>(sg.seq) * w.units + sg.unit] =
                     make_int2(static_cast<int>(slot), whole ? static_cast<int>(blockIdx.x) : line.piece(sg.row_begin + ROW_COST + sg.n - 1));
             tc_fence_before();
-            compute_sync();  // Q, the sums and the results are free again
+            named_bar_sync(1, S::COMPUTE);  // Q, the sums and the results are free again
         } while (w.next(p.kv));
     }
     __syncthreads();
@@ -505,7 +519,7 @@ template <typename T, int D, int N, bool SCORES> cudaError_t launch_one(const At
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = paged_smem(reinterpret_cast<const void *>(attend_wide_kernel<T, D, N, SCORES>), smem, done);
     if (e != cudaSuccess) return e;
-    attend_wide_kernel<T, D, N, SCORES><<<pieces, W_THREADS, smem, st>>>(p);
+    attend_wide_kernel<T, D, N, SCORES><<<pieces, Wide<D, N>::THREADS, smem, st>>>(p);
     return cudaGetLastError();
 }
 template <typename T, int D, int N> cudaError_t launch_scores(const AttendArgs &p, int pieces, bool scores, cudaStream_t st) {

@@ -295,12 +295,12 @@ int64_t workspace_bytes_of(const abra_paged_kv *kv, int32_t budget) {
 constexpr int HELD_MOST = 40960;  // keys in a CTA's shared memory
 
 // CTAs of a cluster: doubled while all clusters stay resident together and
-// every CTA keeps eight slots a thread; adding up histograms of a cluster costs
+// every CTA keeps four slots a thread; adding up histograms of a cluster costs
 // more than a few slots do.
 int cluster_of(const abra_paged_kv *kv, int sms) {
     const int64_t slots = static_cast<int64_t>(kv->max_pages) * kv->page_size;
     int c = 1;
-    while (c < MOST_CTAS && ((rows_of(kv) * c * 2 <= 2 * sms && slots / c > 8 * SEL_THREADS) || slots / c > HELD_MOST)) c *= 2;
+    while (c < MOST_CTAS && ((rows_of(kv) * c * 2 <= 2 * sms && slots / c > 4 * SEL_THREADS) || slots / c > HELD_MOST)) c *= 2;
     return c;
 }
 

@@ -143,7 +143,7 @@ class PagedKV:
         self._index = k.get_device()
         # the current stream's handle without building a Stream object, where torch has it
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        self._current_device = torch.cuda.current_device
+        self._current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
     def _stream(self, stream) -> int:
         """The stream of a call on this cache, whose device must be the current one."""
