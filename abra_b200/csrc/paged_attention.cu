@@ -603,7 +603,7 @@ int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumu
     const int64_t steps = (static_cast<int64_t>(kv->max_pages) * kv->page_size + step - 1) / step + ROW_COST;
     if (steps * triples > 0x7fffffff || static_cast<int64_t>(kv->n_seqs) * n_heads * n_q > 0x3fffffff) return paged_fail(ABRA_E_UNSUPPORTED, "the tables name over 2^31 steps of %d slots", step);
     pl.resident = pl.sms * (pl.wide ? 1 : CTAS);
-    pl.pieces = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(pl.resident) * WAVES, steps * triples));
+    pl.pieces = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(pl.resident) * (pl.wide ? 1 : WAVES), steps * triples));
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     int64_t at = 0;
     pl.part_o = at, at = up(at + static_cast<int64_t>(pl.pieces) * 2 * pl.block * kv->head_dim * 4);

@@ -7,7 +7,8 @@
 namespace abra {
 
 constexpr int PIECE = 16;                 // steps of a piece, where there are enough to fill the GPU
-constexpr int WAVES = 4;                  // pieces for each CTA that the GPU holds, at most
+constexpr int WAVES = 4;                  // pieces for each CTA that the GPU holds, at most; the wide kernel's CTA fills its
+                                          // multiprocessor, so that nothing runs beside a new one's start, and takes one
 // A row's maximum is raised only when a score passes it by 2^RAISE: weights
 // stay below 2^RAISE (well inside fp16), and most tiles need no reduction.
 constexpr float RAISE = 10.0f;
