@@ -24,6 +24,12 @@ def pytest_configure(config):
 
 
 def pytest_collection_modifyitems(config, items):
+    if not (ROOT / "oracle" / "_ref" / "libq4k_ref.so").exists():
+        # built from the reference's sources (make -C oracle ref), where they are at hand
+        no_ref = pytest.mark.skip(reason="the reference's kernels are not built here")
+        for item in items:
+            if item.name == "test_reference_family_agrees":
+                item.add_marker(no_ref)
     try:
         import torch
 
