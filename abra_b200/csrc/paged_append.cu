@@ -48,7 +48,7 @@ constexpr int APPEND_TOKENS = 4;  // of a CTA, where there are many
 // table) runs under the large ones, and several tokens share it.
 template <typename TI, typename T, int D>
 __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_constant__ AppendArgs p) {
-    constexpr int HALF = D / 2, LANES = D == 64 ? 8 : 16, GROUPS = APPEND_THREADS / LANES, BATCH = 3;
+    constexpr int HALF = D / 2, LANES = D == 64 ? 8 : 16, GROUPS = APPEND_THREADS / LANES, BATCH = 2;
     __shared__ int s_page[APPEND_TOKENS], s_off[APPEND_TOKENS], s_at[APPEND_TOKENS];
     const int group = threadIdx.x / LANES, j = threadIdx.x % LANES;
     const unsigned lanes = ((1u << LANES) - 1u) << (threadIdx.x % 32 / LANES * LANES);  // the group's
@@ -56,8 +56,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
     const int nq = p.q ? p.n_heads : 0, nkv = p.kv.a.n_kv_heads, heads = nq + 2 * nkv;
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tokens;
     const int nt = static_cast<int>(min(static_cast<int64_t>(p.tokens), p.n_tokens - t0)), items = nt * heads;
-    float4 lo[BATCH], hi[BATCH];
-    auto load = [&](int base) {
+    float4 lo[BATCH], hi[BATCH], lo_next[BATCH], hi_next[BATCH];
+    auto load = [&](int base, float4 (&lo)[BATCH], float4 (&hi)[BATCH]) {
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
             const int x = base + b * GROUPS;
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
         }
     };
     int base = group;
-    load(base);
+    load(base, lo, hi);
     // the first token's sequence: how many end at or before it
     int s = 0;
     if (p.cu_new) {
@@ -109,6 +109,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
     }
     __syncthreads();
     for (;;) {
+        load(base + BATCH * GROUPS, lo_next, hi_next);  // zeros beyond the last item
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
             const int item = base + b * GROUPS;
@@ -156,7 +157,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
         }
         base += BATCH * GROUPS;
         if (base >= items) return;
-        load(base);
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) lo[b] = lo_next[b], hi[b] = hi_next[b];
     }
 }
 
