@@ -50,6 +50,8 @@ template <typename TI, typename T, int D>
 __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_constant__ AppendArgs p) {
     constexpr int HALF = D / 2, LANES = D == 64 ? 8 : 16, GROUPS = APPEND_THREADS / LANES, BATCH = 2;
     __shared__ int s_page[APPEND_TOKENS], s_off[APPEND_TOKENS], s_at[APPEND_TOKENS];
+    pdl_wait();
+    pdl_launch_dependents();
     const int group = threadIdx.x / LANES, j = threadIdx.x % LANES;
     const unsigned lanes = ((1u << LANES) - 1u) << (threadIdx.x % 32 / LANES * LANES);  // the group's
     const bool on = 4 * j < HALF;  // heads of 96 use 12 lanes of a group
@@ -166,11 +168,10 @@ template <typename TI, typename T>
 cudaError_t launch(const AppendArgs &p, cudaStream_t stream) {
     const dim3 grid((p.n_tokens + p.tokens - 1) / p.tokens);
     switch (p.kv.a.head_dim) {
-        case 64: append_kernel<TI, T, 64><<<grid, APPEND_THREADS, 0, stream>>>(p); break;
-        case 96: append_kernel<TI, T, 96><<<grid, APPEND_THREADS, 0, stream>>>(p); break;
-        default: append_kernel<TI, T, 128><<<grid, APPEND_THREADS, 0, stream>>>(p); break;
+        case 64: return paged_launch(append_kernel<TI, T, 64>, grid, APPEND_THREADS, 0, stream, p);
+        case 96: return paged_launch(append_kernel<TI, T, 96>, grid, APPEND_THREADS, 0, stream, p);
+        default: return paged_launch(append_kernel<TI, T, 128>, grid, APPEND_THREADS, 0, stream, p);
     }
-    return cudaGetLastError();
 }
 
 }  // namespace

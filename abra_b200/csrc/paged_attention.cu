@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
     float *s_m = s_o + 2 * ROWS * S::PITCH, *s_l = s_m + AT_WARPS * ROWS;  // [warp][ROWS]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
 
+    pdl_wait();
     pdl_launch_dependents();  // the join may take its place; it waits for the whole grid
     Walk<STEP> w;
     Line line(0, 0);
@@ -580,6 +581,7 @@ __device__ __forceinline__ void accumulate(const JoinArgs &ja, int cta, int ctas
 // rows that were split, and adds the slots' weights, side by side.
 template <typename T, int D> __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ JoinArgs ja) {
     pdl_wait();
+    pdl_launch_dependents();
     const int cta = blockIdx.x;
     if (cta < ja.joins) join_rows<T, D>(ja, cta);
     else accumulate(ja, cta - ja.joins, gridDim.x - ja.joins);
@@ -624,22 +626,7 @@ template <typename T, int D, bool SCORES> cudaError_t launch_narrow(const Attend
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = paged_smem(reinterpret_cast<const void *>(attend_kernel<T, D, SCORES>), smem, done);
     if (e != cudaSuccess) return e;
-    attend_kernel<T, D, SCORES><<<pl.pieces, AT_THREADS, smem, st>>>(p);
-    return cudaGetLastError();
-}
-// A launch that may begin before the kernel in front of it has ended (its
-// pdl_wait waits for that).
-template <typename... A> cudaError_t launch_after(void (*k)(A...), dim3 grid, int threads, cudaStream_t st, A... a) {
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.stream = st;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k, a...);
+    return paged_launch(attend_kernel<T, D, SCORES>, dim3(pl.pieces), AT_THREADS, smem, st, p);
 }
 template <typename T, int D> cudaError_t launch_all(const AttendArgs &p, const Plan &pl, bool accumulate, cudaStream_t st) {
     cudaError_t e = pl.wide ? launch_attend_wide(p, pl.block, pl.pieces, accumulate, st)
@@ -652,7 +639,7 @@ template <typename T, int D> cudaError_t launch_all(const AttendArgs &p, const P
     while (warps > 1 && groups * p.rows * warps > pl.sms * 4 * JOIN_WARPS) warps /= 2;
     const int per = JOIN_WARPS / warps, row_ctas = (p.rows + per - 1) / per;
     const JoinArgs ja{p, pl.block, warps, row_ctas, static_cast<int>(groups * row_ctas)};
-    return launch_after(join_kernel<T, D>, dim3(ja.joins + (accumulate ? pl.sms * 4 : 0)), JOIN_THREADS, st, ja);
+    return paged_launch(join_kernel<T, D>, dim3(ja.joins + (accumulate ? pl.sms * 4 : 0)), JOIN_THREADS, 0, st, ja);
 }
 template <typename T> cudaError_t launch(const AttendArgs &p, const Plan &pl, bool accumulate, cudaStream_t st) {
     switch (p.kv.a.head_dim) {

@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
     float *s_m = w_sum + 4 * N, *s_sub = s_m + N, *s_fac = s_sub + N;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
+    pdl_wait();
     pdl_launch_dependents();  // the join may take its place; it waits for the whole grid
     Walk<WIDE_STEP> w;
     Line line(0, 0);
@@ -519,8 +520,7 @@ template <typename T, int D, int N, bool SCORES> cudaError_t launch_one(const At
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = paged_smem(reinterpret_cast<const void *>(attend_wide_kernel<T, D, N, SCORES>), smem, done);
     if (e != cudaSuccess) return e;
-    attend_wide_kernel<T, D, N, SCORES><<<pieces, Wide<D, N>::THREADS, smem, st>>>(p);
-    return cudaGetLastError();
+    return paged_launch(attend_wide_kernel<T, D, N, SCORES>, dim3(pieces), Wide<D, N>::THREADS, smem, st, p);
 }
 template <typename T, int D, int N> cudaError_t launch_scores(const AttendArgs &p, int pieces, bool scores, cudaStream_t st) {
     return scores ? launch_one<T, D, N, true>(p, pieces, st) : launch_one<T, D, N, false>(p, pieces, st);

@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const __grid_consta
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = cluster_rank(), size = cluster_size();
     const int g = blockIdx.y, s = blockIdx.z;
+    pdl_wait();
     pdl_launch_dependents();
     const int len = paged_len(p.kv, s);
     const int64_t row = static_cast<int64_t>(s) * p.kv.a.n_kv_heads + g;
@@ -241,6 +242,7 @@ __global__ void __launch_bounds__(MOVE_THREADS, 4) move_kernel(const __grid_cons
     const int g = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
     const int64_t row = static_cast<int64_t>(s) * p.kv.a.n_kv_heads + g;
     pdl_wait();
+    pdl_launch_dependents();
     const int first = blockIdx.x * MOVES, n = min(MOVES, __ldcg(p.counts + row) - first);
     if (n <= 0) return;
     const int32_t *hole = p.moves + row * 2 * p.cap + first, *mover = hole + p.cap;
@@ -307,27 +309,6 @@ int cluster_of(const abra_paged_kv *kv, int sms) {
     return c;
 }
 
-cudaError_t launch_kernel(const void *k, dim3 grid, int threads, int smem, int cluster, cudaStream_t st, EvictArgs &p) {
-    cudaLaunchAttribute at{};
-    if (cluster) {
-        at.id = cudaLaunchAttributeClusterDimension;
-        at.val.clusterDim.x = cluster;
-        at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    } else {  // may begin before the kernel in front of it has ended; its pdl_wait waits for that
-        at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at.val.programmaticStreamSerializationAllowed = 1;
-    }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    void *args[] = {&p};
-    return cudaLaunchKernelExC(&cfg, k, args);
-}
-
 cudaError_t launch(EvictArgs &p, cudaStream_t st) {
     const int64_t slots = static_cast<int64_t>(p.kv.a.max_pages) * p.kv.a.page_size;
     const int cluster = cluster_of(&p.kv.a, device_sm_count());
@@ -337,12 +318,13 @@ cudaError_t launch(EvictArgs &p, cudaStream_t st) {
     cudaError_t e = paged_smem(reinterpret_cast<const void *>(select_kernel), LANE_BINS_BYTES + HELD_MOST * 4, done);
     if (e != cudaSuccess) return e;
     const unsigned heads = p.kv.a.n_kv_heads, seqs = p.kv.a.n_seqs;
-    e = launch_kernel(reinterpret_cast<const void *>(select_kernel), dim3(cluster, heads, seqs), SEL_THREADS, smem, cluster, st, p);
+    void *args[] = {&p};
+    e = paged_launch(reinterpret_cast<const void *>(select_kernel), dim3(cluster, heads, seqs), SEL_THREADS, smem, st, args, cluster);
     if (e != cudaSuccess || p.cap == 0) return e;
     const void *k = p.kv.a.head_dim == 64   ? reinterpret_cast<const void *>(move_kernel<64>)
                     : p.kv.a.head_dim == 96 ? reinterpret_cast<const void *>(move_kernel<96>)
                                             : reinterpret_cast<const void *>(move_kernel<128>);
-    return launch_kernel(k, dim3((p.cap + MOVES - 1) / MOVES, heads, seqs), MOVE_THREADS, 0, 0, st, p);
+    return paged_launch(k, dim3((p.cap + MOVES - 1) / MOVES, heads, seqs), MOVE_THREADS, 0, st, args);
 }
 
 }  // namespace

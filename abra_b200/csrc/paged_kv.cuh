@@ -129,6 +129,29 @@ inline cudaError_t paged_smem(const void *k, int bytes, std::atomic<uint64_t> &d
     if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
     return e;
 }
+// A launch that may begin before the kernel in front of it in the stream has
+// ended; the kernel's pdl_wait, ahead of everything it reads, waits for that.
+// Clusters of `cluster` CTAs along x, or none (0).
+inline cudaError_t paged_launch(const void *k, dim3 grid, int threads, int smem, cudaStream_t st, void **args, int cluster = 0) {
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster ? 2 : 1;
+    return cudaLaunchKernelExC(&cfg, k, args);
+}
+template <typename Args> cudaError_t paged_launch(void (*k)(Args), dim3 grid, int threads, int smem, cudaStream_t st, Args a) {
+    void *args[] = {&a};
+    return paged_launch(reinterpret_cast<const void *>(k), grid, threads, smem, st, args);
+}
 inline int paged_cuda(cudaError_t e, const char *what) {
     return e == cudaSuccess ? ABRA_OK : paged_fail(ABRA_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
