@@ -6,6 +6,11 @@
 // the token's position: y = x * rsqrt(mean(x^2) + eps) * w, then for i < D/2
 //   o_i = y_i c_i - y_{i+D/2} s_i,   o_{i+D/2} = y_{i+D/2} c_i + y_i s_i.
 // Everything is fp32 up to the one rounding of the store.
+//
+// Bound: 4 bytes read and 2 written a value; for few tokens the way from the
+// launch through the token's lookups to the store.  Measured (B200, 1965 MHz, 32
+// + 8 + 8 heads of 128): 9,555 tokens of prompts, 358 MB, 64 us = 5.6 TB/s, with
+// 63 % of the issue slots used; one token 5.1 us, 32 of as many sequences 5.1.
 #include "paged_kv.cuh"
 
 namespace abra {
@@ -39,13 +44,14 @@ __device__ __forceinline__ float4 ldg4(const float *p) { return __ldg(reinterpre
 __device__ __forceinline__ float4 mul4(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
 
 constexpr int APPEND_THREADS = 256;
-constexpr int APPEND_TOKENS = 4;  // of a CTA, where there are many
+constexpr int APPEND_TOKENS = 4;  // of a CTA, where there are many (2: 67 us, 8: 71, for 64 us)
 
 // A CTA takes a few neighbouring tokens, a group of 16 lanes (8 for heads of
 // 64) a head: lane j holds the pairs (4 j + u, 4 j + u + D/2), u = 0..3.  The
 // first heads' values are asked for before the tokens' sequences, slots and
 // pages are looked up, so that the chain of small reads (offsets, length,
-// table) runs under the large ones, and several tokens share it.
+// table) runs under the large ones, and several tokens share it; after that the
+// next heads' loads run under this batch's arithmetic and stores (69 us without).
 template <typename TI, typename T, int D>
 __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_constant__ AppendArgs p) {
     constexpr int HALF = D / 2, LANES = D == 64 ? 8 : 16, GROUPS = APPEND_THREADS / LANES, BATCH = 2;

@@ -2,9 +2,13 @@
 // head (several new tokens of a group: verification of drafts, or wide groups),
 // on the 5th-generation tensor cores.
 //
-// With R = group x n_q rows a slot of a kv head costs 8 R D flops (the weights
-// go in twice, below) for 4 D bytes.  At 64 rows that is 128 flops a byte: four
-// times what mma.sync reaches at the HBM's rate, a third of tcgen05's.
+// With R = group x n_q rows a slot of a kv head costs 6 R D flops (the weights
+// go in twice, below) for 4 D bytes: at 64 rows 96 flops a byte, 630 TFLOP/s at
+// the HBM's rate.  mma.sync's pipe does 580 at most here (two cycles a 16x8x16
+// product and multiprocessor), before anything else is issued; tcgen05's limit
+// is the shared memory that its operands are read from, about 60 cycles for a
+// 128-row one of 16 columns whatever N is, 1,440 a step of 128 slots against the
+// 2,900 that the step's bytes take.
 //
 // A CTA takes steps of 128 slots.  Three loader warps copy K and V rows into
 // rings of tiles, one warp issues the tensor core's work, and a thread of the
@@ -16,10 +20,18 @@
 // in rows of 128 bytes (64 elements; wider rows in planes) with the 128-byte
 // swizzle: 16-byte chunk c of row r at r * 128 + (c ^ r % 8) * 16.  The same
 // bytes are a K-major operand (K and Q: the chunks walk along D) and an M-major
-// one (V and P: the rows are the contracted slots).  The next step's
-// scores are issued before this step's softmax where its rows have landed.  For heads of less than 128 the
-// O^T product also takes what lies behind V in shared memory: into rows beyond D
-// of O^T that nobody reads.
+// one (V and P: the rows are the contracted slots).  The next step's scores are
+// issued as soon as its keys have landed, this step's sum as soon as its weights
+// are written, by a warp in uniform control flow: issued by one thread of a
+// branch, each product cost 40 to 80 ns of register moves, five times its work.
+// For heads of less than 128 the O^T product also takes what lies behind V in
+// shared memory: into rows beyond D of O^T that nobody reads.
+//
+// Measured (B200, 1965 MHz): 16 queries of 4 heads over 4 sequences of up to
+// 8,192 slots 26 us (mma.sync with 32 rows a block: 68); 16 heads of one token
+// over 131,072 slots, 0.54 GB, 100 us = 5.4 TB/s.  A step of 64 rows takes 1.2
+// us of softmax and 1.7 of copies; a CTA's start, 3.5 us to its first scores,
+// and a row's end, 2 us, run beside nothing and bound the smaller calls.
 #include "paged_attention.cuh"
 #include "tc_common.cuh"
 
@@ -30,7 +42,8 @@ constexpr int W_LOAD = 96;  // three loader warps
 
 template <int D, int N> struct Wide {
     // compute warps: four, or eight that share the rows of a slot where these
-    // are so many that four take longer than the copies (2.0 us a step of 64)
+    // are so many that four take longer than the copies (2.0 us a step of 64
+    // rows; 16 queries of 4 sequences 31.7 us with four, 27.2 with eight)
     static constexpr int CW = N >= 64 ? 8 : 4, COMPUTE = 32 * CW, THREADS = COMPUTE + W_LOAD + 32;
     static constexpr int NH = N / (CW / 4);             // rows of a compute thread
     static constexpr int CHUNKS = D / 8;                // of 16 bytes in a row

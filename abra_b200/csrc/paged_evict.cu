@@ -13,8 +13,14 @@
 // reads weights and positions once, keeps the keys in shared memory, finds the
 // budget-th largest by four passes of 8 bits over them (histograms added up
 // through the cluster's shared memory) and writes the lists of holes and movers
-// in slot order.  The second copies, a CTA for every 128 moves of a list; it is
-// bound by the rows it reads and writes.
+// in slot order.  The second copies, a CTA for every 128 moves of a list.
+//
+// Bound: 8 bytes a slot to choose among and the moved rows, read and written.
+// Measured (B200, 1965 MHz, 8 kv heads of 128): one sequence of 131,072 slots to
+// 32,768, 213 MB, 66 us, 27 of them the selection on 64 multiprocessors and 38
+// the copies (5.3 TB/s); 32 prompts of up to 8,192 to 2,048, 126 MB, 43 us, 16
+// and 20; one page over 4,096 slots 16 us, all of it the chain of the selection
+// (3 us to the keys, 1.5 a radix pass, 4 for the lists) and a launch.
 #include <algorithm>
 
 #include "paged_kv.cuh"
