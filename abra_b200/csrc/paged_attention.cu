@@ -699,6 +699,7 @@ extern "C" int abra_paged_attention(const abra_paged_kv *kv, const void *q, int6
     if (!paged_aligned(workspace, 256)) return paged_fail(ABRA_E_INVALID, "the workspace must be 256-byte aligned");
     if (workspace_bytes < 256) return paged_fail(ABRA_E_INVALID, "workspace of %lld bytes", (long long)workspace_bytes);
     if (kv->n_seqs == 0) return ABRA_OK;
+    if (q == out) return paged_fail(ABRA_E_INVALID, "out must not be q's memory");
     const bool accumulate = flags & ABRA_PAGED_ACCUMULATE;
     Plan pl;
     rc = make_plan(kv, n_heads, n_q, accumulate, pl);

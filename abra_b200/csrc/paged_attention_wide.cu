@@ -366,18 +366,19 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
 #pragma unroll
                 for (int n0 = 0; n0 < NH; n0 += 16) tmem_ld16(mine + (it & 1) * N + n0, *reinterpret_cast<float (*)[16]>(s + n0));
                 tmem_wait_ld();
+#pragma unroll
+                for (int n = 0; n < NH; ++n) s[n] *= p.scale_log2;
                 if (edge) {
                     int j = j0, rem = rem0;
 #pragma unroll
                     for (int n = 0; n < NH; ++n) {
-                        if (t >= min(sg.slot_end, all_see + min(j, p.n_q - 1))) s[n] = p.scale_log2 < 0.0f ? INFINITY : -INFINITY;
+                        if (t >= min(sg.slot_end, all_see + min(j, p.n_q - 1))) s[n] = -INFINITY;
                         if (++rem == p.group) rem = 0, ++j;
                     }
                 }
 #pragma unroll
                 for (int n0 = 0; n0 < NH; n0 += 4) {
                     const float4 m = *reinterpret_cast<const float4 *>(s_m + n_first + n0);
-                    s[n0] *= p.scale_log2, s[n0 + 1] *= p.scale_log2, s[n0 + 2] *= p.scale_log2, s[n0 + 3] *= p.scale_log2;
                     raise |= s[n0] > m.x + RAISE || s[n0 + 1] > m.y + RAISE || s[n0 + 2] > m.z + RAISE || s[n0 + 3] > m.w + RAISE;
                 }
                 if (SCORES && t < sg.slot_end) {

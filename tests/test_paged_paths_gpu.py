@@ -179,3 +179,32 @@ def test_evict_from_a_cache_beyond_shared_memory(dev, n, budget):
     want[:] = weight
     want[pg[holes], 0, off[holes]] = weight[pg[movers], 0, off[movers]]
     assert np.array_equal(acc.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+@pytest.mark.parametrize("hq,n_q", [(4, 1), (4, 2), (12, 3)])
+def test_scales_of_zero_and_below(dev, scale, hq, n_q):
+    """Zero: the mean of the seen rows."""
+    import abra_b200 as A
+
+    rng = np.random.default_rng(13)
+    lens = [1, 2, 17, 200]
+    c = R.make_cache(rng, lens, 1, 64, 16, "f16")
+    q = torch.from_numpy(rng.standard_normal((len(lens), n_q, hq, 64))).half()
+    cd = R.to_dev(c, dev)
+    kv = _kv(cd, acc=cd["acc"])
+    before = cd["acc"].clone()
+    lse = torch.empty(len(lens), n_q, hq, device=dev)
+    out = A.paged_attention(kv, q.to(dev), scale, lse=lse, accumulate=True)
+    _no_error()
+    _check_attention(c, q, scale, out, lse, "f16", before, cd["acc"])
+
+
+def test_results_do_not_go_over_the_queries(dev):
+    import abra_b200 as A
+
+    rng = np.random.default_rng(14)
+    c = R.make_cache(rng, [20], 1, 64, 16, "f16")
+    q = torch.zeros(1, 1, 2, 64, dtype=torch.float16, device=dev)
+    with pytest.raises(ValueError, match="memory"):
+        A.paged_attention(_kv(R.to_dev(c, dev)), q, 0.1, out=q)
