@@ -40,7 +40,7 @@ template <typename T> __device__ __forceinline__ void store4(T *p, float4 x) {
     const T h[4] = {Half16<T>::down(x.x), Half16<T>::down(x.y), Half16<T>::down(x.z), Half16<T>::down(x.w)};
     *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(h);
 }
-__device__ __forceinline__ float4 ldg4(const float *p) { return __ldg(reinterpret_cast<const float4 *>(p)); }
+__device__ __forceinline__ float4 read4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
 __device__ __forceinline__ float4 mul4(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
 
 constexpr int APPEND_THREADS = 256;
@@ -87,15 +87,15 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
     if (p.cu_new) {
         for (int x = 0; x < p.kv.a.n_seqs; x += APPEND_THREADS) {
             const int y = x + threadIdx.x;
-            s += __syncthreads_count(y < p.kv.a.n_seqs && __ldg(p.cu_new + y + 1) <= t0);
+            s += __syncthreads_count(y < p.kv.a.n_seqs && p.cu_new[y + 1] <= t0);
         }
     }
     if (threadIdx.x < nt) {  // each token's slot, position and page
         const int t = static_cast<int>(t0) + threadIdx.x;
         int end, page = -1, off = 0, at = -1;
         if (p.cu_new) {
-            while (s < p.kv.a.n_seqs && __ldg(p.cu_new + s + 1) <= t) ++s;
-            end = s < p.kv.a.n_seqs ? __ldg(p.cu_new + s + 1) : 0;
+            while (s < p.kv.a.n_seqs && p.cu_new[s + 1] <= t) ++s;
+            end = s < p.kv.a.n_seqs ? p.cu_new[s + 1] : 0;
         } else {
             const int m = p.n_tokens / p.kv.a.n_seqs;
             s = t / m;
@@ -131,13 +131,13 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
                 for (int m = LANES / 2; m >= 1; m >>= 1) ss += __shfl_xor_sync(lanes, ss, m);
                 const float r = rsqrtf(ss * (1.0f / D) + p.eps);
                 if (on) {
-                    x = mul4(mul4(x, make_float4(r, r, r, r)), ldg4(nw + 4 * j));
-                    y = mul4(mul4(y, make_float4(r, r, r, r)), ldg4(nw + 4 * j + HALF));
+                    x = mul4(mul4(x, make_float4(r, r, r, r)), read4(nw + 4 * j));
+                    y = mul4(mul4(y, make_float4(r, r, r, r)), read4(nw + 4 * j + HALF));
                 }
             }
             if (p.rope && h < nq + nkv && on && at >= 0 && at < p.rope_len) {
                 const float *row = p.rope + static_cast<int64_t>(at) * D + 8 * j;
-                const float4 c01 = ldg4(row), c23 = ldg4(row + 4), u = x;  // cos, sin of two pairs each
+                const float4 c01 = read4(row), c23 = read4(row + 4), u = x;  // cos, sin of two pairs each
                 x = make_float4(u.x * c01.x - y.x * c01.y, u.y * c01.z - y.y * c01.w, u.z * c23.x - y.z * c23.y,
                                 u.w * c23.z - y.w * c23.w);
                 y = make_float4(y.x * c01.x + u.x * c01.y, y.y * c01.z + u.y * c01.w, y.z * c23.x + u.z * c23.y,

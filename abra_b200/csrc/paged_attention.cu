@@ -130,15 +130,13 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
     const bool by8 = p.kv.a.page_size % 8 == 0;
     Walk<STEP> f = w;
     int f_base = f.s.tile0 * STEP + warp * TILE, f_valid = 0;
-    int f_page = 0;  // of half l % 2 of tile f_first + l / 2 (16 tiles at a time), or (by8 false) of row l % 16 of this tile
-    int f_tile = 16;
+    int f_page = 0;    // of half l % 2 of the batch's tile l / 2, or (by8 false) of row l % 16 of this tile
+    int f_tile = 16;   // this tile's place in its batch of 16; 16: the next batch is to be read
     uint32_t f_at = ring;
     bool f_more = true;
     int64_t f_v0 = 0, f_v1 = 0;  // V offsets of the halves' first rows, or (by8 false) f_v0 of row lane % 16
     auto page_of = [&](int t) {
-        return t < f.s.slot_end
-                   ? __ldg(p.kv.a.table + static_cast<int64_t>(f.s.seq) * p.kv.a.table_stride + p.kv.page.div(t))
-                   : 0;
+        return t < f.s.slot_end ? p.kv.a.table[static_cast<int64_t>(f.s.seq) * p.kv.a.table_stride + p.kv.page.div(t)] : 0;
     };
     auto fetch_settle = [&]() {  // on to the next tile that exists, and its pages
         while (f_base >= f.s.slot_end) {
@@ -229,8 +227,8 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             const T *q = static_cast<const T *>(p.q) + (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldq + static_cast<int64_t>(h) * D + 2 * c;
 #pragma unroll
             for (int ks = 0; ks < S::KS; ++ks)
-                qf[ks] = g < p.rows ? make_uint2(__ldg(reinterpret_cast<const unsigned *>(q + 16 * ks)),
-                                                 __ldg(reinterpret_cast<const unsigned *>(q + 16 * ks + 8)))
+                qf[ks] = g < p.rows ? make_uint2(*reinterpret_cast<const unsigned *>(q + 16 * ks),
+                                                 *reinterpret_cast<const unsigned *>(q + 16 * ks + 8))
                                     : make_uint2(0, 0);
         }
         // slots below are seen by every row; row 2 c + e sees `seen` of them
@@ -601,7 +599,6 @@ struct Plan {
     int64_t part_o, part_ml, split, row_lse, scores, bytes;  // workspace offsets
 };
 
-
 int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumulate, Plan &pl) {
     pl.sms = device_sm_count();
     const int rows = n_heads / kv->n_kv_heads * n_q;
@@ -611,7 +608,8 @@ int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumu
     const int64_t triples = static_cast<int64_t>(kv->n_seqs) * kv->n_kv_heads * pl.row_blocks;
     const int step = pl.wide ? WIDE_STEP : STEP;
     const int64_t steps = (static_cast<int64_t>(kv->max_pages) * kv->page_size + step - 1) / step + ROW_COST;
-    if (steps * triples > 0x7fffffff || static_cast<int64_t>(kv->n_seqs) * n_heads * n_q > 0x3fffffff) return paged_fail(ABRA_E_UNSUPPORTED, "the tables name over 2^31 steps of %d slots", step);
+    if (steps * triples > 0x7fffffff || static_cast<int64_t>(kv->n_seqs) * n_heads * n_q > 0x3fffffff)
+        return paged_fail(ABRA_E_UNSUPPORTED, "over 2^31 steps of %d slots in the tables, or over 2^30 output rows", step);
     pl.resident = pl.sms * (pl.wide ? 1 : CTAS);
     pl.pieces = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(pl.resident) * (pl.wide ? 1 : WAVES), steps * triples));
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };

@@ -336,8 +336,8 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
                 q[i] = make_uint4(0, 0, 0, 0);
                 if (r < N && row < p.rows) {
                     const int j = row / p.group, h = head * p.group + row - j * p.group;
-                    q[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldq +
-                                                                 static_cast<int64_t>(h) * D + 8 * chunk));
+                    q[i] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.q) + (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldq +
+                                                            static_cast<int64_t>(h) * D + 8 * chunk);
                 }
             }
 #pragma unroll

@@ -37,20 +37,25 @@ struct PagedKv {
     FastDiv page;
 };
 
+// What a step's earlier kernels may have written (lengths, tables, queries) is
+// read with ordinary loads: these kernels start before the one in front of them
+// has ended, and the read-only path asks for data that stays as it is from then
+// on.
+
 // Slots of sequence s, clamped to what the table can name.
 __device__ __forceinline__ int paged_len(const PagedKv &kv, int s) {
-    const int n = __ldg(kv.a.lens + s), cap = kv.a.max_pages * kv.a.page_size;
+    const int n = kv.a.lens[s], cap = kv.a.max_pages * kv.a.page_size;
     if (n >= 0 && n <= cap) return n;
     report_error(ERR_BAD_INDEX);
     return n < 0 ? 0 : cap;
 }
 __device__ __forceinline__ int paged_next_pos(const PagedKv &kv, int s, int len) {
-    return kv.a.next_pos ? __ldg(kv.a.next_pos + s) : len;
+    return kv.a.next_pos ? kv.a.next_pos[s] : len;
 }
 // Page number of table entry p of sequence s; -1 (and the error bit) when it
 // is outside the pool.
 __device__ __forceinline__ int paged_page(const PagedKv &kv, int s, int p) {
-    const int page = __ldg(kv.a.table + static_cast<int64_t>(s) * kv.a.table_stride + p);
+    const int page = kv.a.table[static_cast<int64_t>(s) * kv.a.table_stride + p];
     if (static_cast<unsigned>(page) < static_cast<unsigned>(kv.a.n_pages)) return page;
     report_error(ERR_BAD_INDEX);
     return -1;

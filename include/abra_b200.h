@@ -546,7 +546,8 @@ int abra_paged_append(const abra_paged_kv *kv, const void *q, const void *k, con
  * takes log sum_t exp(scale q.k_t).  A query that sees no slot gives zeros and
  * -infinity.  With ABRA_PAGED_ACCUMULATE every slot's softmax weight, summed
  * over the n_q queries and the group's heads, is added to acc.
- * workspace (256-byte aligned, abra_paged_attention_workspace bytes) may hold
+ * workspace (256-byte aligned, abra_paged_attention_workspace bytes; when
+ * accumulating it has room for the scores of all the pools' slots) may hold
  * anything; calls that can overlap need one each.
  * head_dim 64, 96 or 128. */
 #define ABRA_PAGED_ACCUMULATE 1
