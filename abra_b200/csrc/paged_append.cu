@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
 
 template <typename TI, typename T>
 cudaError_t launch(const AppendArgs &p, cudaStream_t stream) {
-    const dim3 grid((p.n_tokens + p.tokens - 1) / p.tokens);
+    const dim3 grid((p.n_tokens - 1) / p.tokens + 1);
     switch (p.kv.a.head_dim) {
         case 64: return paged_launch(append_kernel<TI, T, 64>, grid, APPEND_THREADS, 0, stream, p);
         case 96: return paged_launch(append_kernel<TI, T, 96>, grid, APPEND_THREADS, 0, stream, p);

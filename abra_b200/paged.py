@@ -154,6 +154,20 @@ class PagedKV:
         return stream_handle(stream)
 
 
+def _empty(kv: PagedKV, shape, dtype, stream):
+    """Uninitialised memory for a call on ``stream``: of that stream's pool, so
+    that neither what else ran on it before nor what takes it afterwards meets
+    the call."""
+    import torch
+
+    if stream is None or stream_handle(stream) == stream_handle():
+        return torch.empty(shape, dtype=dtype, device=kv.device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, kv.device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=kv.device)
+
+
 def _vector(t, name: str, n: int, kv: PagedKV):
     if t is None:
         return 0
@@ -190,9 +204,7 @@ def paged_append(kv: PagedKV, k, v, q=None, q_out=None, cu_new=None, q_norm=None
         if heads * hd != width or nq != n or q.dtype != dtype:
             raise ValueError("q must be whole heads with the rows and the type of k and v")
         if q_out is None:
-            import torch
-
-            q_out = torch.empty((n, heads, hd), dtype=kv.dtype, device=kv.device)
+            q_out = _empty(kv, (n, heads, hd), kv.dtype, stream)
         no, ldqo = _rows(q_out, "q_out", width, dev)
         if no != n or q_out.dtype != kv.dtype:
             raise ValueError("q_out must have q's rows and the cache's type")
@@ -231,14 +243,15 @@ def _size(n: int, func: str) -> int:
     return n
 
 
-def paged_attention_workspace(kv: PagedKV, n_heads: int, n_q: int = 1, accumulate: bool = False):
+def paged_attention_workspace(kv: PagedKV, n_heads: int, n_q: int = 1, accumulate: bool = False, stream=None):
     """A workspace for :func:`paged_attention` with these arguments
-    (uninitialised bytes).  One serves any number of calls that follow one
-    another, all layers' among them; calls on several streams need one each."""
+    (uninitialised bytes, allocated on ``stream``).  One serves any number of
+    calls that follow one another, all layers' among them; calls on several
+    streams need one each."""
     import torch
 
     n = lib.abra_paged_attention_workspace(kv._ref, n_heads, n_q, ABRA_PAGED_ACCUMULATE if accumulate else 0)
-    return torch.empty(_size(n, "abra_paged_attention_workspace"), dtype=torch.uint8, device=kv.device)
+    return _empty(kv, _size(n, "abra_paged_attention_workspace"), torch.uint8, stream)
 
 
 def paged_attention(kv: PagedKV, q, scale: float, out=None, lse=None, accumulate: bool = False,
@@ -257,16 +270,14 @@ def paged_attention(kv: PagedKV, q, scale: float, out=None, lse=None, accumulate
     width = heads * hd
     _, ldq = _rows(q, "q", width, dev)
     if out is None:
-        import torch
-
-        out = torch.empty(shape, dtype=kv.dtype, device=kv.device)
+        out = _empty(kv, shape, kv.dtype, stream)
     out_type = kv._types.get(out.dtype)
     if out.numel() != q.numel() or (out.dtype != kv.dtype and out_type != ABRA_GGML_F32):
         raise ValueError("out must be like q, in the cache's type or float32")
     _, ldo = _rows(out, "out", width, dev)
     flags = ABRA_PAGED_ACCUMULATE if accumulate else 0
     if workspace is None:
-        workspace = paged_attention_workspace(kv, heads, n_q, accumulate)
+        workspace = paged_attention_workspace(kv, heads, n_q, accumulate, stream)
     rc = lib.abra_paged_attention(
         kv._ref, q.data_ptr(), ldq, heads, n_q, scale, out.data_ptr(), out_type, ldo,
         _vector(lse, "lse", kv.n_seqs * n_q * heads, kv), flags, *_bytes(workspace, kv), kv._stream(stream))
@@ -275,12 +286,13 @@ def paged_attention(kv: PagedKV, q, scale: float, out=None, lse=None, accumulate
     return out
 
 
-def paged_evict_workspace(kv: PagedKV, budget: int):
-    """A workspace for :func:`paged_evict` with this budget (uninitialised bytes)."""
+def paged_evict_workspace(kv: PagedKV, budget: int, stream=None):
+    """A workspace for :func:`paged_evict` with this budget (uninitialised
+    bytes, allocated on ``stream``)."""
     import torch
 
     n = lib.abra_paged_evict_workspace(kv._ref, budget)
-    return torch.empty(_size(n, "abra_paged_evict_workspace"), dtype=torch.uint8, device=kv.device)
+    return _empty(kv, _size(n, "abra_paged_evict_workspace"), torch.uint8, stream)
 
 
 def paged_evict(kv: PagedKV, budget: int, n_sink: int = 0, n_recent: int = 0, new_lens=None,
@@ -292,14 +304,12 @@ def paged_evict(kv: PagedKV, budget: int, n_sink: int = 0, n_recent: int = 0, ne
     is not changed, so that every layer's cache can be cut before
     ``kv.lens.copy_(new_lens)``."""
     if new_lens is None:
-        import torch
-
-        new_lens = torch.empty(kv.n_seqs, dtype=torch.int32, device=kv.device)
+        new_lens = _empty(kv, kv.n_seqs, kv.lens.dtype, stream)
     elif not (new_lens.get_device() == kv._index and new_lens.dtype == kv.lens.dtype
               and new_lens.is_contiguous() and new_lens.numel() == kv.n_seqs):
         raise ValueError("new_lens must be contiguous int32 [n_seqs] on the cache's device")
     if workspace is None:
-        workspace = paged_evict_workspace(kv, budget)
+        workspace = paged_evict_workspace(kv, budget, stream)
     rc = lib.abra_paged_evict(kv._ref, budget, n_sink, n_recent, new_lens.data_ptr(), *_bytes(workspace, kv),
                               kv._stream(stream))
     if rc:

@@ -208,3 +208,33 @@ def test_results_do_not_go_over_the_queries(dev):
     q = torch.zeros(1, 1, 2, 64, dtype=torch.float16, device=dev)
     with pytest.raises(ValueError, match="memory"):
         A.paged_attention(_kv(R.to_dev(c, dev)), q, 0.1, out=q)
+
+
+def test_memory_on_the_calls_stream(dev, monkeypatch):
+    """Results and workspaces that a call allocates come from the pool of the
+    stream it runs on, where the memory is reused in the order of its work."""
+    import abra_b200 as A
+    from abra_b200 import paged
+
+    rng = np.random.default_rng(1)
+    c = R.make_cache(rng, [300], 2, 64, 16, "f16")
+    cd = R.to_dev(c, dev)
+    kv = _kv(cd, acc=cd["acc"], pos=cd["pos"])
+    q = torch.from_numpy(rng.standard_normal((1, 4, 64))).half().to(dev)
+    row = torch.randn(1, 2 * 64, device=dev)
+    taken = []
+    bytes_of = paged._bytes
+    monkeypatch.setattr(paged, "_bytes", lambda ws, kv: taken.append(ws) or bytes_of(ws, kv))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for stream in (side, side.cuda_stream):
+        taken += [A.paged_attention(kv, q, 0.1, accumulate=True, stream=stream), A.paged_evict(kv, 100, stream=stream),
+                  A.paged_append(kv, row, row, q=row, stream=stream)]
+    _no_error()
+    pool = {}
+    for seg in torch.cuda.memory_snapshot():
+        at = seg["address"]
+        for block in seg["blocks"]:
+            pool[at] = seg["stream"]
+            at += block["size"]
+    assert len(taken) == 10 and [pool[t.data_ptr()] for t in taken] == [side.cuda_stream] * 10
