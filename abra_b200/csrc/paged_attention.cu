@@ -241,6 +241,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
         for (int mt = 0; mt < S::KS; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.0f;
         m[0] = m[1] = -INFINITY;
         sub[0] = sub[1] = l[0] = l[1] = 0.0f;
+        bool odd = false;  // an infinity or NaN was taken out of a tile
 
         for (int base = sg.tile0 * STEP + warp * TILE; base < sg.slot_end; base += STEP) {
             // scores: slots g, g + 8 of the tile by rows 2c, 2c + 1; two sums, for
@@ -311,11 +312,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             }
             copy_wait<2 * S::DEPTH - 1>();
             __syncwarp();
-            // A slot that only some rows see has weight 0 in the others, and 0
-            // times an infinity or NaN in its V row would reach them: such
-            // elements count as zeros here and are added row by row below.
-            bool odd = false;
-            if (edge && p.n_q > 1) {
+            if (edge && p.n_q > 1) {  // not every row sees them all: unbounded_sum
 #pragma unroll 1
                 for (int i = 0; i < S::COPIES; ++i) {
                     const int x = 32 * i + lane, row = x / S::CHUNKS, chunk = x - row * S::CHUNKS;
@@ -325,7 +322,6 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
                                                finite_part<T>(v->w, any));
                     if (any) *v = y, odd = true;
                 }
-                odd = __any_sync(0xffffffffu, odd);
                 __syncwarp();
             }
 #pragma unroll
@@ -339,25 +335,6 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             fetch_v();
             at += 2 * S::TILE_BYTES;
             if (at == ring + S::DEPTH * 2 * S::TILE_BYTES) at = ring;
-            if (odd) {
-                for (int t = 0; t < TILE && base + t < sg.slot_end; ++t) {
-                    const int e = p.kv.page.div(base + t), page = max(0, paged_page(p.kv, sg.seq, e));
-                    const T *src = static_cast<const T *>(p.kv.a.v) +
-                                   paged_v_at(p.kv, page, head, base + t - e * p.kv.a.page_size) + g;
-                    const int from = (t & 7) * 4 + c;
-                    const float w0 = __shfl_sync(0xffffffffu, t < 8 ? sc[0] : sc[2], from);
-                    const float w1 = __shfl_sync(0xffffffffu, t < 8 ? sc[1] : sc[3], from);
-#pragma unroll
-                    for (int mt = 0; mt < S::KS; ++mt)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const float v = Half16<T>::up(src[16 * mt + 8 * y]);
-                            if (isfinite(v)) continue;
-                            if (base + t < seen(0)) o[mt][2 * y] += w0 * v;
-                            if (base + t < seen(1)) o[mt][2 * y + 1] += w1 * v;
-                        }
-                }
-            }
         }
 
         // ---- join the warps: maxima, then the scaled sums, two warps after two ----
@@ -367,7 +344,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             for (int x = 4; x <= 16; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
             if (g == 0) s_m[warp * ROWS + 2 * c + e] = m[e], s_l[warp * ROWS + 2 * c + e] = l[e];
         }
-        __syncthreads();
+        odd = __syncthreads_or(odd);
         auto top_of = [&](int r) {
             float top = s_m[r];
 #pragma unroll
@@ -405,6 +382,14 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             float4 sum = *reinterpret_cast<const float4 *>(s_o + r * S::PITCH + d);
             const float4 y = *reinterpret_cast<const float4 *>(s_o + (ROWS + r) * S::PITCH + d);
             sum.x += y.x, sum.y += y.y, sum.z += y.z, sum.w += y.w;
+            if (odd || isnan(sum.x + sum.y + sum.z + sum.w)) {
+                const int to = min(sg.slot_end, all_see + r / p.group);
+                auto replace = [&](float &x, int at) {
+                    const float z = unbounded_sum<T>(p, sg.seq, head, at, sg.tile0 * STEP, to);
+                    if (z != 0.0f) x = z;
+                };
+                replace(sum.x, d), replace(sum.y, d + 1), replace(sum.z, d + 2), replace(sum.w, d + 3);
+            }
             if (whole) {
                 finish_row<T>(p, sg.seq, head, r, d, D, sum, top, total);
             } else {

@@ -48,8 +48,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// What a sum relative to the maximum m counts relative to `top`.
-__device__ __forceinline__ float scaled(float m, float top) { return m == top ? 1.0f : exp2_fast(m - top); }
+// What a sum relative to the maximum m counts relative to `top`; never zero, so
+// that a sum of infinity stays one.
+__device__ __forceinline__ float scaled(float m, float top) { return m == top ? 1.0f : exp2_fast(fmaxf(m - top, -126.0f)); }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -187,6 +188,23 @@ __device__ __forceinline__ bool find_start(const PagedKv &kv, int blocks, int pi
     w.seq_begin = s_begin;
     w.length(s_len);
     return w.enter(kv);
+}
+
+// Infinities and NaNs among the values: a weight goes in as two 16-bit parts, of
+// which the second may be zero or negative, and a row that does not see a slot
+// gives it weight zero; either makes a NaN of what should be infinity or finite.
+// So the steps that not every row sees count such values as zeros, and an element
+// that saw one is set to their sum instead (0: there were none): slots [from, to)
+// of element d of head `head`.
+template <typename T>
+__device__ __noinline__ float unbounded_sum(const AttendArgs &p, int seq, int head, int d, int from, int to) {
+    float sum = 0.0f;
+    for (int t = from; t < to; ++t) {
+        const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, seq, e));
+        const float v = Half16<T>::up(static_cast<const T *>(p.kv.a.v)[paged_v_at(p.kv, page, head, t - e * p.kv.a.page_size) + d]);
+        if (!isfinite(v)) sum += v;
+    }
+    return sum;
 }
 
 template <typename T>

@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
             float l[NH];
 #pragma unroll
             for (int n = 0; n < NH; ++n) l[n] = 0.0f;
-            bool odd = false;  // an infinity or NaN among the values of a step that not all rows see
+            bool odd = false;  // an infinity or NaN was taken out of a step
             const int j0 = (r0 + n_first) / p.group, rem0 = r0 + n_first - j0 * p.group;  // query of this thread's first row, head in the group
             for (int t0 = sg.tile0 * WIDE_STEP; t0 < sg.slot_end; t0 += WIDE_STEP, ++it) {
                 const bool first = t0 == sg.tile0 * WIDE_STEP, edge = t0 + WIDE_STEP > all_see;
@@ -422,10 +422,7 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
                         tmem_wait_st();
                     }
                 }
-                // A slot that only some rows see has weight 0 in the others, and 0
-                // times an infinity or NaN in its V row would reach them: such
-                // elements count as zeros here and are added at the row's end.
-                if (edge && p.n_q > 1 && n_first == 0) {
+                if (edge && p.n_q > 1 && n_first == 0) {  // not every row sees them all: unbounded_sum
                     wait(&v_full[it % S::VS], (it / S::VS) & 1);
                     for (int c = 0; c < S::CHUNKS; ++c) {
                         uint4 *v = reinterpret_cast<uint4 *>(s_v + it % S::VS * S::TILE + (c >> 3) * S::PLANE +
@@ -477,7 +474,6 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
             named_bar_sync(1, S::COMPUTE);
             wait(&o_done, (it - 1) & 1);
             tc_fence_after();
-            const int odd_from = max(sg.tile0 * WIDE_STEP, all_see / WIDE_STEP * WIDE_STEP);  // the first step with an edge
 #pragma unroll 1
             for (int n0 = 0; n0 < NH; n0 += 16) {
                 const int n = n_first + n0, nr = min(16, p.rows - r0 - n);
@@ -485,18 +481,16 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
                 tmem_ld16(mine + t_o + n0, o);
                 tmem_wait_ld();
                 if (st >= D || nr <= 0) continue;
-                if (odd) {
-#pragma unroll 1
-                    for (int t = odd_from; t < sg.slot_end; ++t) {
-                        const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, sg.seq, e));
-                        const float v = Half16<T>::up(static_cast<const T *>(p.kv.a.v)[paged_v_at(p.kv, page, head, t - e * p.kv.a.page_size) + st]);
-                        if (isfinite(v)) continue;
-                        int j = (r0 + n) / p.group, rem = r0 + n - j * p.group;
+                bool unbounded = odd;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            if (t < all_see + min(j, p.n_q - 1)) o[i] += v;
-                            if (++rem == p.group) rem = 0, ++j;
-                        }
+                for (int i = 0; i < 16; ++i) unbounded |= isnan(o[i]);
+                if (unbounded) {
+                    int j = (r0 + n) / p.group, rem = r0 + n - j * p.group;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float z = unbounded_sum<T>(p, sg.seq, head, st, sg.tile0 * WIDE_STEP, min(sg.slot_end, all_see + min(j, p.n_q - 1)));
+                        if (z != 0.0f) o[i] = z;
+                        if (++rem == p.group) rem = 0, ++j;
                     }
                 }
                 if (!whole) {

@@ -210,6 +210,40 @@ def test_results_do_not_go_over_the_queries(dev):
         A.paged_attention(_kv(R.to_dev(c, dev)), q, 0.1, out=q)
 
 
+@pytest.mark.parametrize("dtype,d", [("f16", 128), ("bf16", 96)])
+@pytest.mark.parametrize("hq,n_q", [(4, 1), (4, 2), (3, 7), (24, 1), (8, 8), (30, 4)])
+def test_visible_infinities(dev, dtype, d, hq, n_q):
+    """An infinity or NaN among the values reaches its own element of the
+    queries that see the slot, as the sum of the formula does, and nothing else:
+    the other elements are the bits of a cache without it."""
+    import abra_b200 as A
+
+    rng = np.random.default_rng(hq + n_q)
+    lens = [5, 70, 200, 9000]
+    c = R.make_cache(rng, lens, 1, d, 16, dtype)
+    q = torch.from_numpy(2 * rng.standard_normal((len(lens), n_q, hq, d))).to(R.DTYPE[dtype])
+    bad = dict(c)
+    bad["v"], c["v"] = c["v"].clone(), c["v"].clone()
+    add = np.zeros((len(lens), max(lens), d))  # what a slot adds beside finite values
+    inf, nan = np.inf, np.nan
+    for b, n in enumerate(lens):
+        for e, t, x in ((0, 0, inf), (1, n - 1, -inf), (2, n // 2, nan), (3, n - 2, inf), (3, n // 3, inf), (4, n - 1, inf),
+                        (4, n // 3, -inf), (d - 1, n - 1, nan), (d - 2, n // 2, -inf)):
+            pg, off = int(c["table"][b, t // 16]), t % 16
+            bad["v"][pg, 0, off, e], c["v"][pg, 0, off, e] = x, 0.0
+            add[b, t, e] = x
+    for out_type in (R.DTYPE[dtype], torch.float32):
+        clean, got = (A.paged_attention(_kv(R.to_dev(x, dev)), q.to(dev), d**-0.5,
+                                        out=torch.empty(q.shape, dtype=out_type, device=dev)).cpu() for x in (c, bad))
+        _no_error()
+        assert torch.isfinite(clean).all()
+        for b, n in enumerate(lens):
+            for j in range(n_q):
+                seen = max(0, n - (n_q - 1 - j))
+                want = clean[b, j].double().numpy() + add[b, :seen].sum(0)
+                assert np.array_equal(got[b, j].double().numpy(), want, equal_nan=True), (b, j)
+
+
 def test_memory_on_the_calls_stream(dev, monkeypatch):
     """Results and workspaces that a call allocates come from the pool of the
     stream it runs on, where the memory is reused in the order of its work."""
