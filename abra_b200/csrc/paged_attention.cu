@@ -415,6 +415,10 @@ struct Parts {
 
 constexpr int JOIN_WARPS = 8, JOIN_THREADS = JOIN_WARPS * 32;
 constexpr int ACC_ROWS = 64;  // rows whose lse is held at a time
+// CTAs that accumulate, on a multiprocessor; four of them fit, and those that
+// join come behind them (the other way round, with two lanes a slot and three
+// CTAs: 36 against 32 us for 16 sequences of up to 8,192 slots, 64 heads).
+constexpr int ACC_CTAS = 4;
 
 struct JoinArgs {
     AttendArgs a;
@@ -502,20 +506,28 @@ template <typename T, int D> __device__ __forceinline__ void join_rows(const Joi
 }
 
 // acc += the slots' weights, exp2(score - lse) summed over the rows, on pieces
-// of the same kind of line; two neighbouring lanes share a slot.  A row's lse
-// comes from its parts, so this needs the first kernel only.
+// of the same kind of line; a lane takes eight rows of a slot, as many lanes a
+// slot as a block has eights.  A row's lse comes from its parts, so this needs
+// the first kernel only.
 __device__ __forceinline__ void accumulate(const JoinArgs &ja, int cta, int ctas) {
     const AttendArgs &p = ja.a;
-    __shared__ float s_lse[ACC_ROWS];
-    const int tid = threadIdx.x, heads = p.kv.a.n_kv_heads, half = tid & 1, padded = p.row_blocks * ja.block;
+    __shared__ __align__(16) float s_lse[ACC_ROWS];
+    const int tid = threadIdx.x, heads = p.kv.a.n_kv_heads, lanes = ja.block / 8, slots = JOIN_THREADS / lanes;
+    const int mine = 8 * (tid % lanes), padded = p.row_blocks * ja.block;
     Walk<STEP> w;
     Line line(0, 0);
     if (!find_start<JOIN_THREADS>(p.kv, 1, cta, ctas, ctas, line, w)) return;
+    // rows that see nothing, and what lies behind the last row, have an lse of +infinity and no weight
+    auto weight = [](float x, float lse) { return lse == INFINITY ? 0.0f : exp2_fast(x - lse); };
     do {
         const Segment &sg = w.s;
+        const int first = sg.tile0 * STEP + tid / lanes;  // this thread's slot, and every `slots` after it
+        auto page_of = [&](int t) { return t < sg.slot_end ? paged_page(p.kv, sg.seq, p.kv.page.div(t)) : -1; };
         for (int r0 = 0; r0 < p.rows; r0 += ACC_ROWS) {
             const int nr = min(ACC_ROWS, p.rows - r0);
+            int page = page_of(first);  // runs beside the rows' lse
             __syncthreads();
+            if (tid < ACC_ROWS && tid >= nr) s_lse[tid] = INFINITY;
             for (int i = tid >> 5; i < nr; i += JOIN_WARPS) {  // a warp a row
                 const int r = r0 + i, block = r / ja.block;
                 const int64_t triple = (static_cast<int64_t>(sg.seq) * heads + sg.head);
@@ -541,28 +553,28 @@ __device__ __forceinline__ void accumulate(const JoinArgs &ja, int cta, int ctas
                     }
                     lse = total != 0.0f ? top + log2f(total) : -INFINITY;
                 }
-                if (lane == 0) s_lse[i] = lse == -INFINITY ? INFINITY : lse;  // a row that sees nothing weighs nothing
+                if (lane == 0) s_lse[i] = lse == -INFINITY ? INFINITY : lse;
             }
             __syncthreads();
-            for (int t0 = sg.tile0 * STEP; t0 < sg.slot_end; t0 += JOIN_THREADS / 2) {
-                const int t = t0 + (tid >> 1);
-                float sum = 0.0f;
-                int64_t meta = -1;
-                if (t < sg.slot_end) {
-                    const int e = p.kv.page.div(t), page = paged_page(p.kv, sg.seq, e);
-                    if (page >= 0) {
-                        meta = paged_meta_at(p.kv, page, sg.head, t - e * p.kv.a.page_size);
-                        for (int i = 4 * half; i < nr; i += 8) {
-                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p.scores + meta * padded + r0 + i));
-                            sum += exp2_fast(x.x - s_lse[i]);
-                            if (i + 1 < nr) sum += exp2_fast(x.y - s_lse[i + 1]);
-                            if (i + 2 < nr) sum += exp2_fast(x.z - s_lse[i + 2]);
-                            if (i + 3 < nr) sum += exp2_fast(x.w - s_lse[i + 3]);
-                        }
-                    }
+            for (int t = first; t - tid / lanes < sg.slot_end; t += slots) {
+                const int64_t meta = page < 0 ? -1 : paged_meta_at(p.kv, page, sg.head, t - p.kv.page.div(t) * p.kv.a.page_size);
+                const float acc = meta >= 0 && mine == 0 ? p.kv.a.acc[meta] : 0.0f;
+                float4 x[2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    x[y] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (meta >= 0 && mine + 4 * y < nr)
+                        x[y] = __ldcg(reinterpret_cast<const float4 *>(p.scores + meta * padded + r0 + mine + 4 * y));
                 }
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                if (meta >= 0 && half == 0) p.kv.a.acc[meta] += sum;
+                page = page_of(t + slots);
+                float sum = 0.0f;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const float4 lse = *reinterpret_cast<const float4 *>(s_lse + mine + 4 * y);
+                    sum += weight(x[y].x, lse.x) + weight(x[y].y, lse.y) + weight(x[y].z, lse.z) + weight(x[y].w, lse.w);
+                }
+                for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                if (meta >= 0 && mine == 0) p.kv.a.acc[meta] = acc + sum;
             }
         }
     } while (w.next(p.kv));
@@ -570,12 +582,13 @@ __device__ __forceinline__ void accumulate(const JoinArgs &ja, int cta, int ctas
 
 // The second kernel: it writes the rows of empty sequences (zeros), joins the
 // rows that were split, and adds the slots' weights, side by side.
-template <typename T, int D> __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ JoinArgs ja) {
+template <typename T, int D, bool SCORES> __global__ void __launch_bounds__(JOIN_THREADS, SCORES ? 4 : 3) join_kernel(const __grid_constant__ JoinArgs ja) {
     pdl_wait();
     pdl_launch_dependents();
     const int cta = blockIdx.x;
-    if (cta < ja.joins) join_rows<T, D>(ja, cta);
-    else accumulate(ja, cta - ja.joins, gridDim.x - ja.joins);
+    const int adding = SCORES ? gridDim.x - ja.joins : 0;
+    if (SCORES && cta < adding) accumulate(ja, cta, adding);
+    else join_rows<T, D>(ja, cta - adding);
 }
 
 // ------------------------------------------------------------------ host ---
@@ -630,7 +643,8 @@ template <typename T, int D> cudaError_t launch_all(const AttendArgs &p, const P
     while (warps > 1 && groups * p.rows * warps > pl.sms * 4 * JOIN_WARPS) warps /= 2;
     const int per = JOIN_WARPS / warps, row_ctas = (p.rows + per - 1) / per;
     const JoinArgs ja{p, pl.block, warps, row_ctas, static_cast<int>(groups * row_ctas)};
-    return paged_launch(join_kernel<T, D>, dim3(ja.joins + (accumulate ? pl.sms * 4 : 0)), JOIN_THREADS, 0, st, ja);
+    return accumulate ? paged_launch(join_kernel<T, D, true>, dim3(ja.joins + pl.sms * ACC_CTAS), JOIN_THREADS, 0, st, ja)
+                      : paged_launch(join_kernel<T, D, false>, dim3(ja.joins), JOIN_THREADS, 0, st, ja);
 }
 template <typename T> cudaError_t launch(const AttendArgs &p, const Plan &pl, bool accumulate, cudaStream_t st) {
     switch (p.kv.a.head_dim) {
