@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             for (int e = 0; e < 4; ++e) {
                 sc[e] = (part[0][e] + part[1][e]) * p.scale_log2;
                 if (edge && base + g + 8 * (e >> 1) >= seen(e & 1)) sc[e] = -INFINITY;
-                raise |= sc[e] > m[e & 1] + RAISE;
+                raise |= sc[e] - m[e & 1] > Weigh<T>::RAISE;
             }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             uint32_t hi[2], lo[2];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                sc[e] = exp2_fast(sc[e] - sub[e & 1]);
+                sc[e] = weight_of<T>(sc[e], sub[e & 1]);
                 l[e & 1] += sc[e];
             }
 #pragma unroll
@@ -509,7 +509,7 @@ template <typename T, int D> __device__ __forceinline__ void join_rows(const Joi
 // of the same kind of line; a lane takes eight rows of a slot, as many lanes a
 // slot as a block has eights.  A row's lse comes from its parts, so this needs
 // the first kernel only.
-__device__ __forceinline__ void accumulate(const JoinArgs &ja, int cta, int ctas) {
+template <typename T> __device__ __forceinline__ void accumulate(const JoinArgs &ja, int cta, int ctas) {
     const AttendArgs &p = ja.a;
     __shared__ __align__(16) float s_lse[ACC_ROWS];
     const int tid = threadIdx.x, heads = p.kv.a.n_kv_heads, lanes = ja.block / 8, slots = JOIN_THREADS / lanes;
@@ -551,7 +551,7 @@ __device__ __forceinline__ void accumulate(const JoinArgs &ja, int cta, int ctas
                         total = total * scaled(top, t) + on * scaled(ot, t);
                         top = t;
                     }
-                    lse = total != 0.0f ? top + log2f(total) : -INFINITY;
+                    lse = row_lse2<T>(top, total);
                 }
                 if (lane == 0) s_lse[i] = lse == -INFINITY ? INFINITY : lse;
             }
@@ -587,7 +587,7 @@ template <typename T, int D, bool SCORES> __global__ void __launch_bounds__(JOIN
     pdl_launch_dependents();
     const int cta = blockIdx.x;
     const int adding = SCORES ? gridDim.x - ja.joins : 0;
-    if (SCORES && cta < adding) accumulate(ja, cta, adding);
+    if (SCORES && cta < adding) accumulate<T>(ja, cta, adding);
     else join_rows<T, D>(ja, cta - adding);
 }
 

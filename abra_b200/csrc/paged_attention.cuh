@@ -10,9 +10,23 @@ constexpr int PIECE = 16;                 // steps of a piece, where there are e
                                           // with 8, and so twice the parts to join, 111)
 constexpr int WAVES = 4;                  // pieces for each CTA that the GPU holds, at most; the wide kernel's CTA fills its
                                           // multiprocessor, so that nothing runs beside a new one's start, and takes one
-// A row's maximum is raised only when a score passes it by 2^RAISE: weights
-// stay below 2^RAISE (well inside fp16), and most tiles need no reduction.
-constexpr float RAISE = 10.0f;
+// A row's weights are 2^(s - m + SHIFT) of its running maximum m, and so are its
+// sums until its log-sum-exp takes SHIFT off again.  m is raised only when a score
+// passes it by RAISE, so that most tiles need no reduction; weights stay below
+// 2^(RAISE + SHIFT), for which compare and weight both take the difference s - m
+// first (m + RAISE or m - SHIFT would be rounded where m is large).  bf16 has
+// fp32's range.  fp16 ends at 2^-24, so its weights go up to the top of its range:
+// of a weight at most 2^-36 of the row's largest is lost, without SHIFT 2^-25,
+// which beside a slot far above the others is all of them.  RAISE 2 and SHIFT 13
+// raise more often than they are worth (16 new tokens of four sequences of up to
+// 8,192 slots 26.5 us, 25.6 with 4 and 11, 25.4 with 10 and 5).
+template <typename T> struct Weigh;
+template <> struct Weigh<__half> {
+    static constexpr float RAISE = 4.0f, SHIFT = 11.0f;
+};
+template <> struct Weigh<__nv_bfloat16> {
+    static constexpr float RAISE = 10.0f, SHIFT = 0.0f;
+};
 // What beginning and ending a row costs beside its steps, in steps (its
 // queries, the join of its warps): with 1 the pieces full of short rows end
 // last (25.8 against 23.9 us for 32 sequences of 1 to 4,096 slots), with 3
@@ -47,6 +61,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// A score's weight against `ref`, the row's maximum (0 while that is -infinity).
+template <typename T> __device__ __forceinline__ float weight_of(float s, float ref) {
+    return exp2_fast(Weigh<T>::SHIFT != 0.0f ? s - ref + Weigh<T>::SHIFT : s - ref);
 }
 // What a sum relative to the maximum m counts relative to `top`; never zero, so
 // that a sum of infinity stays one.
@@ -216,10 +234,16 @@ __device__ __forceinline__ void store_out(const AttendArgs &p, int64_t at, float
     }
 }
 
+// log2 of a row's sum of 2^s.
+template <typename T> __device__ __forceinline__ float row_lse2(float m, float total) {
+    return total != 0.0f ? m + (log2f(total) - Weigh<T>::SHIFT) : -INFINITY;
+}
+
 // A finished row's lse; total == 0: the row saw nothing.
+template <typename T>
 __device__ __forceinline__ void finish_lse(const AttendArgs &p, int seq, int head, int r, float m, float total) {
     const int j = r / p.group, h = head * p.group + r - j * p.group;
-    const float l2 = total != 0.0f ? m + log2f(total) : -INFINITY;
+    const float l2 = row_lse2<T>(m, total);
     if (p.lse) p.lse[(static_cast<int64_t>(seq) * p.n_q + j) * p.n_heads + h] = l2 * 0.69314718055994531f;
     if (p.row_lse) p.row_lse[(static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.rows + r] = l2;
 }
@@ -233,7 +257,7 @@ __device__ __forceinline__ void finish_row(const AttendArgs &p, int seq, int hea
     const float inv = total != 0.0f ? 1.0f / total : 0.0f;
     store_out<T>(p, row * p.ldo + static_cast<int64_t>(h) * D + d,
                  total != 0.0f ? make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv) : make_float4(0, 0, 0, 0));
-    if (d == 0) finish_lse(p, seq, head, r, m, total);
+    if (d == 0) finish_lse<T>(p, seq, head, r, m, total);
 }
 
 // The kernel for blocks of 16 to 64 rows (paged_attention_wide.cu); one CTA a

@@ -14,7 +14,7 @@
 // rings of tiles, one warp issues the tensor core's work, and a thread of the
 // four or eight compute warps stands for a slot.  Per step
 //   S^T[128 slots x N] = K Q^T      (M 128, N rows, K = D)
-//   P^T = 2^(S^T - m), split into two 16-bit values, to shared memory
+//   P^T = 2^(S^T - m + SHIFT), split into two 16-bit values, to shared memory
 //   O^T[D x N] += V^T P^T           (M 128, K = 128 slots, twice)
 // with S^T (two buffers) and O^T in tensor memory, all operands in shared memory
 // in rows of 128 bytes (64 elements; wider rows in planes) with the 128-byte
@@ -379,7 +379,8 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
 #pragma unroll
                 for (int n0 = 0; n0 < NH; n0 += 4) {
                     const float4 m = *reinterpret_cast<const float4 *>(s_m + n_first + n0);
-                    raise |= s[n0] > m.x + RAISE || s[n0 + 1] > m.y + RAISE || s[n0 + 2] > m.z + RAISE || s[n0 + 3] > m.w + RAISE;
+                    raise |= s[n0] - m.x > Weigh<T>::RAISE || s[n0 + 1] - m.y > Weigh<T>::RAISE || s[n0 + 2] - m.z > Weigh<T>::RAISE ||
+                             s[n0 + 3] - m.w > Weigh<T>::RAISE;
                 }
                 if (SCORES && t < sg.slot_end) {
                     const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, sg.seq, e));
@@ -442,7 +443,7 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
                     for (int i = 0; i < 8; i += 2) {
                         const int n = n0 + i;
                         const float2 sub = *reinterpret_cast<const float2 *>(s_sub + n_first + n);
-                        const float a = exp2_fast(s[n] - sub.x), b = exp2_fast(s[n + 1] - sub.y);
+                        const float a = weight_of<T>(s[n], sub.x), b = weight_of<T>(s[n + 1], sub.y);
                         l[n] += a;
                         l[n + 1] += b;
                         hi[i / 2] = pack2<T>(a, b);
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
             const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (w.pos == begin ? 0 : 1);
             if (tid < N && r0 + tid < p.rows) {
                 const float total = w_sum[tid] + w_sum[N + tid] + w_sum[2 * N + tid] + w_sum[3 * N + tid];
-                if (whole) finish_lse(p, sg.seq, head, r0 + tid, s_m[tid], total);
+                if (whole) finish_lse<T>(p, sg.seq, head, r0 + tid, s_m[tid], total);
                 else p.part_ml[slot * N + tid] = make_float2(s_m[tid], total);
                 s_fac[tid] = total != 0.0f ? 1.0f / total : 0.0f;
             }
