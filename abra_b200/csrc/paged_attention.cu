@@ -287,8 +287,8 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const int t = base + g + 8 * x, e = p.kv.page.div(t);
-                    if (t < sg.slot_end) {
-                        const int page = max(0, paged_page(p.kv, sg.seq, e));
+                    const int page = t < sg.slot_end ? paged_page(p.kv, sg.seq, e) : -1;
+                    if (page >= 0) {  // a page outside the pool has no place for them
                         float *to = p.scores + paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size) * ROWS;
                         *reinterpret_cast<float2 *>(to + 2 * c) = make_float2(sc[2 * x], sc[2 * x + 1]);
                     }
