@@ -97,7 +97,7 @@ template <int D> struct Shape {
     static constexpr int TILE_BYTES = TILE * ROW;             // K or V of one tile
     static constexpr int STAGE = AT_WARPS * 2 * TILE_BYTES;   // the CTA's K and V tiles
     static constexpr int PITCH = D + 4;                       // floats of a row in a join buffer
-    static constexpr int JOIN_BYTES = 2 * ROWS * PITCH * 4 + 2 * AT_WARPS * ROWS * 4;
+    static constexpr int JOIN_BYTES = 2 * ROWS * PITCH * 4 + 2 * AT_WARPS * ROWS * 4 + ROWS * D / 4;
     // the ring: as many tiles as leave room for the CTAs (1 KB each is the system's)
     static constexpr int DEPTH = (233472 / CTAS - 1024 - 256 - JOIN_BYTES) / STAGE;
     static constexpr int SMEM = DEPTH * STAGE + JOIN_BYTES;
@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
     extern __shared__ __align__(256) unsigned char smem[];  // the ring: [warp][stage][K, V][row]
     float *s_o = reinterpret_cast<float *>(smem + S::DEPTH * S::STAGE);  // [2][ROWS][PITCH]
     float *s_m = s_o + 2 * ROWS * S::PITCH, *s_l = s_m + AT_WARPS * ROWS;  // [warp][ROWS]
+    uint32_t *s_saw = reinterpret_cast<uint32_t *>(s_l + AT_WARPS * ROWS);  // [ROWS][D] codes of two bits
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
 
     pdl_wait();
@@ -312,7 +313,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             }
             copy_wait<2 * S::DEPTH - 1>();
             __syncwarp();
-            if (edge && p.n_q > 1) {  // not every row sees them all: unbounded_sum
+            if (edge && p.n_q > 1) {  // not every row sees them all: look_through
 #pragma unroll 1
                 for (int i = 0; i < S::COPIES; ++i) {
                     const int x = 32 * i + lane, row = x / S::CHUNKS, chunk = x - row * S::CHUNKS;
@@ -344,6 +345,14 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             for (int x = 4; x <= 16; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
             if (g == 0) s_m[warp * ROWS + 2 * c + e] = m[e], s_l[warp * ROWS + 2 * c + e] = l[e];
         }
+        // a NaN that the row's weights do not explain comes from the values
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int mt = 0; mt < S::KS; ++mt) sum[0] += o[mt][e], sum[1] += o[mt][e + 2];
+            odd |= isnan(sum[0] + sum[1]) && !isnan(l[e]);
+        }
         odd = __syncthreads_or(odd);
         auto top_of = [&](int r) {
             float top = s_m[r];
@@ -370,6 +379,12 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             }
             __syncthreads();
         }
+        if (odd) {
+            for (int i = tid; i < ROWS * D / 16; i += AT_THREADS) s_saw[i] = 0;
+            __syncthreads();
+            look_through<T, D, AT_THREADS>(p, sg.seq, head, sg.tile0 * STEP, sg.slot_end, all_see, 0, p.rows, tid, s_saw);
+            __syncthreads();
+        }
         const bool whole = sg.tile0 == 0 && sg.tile1 == sg.n;
         const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (w.pos == begin ? 0 : 1);
         for (int i = tid; i < ROWS * (D / 4); i += AT_THREADS) {
@@ -382,13 +397,10 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
             float4 sum = *reinterpret_cast<const float4 *>(s_o + r * S::PITCH + d);
             const float4 y = *reinterpret_cast<const float4 *>(s_o + (ROWS + r) * S::PITCH + d);
             sum.x += y.x, sum.y += y.y, sum.z += y.z, sum.w += y.w;
-            if (odd || isnan(sum.x + sum.y + sum.z + sum.w)) {
-                const int to = min(sg.slot_end, all_see + r / p.group);
-                auto replace = [&](float &x, int at) {
-                    const float z = unbounded_sum<T>(p, sg.seq, head, at, sg.tile0 * STEP, to);
-                    if (z != 0.0f) x = z;
-                };
-                replace(sum.x, d), replace(sum.y, d + 1), replace(sum.z, d + 2), replace(sum.w, d + 3);
+            if (odd) {
+                const int at = r * D + d;
+                sum = make_float4(with_saw(sum.x, s_saw, at), with_saw(sum.y, s_saw, at + 1), with_saw(sum.z, s_saw, at + 2),
+                                  with_saw(sum.w, s_saw, at + 3));
             }
             if (whole) {
                 finish_row<T>(p, sg.seq, head, r, d, D, sum, top, total);

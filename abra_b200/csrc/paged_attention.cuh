@@ -211,18 +211,66 @@ __device__ __forceinline__ bool find_start(const PagedKv &kv, int blocks, int pi
 // Infinities and NaNs among the values: a weight goes in as two 16-bit parts, of
 // which the second may be zero or negative, and a row that does not see a slot
 // gives it weight zero; either makes a NaN of what should be infinity or finite.
-// So the steps that not every row sees count such values as zeros, and an element
-// that saw one is set to their sum instead (0: there were none): slots [from, to)
-// of element d of head `head`.
-template <typename T>
-__device__ __noinline__ float unbounded_sum(const AttendArgs &p, int seq, int head, int d, int from, int to) {
-    float sum = 0.0f;
-    for (int t = from; t < to; ++t) {
-        const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, seq, e));
-        const float v = Half16<T>::up(static_cast<const T *>(p.kv.a.v)[paged_v_at(p.kv, page, head, t - e * p.kv.a.page_size) + d]);
-        if (!isfinite(v)) sum += v;
+// So the steps that not every row sees count such values as zeros, and where a
+// segment met one (or a row has a NaN that its weights do not explain) its values
+// are looked through once more: an element that is not finite among the slots that
+// a row sees becomes the sum of what is not.
+enum : uint32_t { SAW_PLUS = 1, SAW_MINUS = 2, SAW_NAN = SAW_PLUS | SAW_MINUS };  // and so both infinities are a NaN
+
+// Which of them are in 16 bits.
+template <typename T> __device__ __forceinline__ uint32_t saw(uint32_t x) {
+    constexpr uint32_t INF = Half16<T>::type == ABRA_GGML_F16 ? 0x7c00u : 0x7f80u;
+    x &= 0xffffu;
+    return (x & 0x7fffu) < INF ? 0u : (x & 0x7fffu) > INF ? SAW_NAN : x >> 15 ? SAW_MINUS : SAW_PLUS;
+}
+// Codes are two bits an element, 16 elements a word: element i's, where x becomes
+// the sum of what is not finite.
+__device__ __forceinline__ float with_saw(float x, const uint32_t *codes, int i) {
+    const uint32_t seen = codes[i >> 4] >> 2 * (i & 15) & 3u;
+    return seen == 0 ? x : seen == SAW_PLUS ? INFINITY : seen == SAW_MINUS ? -INFINITY : NAN;
+}
+
+// Collects in codes [row][D], zeros before, what rows r0 .. r0 + n - 1 see in
+// slots [from, to); row r sees those before all_see + r / group.  All THREADS
+// threads, between barriers.  One more read of the segment's values, 16 bytes a
+// lane and four in flight (8 sequences of 4,096 slots with an infinity each, 64
+// rows a kv head: 66 us for 31 without them; each thread's own walk of one slot
+// after the other took 5,000).
+template <typename T, int D, int THREADS>
+__device__ __noinline__ void look_through(const AttendArgs &p, int seq, int head, int from, int to, int all_see, int r0, int n,
+                                          int tid, uint32_t *codes) {
+    constexpr int CH = D / 8, BATCH = 4;
+    const int64_t end = static_cast<int64_t>(to - from) * CH;
+    for (int64_t x0 = tid; x0 < end; x0 += BATCH * THREADS) {
+        uint4 v[BATCH];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            const int64_t x = x0 + b * THREADS;
+            const int t = from + static_cast<int>(x / CH);
+            v[b] = make_uint4(0, 0, 0, 0);
+            if (x < end) {
+                const int e = p.kv.page.div(t), page = max(0, paged_page(p.kv, seq, e));
+                v[b] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.kv.a.v) +
+                                                        paged_v_at(p.kv, page, head, t - e * p.kv.a.page_size) + 8 * (x % CH));
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            const uint32_t w[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+            uint32_t code = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) code |= saw<T>(w[i / 2] >> 16 * (i % 2)) << 2 * i;
+            if (code == 0) continue;
+            const int64_t x = x0 + b * THREADS;
+            const int t = from + static_cast<int>(x / CH), chunk = static_cast<int>(x % CH);
+            code <<= 16 * (chunk % 2);
+            const int64_t first = static_cast<int64_t>(t - all_see + 1) * p.group - r0;  // the first row that sees it
+            for (int r = static_cast<int>(max(static_cast<int64_t>(0), first)); r < n; ++r) {
+                uint32_t *at = codes + r * (D / 16) + chunk / 2;
+                if (code & ~*reinterpret_cast<volatile uint32_t *>(at)) atomicOr(at, code);
+            }
+        }
     }
-    return sum;
 }
 
 template <typename T>

@@ -162,6 +162,34 @@ template <int N, typename Op> __device__ __forceinline__ void fold_lanes(float (
 // Where fold_lanes leaves element e of lane l.
 template <int N> __device__ __forceinline__ int folded(int lane, int e) { return N >= 32 ? lane * (N / 32) + e : lane >> 1; }
 
+// Puts the infinities and NaNs that each row sees into its results (look_through),
+// in tensor memory at `at`; all compute warps.  `codes`: [N][D], the place of the
+// weights, which are at rest between two rows.
+template <typename T, int D, int N>
+__device__ __noinline__ void correct_results(const AttendArgs &p, int seq, int head, int from, int to, int all_see, int r0, uint32_t at,
+                                             uint32_t *codes) {
+    using S = Wide<D, N>;
+    static_assert(N * D / 4 <= 2 * S::P_BYTES, "the codes fit the weights' place");
+    const int tid = threadIdx.x, st = tid & 127, n_first = (tid >> 7) * S::NH;
+    for (int i = tid; i < N * D / 16; i += S::COMPUTE) codes[i] = 0;
+    named_bar_sync(1, S::COMPUTE);
+    look_through<T, D, S::COMPUTE>(p, seq, head, from, to, all_see, r0, min(N, p.rows - r0), tid, codes);
+    named_bar_sync(1, S::COMPUTE);
+#pragma unroll 1
+    for (int n0 = 0; n0 < S::NH; n0 += 16) {
+        float o[16];
+        tmem_ld16(at + n0, o);
+        tmem_wait_ld();
+        if (st < D) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = with_saw(o[i], codes, (n_first + n0 + i) * D + st);
+        }
+        __syncwarp();
+        tmem_st16(at + n0, o);
+    }
+    tmem_wait_st();
+}
+
 template <typename T, int D, int N, bool SCORES>
 __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(const __grid_constant__ AttendArgs p) {
     using S = Wide<D, N>;
@@ -425,7 +453,7 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
                         tmem_wait_st();
                     }
                 }
-                if (edge && p.n_q > 1 && n_first == 0) {  // not every row sees them all: unbounded_sum
+                if (edge && p.n_q > 1 && n_first == 0) {  // not every row sees them all: look_through
                     wait(&v_full[it % S::VS], (it / S::VS) & 1);
                     for (int c = 0; c < S::CHUNKS; ++c) {
                         uint4 *v = reinterpret_cast<uint4 *>(s_v + it % S::VS * S::TILE + (c >> 3) * S::PLANE +
@@ -477,49 +505,55 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
             named_bar_sync(1, S::COMPUTE);
             wait(&o_done, (it - 1) & 1);
             tc_fence_after();
-#pragma unroll 1
-            for (int n0 = 0; n0 < NH; n0 += 16) {
-                const int n = n_first + n0, nr = min(16, p.rows - r0 - n);
-                float o[16];
-                tmem_ld16(mine + t_o + n0, o);
-                tmem_wait_ld();
-                if (st >= D || nr <= 0) continue;
-                bool unbounded = odd;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) unbounded |= isnan(o[i]);
-                if (unbounded) {
-                    int j = (r0 + n) / p.group, rem = r0 + n - j * p.group;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float z = unbounded_sum<T>(p, sg.seq, head, st, sg.tile0 * WIDE_STEP, min(sg.slot_end, all_see + min(j, p.n_q - 1)));
-                        if (z != 0.0f) o[i] = z;
-                        if (++rem == p.group) rem = 0, ++j;
-                    }
-                }
-                if (!whole) {
-                    float *to = p.part_o + (slot * N + n) * D + st;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (i < nr) to[i * D] = o[i];
-                } else {
-                    int j = (r0 + n) / p.group, rem = r0 + n - j * p.group;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int64_t to = (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldo + static_cast<int64_t>(head * p.group + rem) * D + st;
-                        const float x = s_fac[n + i] != 0.0f ? o[i] * s_fac[n + i] : 0.0f;
-                        if (i < nr) {
-                            if (p.out_f32) static_cast<float *>(p.out)[to] = x;
-                            else static_cast<T *>(p.out)[to] = Half16<T>::down(x);
-                        }
-                        if (++rem == p.group) rem = 0, ++j;
-                    }
-                }
-            }
             if (sg.tile0 == 0 && tid == 0)
                 p.split[static_cast<int64_t>(sg.seq) * w.units + sg.unit] =
                     make_int2(static_cast<int>(slot), whole ? static_cast<int>(blockIdx.x) : line.piece(sg.row_begin + ROW_COST + sg.n - 1));
-            tc_fence_before();
-            named_bar_sync(1, S::COMPUTE);  // Q, the sums and the results are free again
+            auto look = [&]() {
+                correct_results<T, D, N>(p, sg.seq, head, sg.tile0 * WIDE_STEP, sg.slot_end, all_see, r0, mine + t_o, reinterpret_cast<uint32_t *>(s_p));
+            };
+            if (odd) look();
+            for (;;) {
+                bool unexplained = false;  // a NaN of a row whose weights have none
+#pragma unroll 1
+                for (int n0 = 0; n0 < NH; n0 += 16) {
+                    const int n = n_first + n0, nr = min(16, p.rows - r0 - n);
+                    float o[16];
+                    tmem_ld16(mine + t_o + n0, o);
+                    tmem_wait_ld();
+                    if (st >= D || nr <= 0) continue;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[i % 4] += o[i];
+                    if (isnan((sum[0] + sum[1]) + (sum[2] + sum[3]))) {
+#pragma unroll 1
+                        for (int i = 0; i < nr; ++i) unexplained |= !isnan(s_fac[n + i]);
+                    }
+                    if (!whole) {
+                        float *to = p.part_o + (slot * N + n) * D + st;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (i < nr) to[i * D] = o[i];
+                    } else {
+                        int j = (r0 + n) / p.group, rem = r0 + n - j * p.group;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int64_t to = (static_cast<int64_t>(sg.seq) * p.n_q + j) * p.ldo + static_cast<int64_t>(head * p.group + rem) * D + st;
+                            const float x = s_fac[n + i] != 0.0f ? o[i] * s_fac[n + i] : 0.0f;
+                            if (i < nr) {
+                                if (p.out_f32) static_cast<float *>(p.out)[to] = x;
+                                else static_cast<T *>(p.out)[to] = Half16<T>::down(x);
+                            }
+                            if (++rem == p.group) rem = 0, ++j;
+                        }
+                    }
+                }
+                tc_fence_before();
+                // Q, the sums and the results are free again, or are stored once more
+                if (!compute_any<S::COMPUTE>(!odd && unexplained)) break;
+                tc_fence_after();
+                odd = true;
+                look();
+            }
         } while (w.next(p.kv));
     }
     __syncthreads();
