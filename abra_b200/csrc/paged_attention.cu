@@ -708,7 +708,10 @@ extern "C" int abra_paged_attention(const abra_paged_kv *kv, const void *q, int6
     if (!paged_aligned(workspace, 256)) return paged_fail(ABRA_E_INVALID, "the workspace must be 256-byte aligned");
     if (workspace_bytes < 256) return paged_fail(ABRA_E_INVALID, "workspace of %lld bytes", (long long)workspace_bytes);
     if (kv->n_seqs == 0) return ABRA_OK;
-    if (q == out) return paged_fail(ABRA_E_INVALID, "out must not be q's memory");
+    // rows are finished while others' queries are still to be read
+    const int64_t width = static_cast<int64_t>(n_heads) * kv->head_dim, out_bytes = out_type == ABRA_GGML_F32 ? 4 : 2;
+    if (paged_overlap({q, 2 * width, 2 * ldq}, {out, out_bytes * width, out_bytes * ldo}, static_cast<int64_t>(kv->n_seqs) * n_q))
+        return paged_fail(ABRA_E_INVALID, "out must not share q's memory");
     const bool accumulate = flags & ABRA_PAGED_ACCUMULATE;
     Plan pl;
     rc = make_plan(kv, n_heads, n_q, accumulate, pl);

@@ -95,6 +95,22 @@ inline int paged_fail(int code, const char *fmt, ...) {
 }
 inline bool paged_aligned(const void *p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// Rows in memory: `width` bytes every `stride`.
+struct PagedRows {
+    const void *at;
+    int64_t width, stride;
+};
+// Whether two tensors of n rows share memory.  Columns of the same wider rows do
+// not, though they lie in one range.
+inline bool paged_overlap(PagedRows a, PagedRows b, int64_t n) {
+    const __int128 a0 = reinterpret_cast<uintptr_t>(a.at), b0 = reinterpret_cast<uintptr_t>(b.at);
+    const __int128 a1 = a0 + static_cast<__int128>(n - 1) * a.stride + a.width, b1 = b0 + static_cast<__int128>(n - 1) * b.stride + b.width;
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (a.stride != b.stride) return true;
+    const __int128 gap = b0 >= a0 ? (b0 - a0) % a.stride : (a.stride - (a0 - b0) % a.stride) % a.stride;  // from a's columns to b's
+    return gap < a.width || gap + b.width > a.stride;
+}
+
 // The checks every entry point makes of the cache it is given.
 inline int paged_check(const abra_paged_kv *kv) {
     if (!kv) return paged_fail(ABRA_E_INVALID, "null cache");

@@ -541,9 +541,9 @@ int abra_paged_append(const abra_paged_kv *kv, const void *q, const void *k, con
 /* Attention of each sequence's newest n_q tokens over its cache: query j (0 ..
  * n_q - 1) of sequence s sees slots 0 .. lens[s] - n_q + j, q head h reads kv
  * head h / (n_heads / n_kv_heads), out = sum_t softmax_t(scale q.k_t) v_t.
- * q (the pools' type) and out (out_type: the pools' type or F32, other memory
- * than q) have row (s * n_q + j) at stride ldq / ldo; lse (or NULL), fp32 [n_seqs][n_q][n_heads],
- * takes log sum_t exp(scale q.k_t).  A query that sees no slot gives zeros and
+ * q (the pools' type) and out (out_type: the pools' type or F32) have row (s *
+ * n_q + j) at stride ldq / ldo and share no memory (they may be columns of the
+ * same wider rows); lse (or NULL), fp32 [n_seqs][n_q][n_heads], takes log sum_t exp(scale q.k_t).  A query that sees no slot gives zeros and
  * -infinity.  With ABRA_PAGED_ACCUMULATE every slot's softmax weight, summed
  * over the n_q queries and the group's heads, is added to acc.
  * workspace (256-byte aligned, abra_paged_attention_workspace bytes; when

@@ -123,3 +123,23 @@ def test_what_is_not_finite_costs_little(dev, hq, n_q, where):
     _no_error()
     assert torch.isnan(out).all() if where == "query" else torch.isinf(out).all()
     assert after <= 4 * before, (before, after)
+
+
+def test_queries_and_results_in_the_same_rows(dev):
+    """Columns of one wider tensor, the same as in tensors of their own."""
+    import abra_b200 as A
+
+    rng = np.random.default_rng(5)
+    lens, hq, d = [70, 300, 9], 4, 64
+    c = R.make_cache(rng, lens, 2, d, 16, "f16")
+    kv = _kv(R.to_dev(c, dev))
+    rows = torch.zeros(3, 2 * hq * d + 64, dtype=torch.float16, device=dev)
+    q, out = rows[:, : hq * d].unflatten(1, (hq, d)), rows[:, hq * d : 2 * hq * d].unflatten(1, (hq, d))
+    q.copy_(torch.from_numpy(rng.standard_normal((3, hq, d))))
+    want = A.paged_attention(kv, q.clone(), 0.1)
+    was = q.clone()
+    assert A.paged_attention(kv, q, 0.1, out=out) is out
+    _no_error()
+    assert torch.equal(out, want) and torch.equal(q, was) and (rows[:, 2 * hq * d :] == 0).all()
+    with pytest.raises(ValueError, match="share"):
+        A.paged_attention(kv, q, 0.1, out=rows[:, 8 : 8 + hq * d].unflatten(1, (hq, d)))
