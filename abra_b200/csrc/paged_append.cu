@@ -214,6 +214,15 @@ extern "C" int abra_paged_append(const abra_paged_kv *kv, const void *q, const v
         return paged_fail(ABRA_E_INVALID, "rows must start on 16 bytes and their strides be multiples of 8 elements");
     if (!paged_aligned(q_norm, 16) || !paged_aligned(k_norm, 16) || !paged_aligned(rope, 16) || !paged_aligned(cu_new, 4))
         return paged_fail(ABRA_E_INVALID, "norm weights and rope must be 16-byte aligned");
+    if (q) {
+        // heads are stored while others are still to be read; a head of 16-bit values may take its own place
+        const int64_t in = in_type == ABRA_GGML_F32 ? 4 : 2;
+        const PagedRows to{q_out, 2 * qw, 2 * ldqo};
+        const bool own = q == q_out && in == 2 && ldq == ldqo;
+        if ((!own && paged_overlap(to, {q, in * qw, in * ldq}, n_tokens)) || paged_overlap(to, {k, in * kvw, in * ldk}, n_tokens) ||
+            paged_overlap(to, {v, in * kvw, in * ldv}, n_tokens))
+            return paged_fail(ABRA_E_INVALID, "q_out must not share the memory of q, k or v");
+    }
     if (rope && rope_len < 1) return paged_fail(ABRA_E_INVALID, "rope_len must be positive");
     const int64_t heads = (q ? n_heads : 0) + 2ll * kv->n_kv_heads;
     if (heads > 65535) return paged_fail(ABRA_E_UNSUPPORTED, "over 65535 heads of a token");

@@ -528,8 +528,9 @@ typedef struct {
  * sqrt(mean(x^2) + eps) times the head_dim weights; NULL: none) and then the
  * rotation of the pairs (i, i + head_dim/2) by the row of its position in rope
  * [rope_len][head_dim/2][cos, sin] (NULL: none), in fp32, rounded once to the
- * pools' type.  q_out (row stride ldqo) takes the queries in the pools' type;
- * q and q_out may both be NULL.  acc (if not NULL) becomes 0 and pos (if not
+ * pools' type.  q_out (row stride ldqo) takes the queries in the pools' type and
+ * shares no memory with q, k and v (it may be other columns of the same rows, or
+ * q itself where in_type has 16 bits); q and q_out may both be NULL.  acc (if not NULL) becomes 0 and pos (if not
  * NULL) the position at the new slots.  The paged form of the decode model's
  * norm-rope-append step.  head_dim 64, 96 or 128. */
 int abra_paged_append(const abra_paged_kv *kv, const void *q, const void *k, const void *v,
