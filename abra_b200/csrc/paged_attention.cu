@@ -700,6 +700,7 @@ extern "C" int abra_paged_attention(const abra_paged_kv *kv, const void *q, int6
     if (rc) return rc;
     if (out_type != kv->type && out_type != ABRA_GGML_F32)
         return paged_fail(ABRA_E_UNSUPPORTED, "out must be of the cache's type or F32 (got %d)", out_type);
+    if (kv->n_seqs == 0) return ABRA_OK;
     if (!q || !out || !workspace) return paged_fail(ABRA_E_INVALID, "null q, out or workspace");
     if (ldq < static_cast<int64_t>(n_heads) * kv->head_dim || ldo < static_cast<int64_t>(n_heads) * kv->head_dim)
         return paged_fail(ABRA_E_INVALID, "a row stride is smaller than its heads");
@@ -707,7 +708,6 @@ extern "C" int abra_paged_attention(const abra_paged_kv *kv, const void *q, int6
         return paged_fail(ABRA_E_INVALID, "q and out rows must start on 16 bytes and their strides be multiples of 8 elements");
     if (!paged_aligned(workspace, 256)) return paged_fail(ABRA_E_INVALID, "the workspace must be 256-byte aligned");
     if (workspace_bytes < 256) return paged_fail(ABRA_E_INVALID, "workspace of %lld bytes", (long long)workspace_bytes);
-    if (kv->n_seqs == 0) return ABRA_OK;
     // rows are finished while others' queries are still to be read
     const int64_t width = static_cast<int64_t>(n_heads) * kv->head_dim, out_bytes = out_type == ABRA_GGML_F32 ? 4 : 2;
     if (paged_overlap({q, 2 * width, 2 * ldq}, {out, out_bytes * width, out_bytes * ldo}, static_cast<int64_t>(kv->n_seqs) * n_q))

@@ -352,6 +352,7 @@ extern "C" int abra_paged_evict(const abra_paged_kv *kv, int32_t budget, int32_t
         return paged_fail(ABRA_E_INVALID, "n_sink (%d) and n_recent (%d) must not be negative and fit the budget (%d)", n_sink,
                           n_recent, budget);
     if (!kv->acc || !kv->pos) return paged_fail(ABRA_E_INVALID, "eviction needs acc and pos");
+    if (kv->n_seqs == 0) return ABRA_OK;
     if (!new_lens || !workspace) return paged_fail(ABRA_E_INVALID, "null new_lens or workspace");
     if (new_lens < kv->lens + kv->n_seqs && kv->lens < new_lens + kv->n_seqs)
         return paged_fail(ABRA_E_INVALID, "new_lens must not overlap lens");
@@ -360,7 +361,6 @@ extern "C" int abra_paged_evict(const abra_paged_kv *kv, int32_t budget, int32_t
     if (workspace_bytes < workspace_bytes_of(kv, budget))
         return paged_fail(ABRA_E_INVALID, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                           (long long)workspace_bytes_of(kv, budget));
-    if (kv->n_seqs == 0) return ABRA_OK;
     char *ws = static_cast<char *>(workspace);
     EvictArgs p{paged_view(kv), new_lens, reinterpret_cast<int32_t *>(ws), reinterpret_cast<int32_t *>(ws + counts_bytes(kv)),
                 budget, n_sink, n_recent, static_cast<int>(move_cap(kv, budget)), 0};

@@ -114,7 +114,8 @@ inline bool paged_overlap(PagedRows a, PagedRows b, int64_t n) {
 // The checks every entry point makes of the cache it is given.
 inline int paged_check(const abra_paged_kv *kv) {
     if (!kv) return paged_fail(ABRA_E_INVALID, "null cache");
-    if (kv->n_seqs < 0 || kv->n_pages < 1 || kv->n_kv_heads < 1 || kv->page_size < 1 || kv->max_pages < 1)
+    const bool some = kv->n_seqs > 0;  // no sequences need no table
+    if (kv->n_seqs < 0 || kv->n_pages < 1 || kv->n_kv_heads < 1 || kv->page_size < 1 || kv->max_pages < (some ? 1 : 0))
         return paged_fail(ABRA_E_INVALID,
                           "n_seqs must not be negative, n_pages, n_kv_heads, page_size and max_pages positive "
                           "(%d, %d, %d, %d, %d)",
@@ -127,7 +128,7 @@ inline int paged_check(const abra_paged_kv *kv) {
         return paged_fail(ABRA_E_UNSUPPORTED, "head_dim must be 64, 96 or 128 (got %d)", kv->head_dim);
     if (kv->type != ABRA_GGML_F16 && kv->type != ABRA_GGML_BF16)
         return paged_fail(ABRA_E_UNSUPPORTED, "the cache's type must be F16 or BF16 (got %d)", kv->type);
-    if (!kv->k || !kv->v || !kv->table || !kv->lens) return paged_fail(ABRA_E_INVALID, "null pointer in the cache");
+    if (!kv->k || !kv->v || (some && (!kv->table || !kv->lens))) return paged_fail(ABRA_E_INVALID, "null pointer in the cache");
     if (!paged_aligned(kv->k, 16) || !paged_aligned(kv->v, 16))
         return paged_fail(ABRA_E_INVALID, "the pools must be 16-byte aligned");
     if (!paged_aligned(kv->acc, 4) || !paged_aligned(kv->pos, 4) || !paged_aligned(kv->table, 4) ||

@@ -503,7 +503,8 @@ int abra_model_create_batched_tp(const abra_model_config *cfg, int32_t batch, in
  * call writes to it.  Lengths beyond max_pages * page_size (or below 0) and
  * page numbers outside the pool set bit 4 of the device error word: the length
  * is clamped, a write is skipped, a read takes page 0.
- * Table entries past a sequence's last page are not read. */
+ * Table entries past a sequence's last page are not read.  Without sequences the
+ * calls do nothing, and table, lens and what they would read or write may be NULL. */
 typedef struct {
     void *k, *v;             /* the pools, 16-byte aligned */
     float *acc;              /* accumulated weights [n_pages][n_kv_heads][page_size], or NULL */
