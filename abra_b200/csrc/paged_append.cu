@@ -87,21 +87,30 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
     if (p.cu_new) {
         for (int x = 0; x < p.kv.a.n_seqs; x += APPEND_THREADS) {
             const int y = x + threadIdx.x;
-            s += __syncthreads_count(y < p.kv.a.n_seqs && p.cu_new[y + 1] <= t0);
+            const int ends = y < p.kv.a.n_seqs ? p.cu_new[y + 1] : 0x7fffffff;
+            s += __syncthreads_count(ends <= t0);
+            // one CTA looks at all offsets' order and ends
+            if (blockIdx.x == 0 && y < p.kv.a.n_seqs) {
+                const int starts = p.cu_new[y];
+                if (starts > ends || (y == 0 && starts != 0) || (y == p.kv.a.n_seqs - 1 && ends != p.n_tokens)) report_error(ERR_BAD_INDEX);
+            }
         }
     }
     if (threadIdx.x < nt) {  // each token's slot, position and page
         const int t = static_cast<int>(t0) + threadIdx.x;
         int end, page = -1, off = 0, at = -1;
+        bool mine;  // the offsets give the token to sequence s
         if (p.cu_new) {
             while (s < p.kv.a.n_seqs && p.cu_new[s + 1] <= t) ++s;
             end = s < p.kv.a.n_seqs ? p.cu_new[s + 1] : 0;
+            mine = s < p.kv.a.n_seqs && p.cu_new[s] <= t && end <= p.n_tokens;
         } else {
             const int m = p.n_tokens / p.kv.a.n_seqs;
             s = t / m;
             end = (s + 1) * m;
+            mine = true;
         }
-        if (s < p.kv.a.n_seqs) {
+        if (mine) {
             const int len = paged_len(p.kv, s), slot = len - (end - t);
             at = paged_next_pos(p.kv, s, len) - (end - t);
             if (slot >= 0) {
@@ -110,7 +119,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) append_kernel(const __grid_
                 page = paged_page(p.kv, s, e);
             }
             if (slot < 0 || (p.rope && (at < 0 || at >= p.rope_len))) report_error(ERR_BAD_INDEX);
-        } else {  // beyond the last sequence's tokens
+        } else {
             report_error(ERR_BAD_INDEX);
         }
         s_page[threadIdx.x] = page, s_off[threadIdx.x] = off, s_at[threadIdx.x] = at;

@@ -524,6 +524,9 @@ typedef struct {
  * ldv (elements of in_type F32, F16 or BF16; one fused q|k|v row will do).
  * Tokens lie sequence after sequence: cu_new[s] is sequence s's first token
  * and cu_new[n_seqs] = n_tokens; NULL gives every sequence n_tokens / n_seqs.
+ * Offsets that do not begin with 0, end with n_tokens and never fall set bit 4 of
+ * the device error word; a token that lies before its sequence's first one, or
+ * whose sequence ends beyond n_tokens, is not stored, and its query not rotated.
  * A sequence's m tokens go to slots lens - m .. lens - 1 at positions next_pos
  * - m .. next_pos - 1.  Queries and keys get their RMSNorm over the head (x /
  * sqrt(mean(x^2) + eps) times the head_dim weights; NULL: none) and then the
