@@ -532,10 +532,12 @@ typedef struct {
  * sqrt(mean(x^2) + eps) times the head_dim weights; NULL: none) and then the
  * rotation of the pairs (i, i + head_dim/2) by the row of its position in rope
  * [rope_len][head_dim/2][cos, sin] (NULL: none), in fp32, rounded once to the
- * pools' type.  q_out (row stride ldqo) takes the queries in the pools' type and
- * shares no memory with q, k and v (it may be other columns of the same rows, or
- * q itself where in_type has 16 bits); q and q_out may both be NULL.  acc (if not NULL) becomes 0 and pos (if not
- * NULL) the position at the new slots.  The paged form of the decode model's
+ * pools' type.  A position outside rope sets bit 4 of the device error word; that
+ * token's query and key are stored without the rotation.  q_out (row stride ldqo)
+ * takes the queries in the pools' type and shares no memory with q, k and v (it
+ * may be other columns of the same rows, or q itself where in_type has 16 bits); q
+ * and q_out may both be NULL.  acc (if not NULL) becomes 0 and pos (if not NULL)
+ * the position at the new slots.  The paged form of the decode model's
  * norm-rope-append step.  head_dim 64, 96 or 128. */
 int abra_paged_append(const abra_paged_kv *kv, const void *q, const void *k, const void *v,
                       int32_t in_type, int64_t ldq, int64_t ldk, int64_t ldv, int32_t n_heads,
@@ -548,9 +550,10 @@ int abra_paged_append(const abra_paged_kv *kv, const void *q, const void *k, con
  * head h / (n_heads / n_kv_heads), out = sum_t softmax_t(scale q.k_t) v_t.
  * q (the pools' type) and out (out_type: the pools' type or F32) have row (s *
  * n_q + j) at stride ldq / ldo and share no memory (they may be columns of the
- * same wider rows); lse (or NULL), fp32 [n_seqs][n_q][n_heads], takes log sum_t exp(scale q.k_t).  A query that sees no slot gives zeros and
- * -infinity.  With ABRA_PAGED_ACCUMULATE every slot's softmax weight, summed
- * over the n_q queries and the group's heads, is added to acc.
+ * same wider rows); lse (or NULL), fp32 [n_seqs][n_q][n_heads], takes log sum_t
+ * exp(scale q.k_t).  A query that sees no slot gives zeros and -infinity.  With
+ * ABRA_PAGED_ACCUMULATE every slot's softmax weight, summed over the n_q queries
+ * and the group's heads, is added to acc.
  * workspace (256-byte aligned, abra_paged_attention_workspace bytes; when
  * accumulating it has room for the scores of all the pools' slots) may hold
  * anything; calls that can overlap need one each.

@@ -1,4 +1,5 @@
-"""Paged append with offsets of new tokens that do not fit the call."""
+"""Paged append with offsets of new tokens that do not fit the call, and with
+positions beyond the rotation's table."""
 from __future__ import annotations
 
 import numpy as np
@@ -74,3 +75,17 @@ def test_offsets_of_hundreds_of_sequences(dev):
     bad[400] = bad[399] - 1
     _append(dev, lens, bad.tolist(), n)
     _append(dev, lens, (cu + 1).tolist(), n)
+
+
+def test_positions_beyond_the_rotation(dev):
+    """Reported; the token is stored, its query and key as they are without a
+    rotation."""
+    angle = torch.rand(30, D // 2, device=dev)
+    rope = torch.stack([angle.cos(), angle.sin()], -1)
+    c, after, x, out = _append(dev, [40, 12, 20], [0, 2, 3, 5], 5, rope=rope, next_pos=[31, 12, 0])
+    turned = [True, False, True, False, False]  # positions 29, 30, 11, -2, -1
+    for i, (b, t, at) in enumerate([(0, 38, 29), (0, 39, 30), (1, 11, 11), (2, 18, -2), (2, 19, -1)]):
+        pg, off = int(c["table"][b, t // PAGE]), t % PAGE
+        assert torch.equal(after["v"][pg, :, off], x[i, HQ + HKV :]) and (after["pos"][pg, :, off] == at).all()
+        assert torch.equal(out[i], x[i, :HQ]) != turned[i]
+        assert torch.equal(after["k"][pg, :, off], x[i, HQ : HQ + HKV]) != turned[i]
