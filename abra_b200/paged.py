@@ -162,8 +162,8 @@ def _empty(kv: PagedKV, shape, dtype, stream):
 
     if stream is None or stream_handle(stream) == stream_handle():
         return torch.empty(shape, dtype=dtype, device=kv.device)
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, kv.device)
+    if isinstance(stream, int):  # 0, the default stream, is none that could be wrapped
+        stream = torch.cuda.ExternalStream(stream, kv.device) if stream else torch.cuda.default_stream(kv.device)
     with torch.cuda.stream(stream):
         return torch.empty(shape, dtype=dtype, device=kv.device)
 
