@@ -19,12 +19,13 @@ FLOOR = {"f16": 2.0**-25 / 2.0**11, "bf16": 0.0}
 ROWS = [(4, 1), (2, 3), (24, 1), (4, 4), (8, 8)]  # heads of one kv head, queries: two of the narrow kernel, three of the wide
 
 
-def _check(c, q, scale, out, lse, dtype):
-    """Bounds.  The queries have one element that is not zero, so a score is one
-    exact product; scaling it (its factor rounded too) and subtracting the row's
-    reference are three roundings of a magnitude of M log2 units, the exponential
-    is good to four units of 2^-24.  Twice that for the denominator's share, two
-    roundings of 16 slots' sums and 64 for the joins, half a unit of the result."""
+def _bounds(c, q, scale, dtype, fp32):
+    """The exact result, its log-sum-exp, and bounds of both.  The queries have one
+    element that is not zero, so a score is one exact product; scaling it (its
+    factor rounded too) and subtracting the row's reference are three roundings of
+    a magnitude of M log2 units, the exponential is good to four units of 2^-24.
+    Twice that for the denominator's share, two roundings of 16 slots' sums and 64
+    for the joins, half a unit of the result."""
     want, lse64, _, mag, dot = R.attention(c, q, scale)
     n = c["lens"].double().numpy()[:, None, None]
     assert (lse64 > -np.inf).all()
@@ -40,14 +41,25 @@ def _check(c, q, scale, out, lse, dtype):
                 g = h // (q.shape[2] // k.shape[0])
                 top = (scale * (k[g] @ q[b, j, h].double().numpy())).max()
                 size[b, j, h] = np.abs(v[g]).sum(0) / np.exp(lse64[b, j, h] - top)
+    tol = mag * (2 * ds + R.UNIT[dtype] ** 2 + sums)[..., None] + FLOOR[dtype] * size
+    tol += (EPS32 if fp32 else R.UNIT[dtype]) * np.abs(want) + (2.0**-25 if not fp32 and dtype == "f16" else 2.0**-126)
+    return want, tol, lse64, ds + sums + 2 * EPS32 * np.abs(lse64)
+
+
+def _check(c, q, scale, out, lse, dtype):
+    want, tol, lse64, lse_tol = _bounds(c, q, scale, dtype, out.dtype == torch.float32)
     got = out.cpu().double().numpy()
-    unit = EPS32 if out.dtype == torch.float32 else R.UNIT[dtype]
-    tol = mag * (2 * ds + R.UNIT[dtype] ** 2 + sums)[..., None] + FLOOR[dtype] * size + unit * np.abs(want)
-    tol += 2.0**-25 if unit != EPS32 and dtype == "f16" else 2.0**-126
     assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
     if lse is not None:
-        tol = ds + sums + 2 * EPS32 * np.abs(lse64)
-        assert (np.abs(lse.cpu().double().numpy() - lse64) <= tol).all()
+        assert (np.abs(lse.cpu().double().numpy() - lse64) <= lse_tol).all()
+
+
+def _few_bits(rng, shape, dtype):
+    """Queries with one element that is not zero, another for each head."""
+    q = torch.zeros(*shape)
+    at = torch.arange(shape[2]) % shape[3]
+    q[..., torch.arange(shape[2]), at] = torch.from_numpy(rng.choice([-3.0, -1.5, 1.0, 2.5], shape[:3])).float()
+    return q.to(R.DTYPE[dtype])
 
 
 def _attend(dev, c, q, scale, dtype):
@@ -87,6 +99,26 @@ def test_a_sink_over_everything_else(dev, dtype, hq, n_q, gap, where):
     q = torch.zeros(len(lens), n_q, hq, d)
     q[..., 0] = torch.tensor([1.0, 0.875, 0.5, 0.25]).repeat(16)[:hq]
     _attend(dev, c, q.to(R.DTYPE[dtype]), 1.0, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hq,n_q", ROWS)
+def test_both_parts_of_the_weights(dev, dtype, hq, n_q):
+    """Ordinary scores.  The bounds are those of weights of two 16-bit values:
+    the definition with weights of one, which leave out the second, is beyond them."""
+    rng = np.random.default_rng(hq * n_q)
+    lens, d = [n_q + 2, 100, 700], 64
+    c = R.make_cache(rng, lens, 1, d, 16, dtype)
+    q = _few_bits(rng, (len(lens), n_q, hq, d), dtype)
+    _attend(dev, c, q, 0.75, dtype)
+    want, tol, _, _ = _bounds(c, q, 0.75, dtype, True)
+    for b, n in enumerate(lens):
+        k, v = (R.rows(c, c[x], b, n).double() for x in ("k", "v"))
+        s = 0.75 * torch.einsum("qhd,td->qht", q[b].double(), k[0])
+        s += torch.where(torch.arange(n) < n - n_q + 1 + torch.arange(n_q)[:, None], 0.0, -torch.inf)[:, None]
+        w = (s - s.amax(-1, keepdim=True)).exp()
+        one = (w.to(R.DTYPE[dtype]).double() @ v[0]) / w.sum(-1, keepdim=True)
+        assert (np.abs(one.numpy() - want[b]) > tol[b]).any()
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
