@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
                     const int t = base + g + 8 * x, e = p.kv.page.div(t);
                     const int page = t < sg.slot_end ? paged_page(p.kv, sg.seq, e) : -1;
                     if (page >= 0) {  // a page outside the pool has no place for them
-                        float *to = p.scores + paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size) * ROWS;
+                        float *to = p.scores + score_at(p, sg.seq, head, t, paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size)) * ROWS;
                         *reinterpret_cast<float2 *>(to + 2 * c) = make_float2(sc[2 * x], sc[2 * x + 1]);
                     }
                 }
@@ -576,7 +576,7 @@ template <typename T> __device__ __forceinline__ void accumulate(const JoinArgs 
                 for (int y = 0; y < 2; ++y) {
                     x[y] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                     if (meta >= 0 && mine + 4 * y < nr)
-                        x[y] = __ldcg(reinterpret_cast<const float4 *>(p.scores + meta * padded + r0 + mine + 4 * y));
+                        x[y] = __ldcg(reinterpret_cast<const float4 *>(p.scores + score_at(p, sg.seq, sg.head, t, meta) * padded + r0 + mine + 4 * y));
                 }
                 page = page_of(t + slots);
                 float sum = 0.0f;
@@ -606,6 +606,7 @@ template <typename T, int D, bool SCORES> __global__ void __launch_bounds__(JOIN
 // ------------------------------------------------------------------ host ---
 struct Plan {
     int wide, block, row_blocks, resident, pieces, sms;  // block: rows of a block
+    int score_slots;                                         // of a sequence's scores, 0: they lie as the pools do
     int64_t part_o, part_ml, split, row_lse, scores, bytes;  // workspace offsets
 };
 
@@ -628,10 +629,12 @@ int make_plan(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q, bool accumu
     pl.part_ml = at, at = up(at + static_cast<int64_t>(pl.pieces) * 2 * pl.block * 8);
     pl.split = at, at = up(at + triples * 8);
     pl.row_lse = pl.scores = at;
+    const int64_t tables = static_cast<int64_t>(kv->n_seqs) * kv->max_pages;
+    pl.score_slots = tables < kv->n_pages ? kv->max_pages * kv->page_size : 0;
     if (accumulate) {
         at = up(at + static_cast<int64_t>(kv->n_seqs) * kv->n_kv_heads * rows * 4);
         pl.scores = at;
-        at = up(at + static_cast<int64_t>(kv->n_pages) * kv->n_kv_heads * kv->page_size * pl.row_blocks * pl.block * 4);
+        at = up(at + std::min<int64_t>(tables, kv->n_pages) * kv->n_kv_heads * kv->page_size * pl.row_blocks * pl.block * 4);
     }
     pl.bytes = at;
     return ABRA_OK;
@@ -738,7 +741,8 @@ extern "C" int abra_paged_attention(const abra_paged_kv *kv, const void *q, int6
                  reinterpret_cast<float2 *>(ws + pl.part_ml),
                  reinterpret_cast<int2 *>(ws + pl.split),
                  accumulate ? reinterpret_cast<float *>(ws + pl.row_lse) : nullptr,
-                 reinterpret_cast<float *>(ws + pl.scores)};
+                 reinterpret_cast<float *>(ws + pl.scores),
+                 pl.score_slots};
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return paged_cuda(kv->type == ABRA_GGML_F16 ? launch<__half>(p, pl, accumulate, st)
                                                 : launch<__nv_bfloat16>(p, pl, accumulate, st),

@@ -47,8 +47,15 @@ struct AttendArgs {
     float2 *part_ml;    // [piece][2][rows of a block] maximum (log2 units) and sum
     int2 *split;        // [seq][kv head][row block] the first part's place, the last part's piece
     float *row_lse;     // [seq][kv head][row] log2 of the sum of a row that lies in one piece
-    float *scores;      // [page][kv head][offset][padded rows], log2 units
+    float *scores;      // [page][kv head][offset][padded rows], log2 units; or [seq][kv head][slot][padded rows]
+    int score_slots;    // slots of a sequence in the latter, 0: the former
 };
+
+// A slot's place among the scores: that of its page, or its own in the tables where
+// these name fewer slots than the pools have.
+__device__ __forceinline__ int64_t score_at(const AttendArgs &p, int seq, int head, int t, int64_t meta) {
+    return p.score_slots ? (static_cast<int64_t>(seq) * p.kv.a.n_kv_heads + head) * p.score_slots + t : meta;
+}
 
 // ------------------------------------------------------------------ PTX ---
 // 16 bytes into shared memory past L1; `bytes` 0 writes zeros and reads nothing.

@@ -413,7 +413,8 @@ __global__ void __launch_bounds__(Wide<D, N>::THREADS, 1) attend_wide_kernel(con
                 if (SCORES && t < sg.slot_end) {
                     const int e = p.kv.page.div(t), page = paged_page(p.kv, sg.seq, e);
                     if (page >= 0) {  // a page outside the pool has no place for them
-                        float *to = p.scores + paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size) * (p.row_blocks * N) + r0 + n_first;
+                        const int64_t at = score_at(p, sg.seq, head, t, paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size));
+                        float *to = p.scores + at * (p.row_blocks * N) + r0 + n_first;
 #pragma unroll
                         for (int n = 0; n < NH; n += 4) *reinterpret_cast<float4 *>(to + n) = make_float4(s[n], s[n + 1], s[n + 2], s[n + 3]);
                     }

@@ -555,8 +555,9 @@ int abra_paged_append(const abra_paged_kv *kv, const void *q, const void *k, con
  * ABRA_PAGED_ACCUMULATE every slot's softmax weight, summed over the n_q queries
  * and the group's heads, is added to acc.
  * workspace (256-byte aligned, abra_paged_attention_workspace bytes; when
- * accumulating it has room for the scores of all the pools' slots) may hold
- * anything; calls that can overlap need one each.
+ * accumulating it has room for the scores of all slots that the tables can name, or
+ * of all the pools' where these are fewer) may hold anything; calls that can
+ * overlap need one each.
  * head_dim 64, 96 or 128. */
 #define ABRA_PAGED_ACCUMULATE 1
 int64_t abra_paged_attention_workspace(const abra_paged_kv *kv, int32_t n_heads, int32_t n_q,
