@@ -22,11 +22,14 @@ constexpr int WAVES = 4;                  // pieces for each CTA that the GPU ho
 // 8,192 slots 26.5 us, 25.6 with 4 and 11, 25.4 with 10 and 5).
 template <typename T> struct Weigh;
 template <> struct Weigh<__half> {
-    static constexpr float RAISE = 4.0f, SHIFT = 11.0f;
+    static constexpr float RAISE = 4.0f;
+    static constexpr int SHIFT = 11;
 };
 template <> struct Weigh<__nv_bfloat16> {
-    static constexpr float RAISE = 10.0f, SHIFT = 0.0f;
+    static constexpr float RAISE = 10.0f;
+    static constexpr int SHIFT = 0;
 };
+constexpr float power_of_two(int n) { return n < 0 ? 1.0f / power_of_two(-n) : n == 0 ? 1.0f : 2.0f * power_of_two(n - 1); }
 // What beginning and ending a row costs beside its steps, in steps (its
 // queries, the join of its warps): with 1 the pieces full of short rows end
 // last (25.8 against 23.9 us for 32 sequences of 1 to 4,096 slots), with 3
@@ -70,9 +73,8 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 // A score's weight against `ref`, the row's maximum (0 while that is -infinity).
-template <typename T> __device__ __forceinline__ float weight_of(float s, float ref) {
-    return exp2_fast(Weigh<T>::SHIFT != 0.0f ? s - ref + Weigh<T>::SHIFT : s - ref);
-}
+// (a product, not a sum with SHIFT: s - ref keeps its bits)
+template <typename T> __device__ __forceinline__ float weight_of(float s, float ref) { return exp2_fast(s - ref) * power_of_two(Weigh<T>::SHIFT); }
 // What a sum relative to the maximum m counts relative to `top`; never zero, so
 // that a sum of infinity stays one.
 __device__ __forceinline__ float scaled(float m, float top) { return m == top ? 1.0f : exp2_fast(fmaxf(m - top, -126.0f)); }
@@ -291,7 +293,7 @@ __device__ __forceinline__ void store_out(const AttendArgs &p, int64_t at, float
 
 // log2 of a row's sum of 2^s.
 template <typename T> __device__ __forceinline__ float row_lse2(float m, float total) {
-    return total != 0.0f ? m + (log2f(total) - Weigh<T>::SHIFT) : -INFINITY;
+    return total != 0.0f ? m + log2f(total * power_of_two(-Weigh<T>::SHIFT)) : -INFINITY;
 }
 
 // A finished row's lse; total == 0: the row saw nothing.
