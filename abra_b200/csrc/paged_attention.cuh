@@ -14,12 +14,14 @@ constexpr int WAVES = 4;                  // pieces for each CTA that the GPU ho
 // sums until its log-sum-exp takes SHIFT off again.  m is raised only when a score
 // passes it by RAISE, so that most tiles need no reduction; weights stay below
 // 2^(RAISE + SHIFT), for which compare and weight both take the difference s - m
-// first (m + RAISE or m - SHIFT would be rounded where m is large).  bf16 has
-// fp32's range.  fp16 ends at 2^-24, so its weights go up to the top of its range:
-// of a weight at most 2^-36 of the row's largest is lost, without SHIFT 2^-25,
-// which beside a slot far above the others is all of them.  RAISE 2 and SHIFT 13
-// raise more often than they are worth (16 new tokens of four sequences of up to
-// 8,192 slots 26.5 us, 25.6 with 4 and 11, 25.4 with 10 and 5).
+// first (m + RAISE or m - SHIFT would be rounded where m is large).  fp16 ends at
+// 2^-24, so its weights go up to the top of its range: of a weight at most 2^-36 of
+// the row's largest is lost, without SHIFT 2^-25, which beside a slot far above the
+// others is all of them.  RAISE 2 and SHIFT 13 raise more often than they are worth
+// (16 new tokens of four sequences of up to 8,192 slots 26.5 us, 25.6 with 4 and 11,
+// 25.4 with 10 and 5).  bf16 has fp32's range, in values too: its weights are so
+// small that 2^22 of the largest values do not add up to infinity before the row is
+// divided by its sum, and large enough for products of values above 2^-90.
 template <typename T> struct Weigh;
 template <> struct Weigh<__half> {
     static constexpr float RAISE = 4.0f;
@@ -27,7 +29,7 @@ template <> struct Weigh<__half> {
 };
 template <> struct Weigh<__nv_bfloat16> {
     static constexpr float RAISE = 10.0f;
-    static constexpr int SHIFT = 0;
+    static constexpr int SHIFT = -32;
 };
 constexpr float power_of_two(int n) { return n < 0 ? 1.0f / power_of_two(-n) : n == 0 ? 1.0f : 2.0f * power_of_two(n - 1); }
 // What beginning and ending a row costs beside its steps, in steps (its

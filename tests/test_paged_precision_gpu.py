@@ -123,6 +123,21 @@ def test_both_parts_of_the_weights(dev, dtype, hq, n_q):
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("hq,n_q", ROWS)
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_values_at_the_end_of_their_type(dev, dtype, hq, n_q, sign):
+    """Thousands of values near the largest, or the lowest, of the type: their
+    mean is one too, though their sum is far beyond fp32 in bf16."""
+    rng = np.random.default_rng(hq + n_q)
+    lens, d = [50, 6000], 64
+    c = R.make_cache(rng, lens, 1, d, 16, dtype)
+    most = float(torch.finfo(R.DTYPE[dtype]).max)
+    c["v"] = torch.from_numpy(sign * most * rng.uniform(0.5, 0.9, c["v"].shape)).to(R.DTYPE[dtype])
+    q = _few_bits(rng, (len(lens), n_q, hq, d), dtype)
+    _attend(dev, c, q, 1.0, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hq,n_q", ROWS)
 def test_scores_beyond_single_units(dev, dtype, hq, n_q):
     """Scores around 2^27, 2^28 log2 units, which fp32 holds in steps of 16 or
     32: which slot is the largest is lost, but the result stays among the values
