@@ -529,8 +529,9 @@ template <typename T> __device__ __forceinline__ void accumulate(const JoinArgs 
     Walk<STEP> w;
     Line line(0, 0);
     if (!find_start<JOIN_THREADS>(p.kv, 1, cta, ctas, ctas, line, w)) return;
-    // rows that see nothing, and what lies behind the last row, have an lse of +infinity and no weight
-    auto weight = [](float x, float lse) { return lse == INFINITY ? 0.0f : exp2_fast(x - lse); };
+    // rows that see nothing, and what lies behind the last row, have an lse of +infinity and no weight;
+    // nor has a slot that a row does not see, whose own lse may be NaN
+    auto weight = [](float x, float lse) { return lse == INFINITY || x == -INFINITY ? 0.0f : exp2_fast(x - lse); };
     do {
         const Segment &sg = w.s;
         const int first = sg.tile0 * STEP + tid / lanes;  // this thread's slot, and every `slots` after it

@@ -84,6 +84,28 @@ def test_nan_beside_healthy_sequences(dev, dtype, d, page, hq, n_q, where):
         assert torch.isnan(now[0][: n - n_q + 1]).all() if b == 1 else torch.equal(now[0], was[0])
 
 
+@pytest.mark.parametrize("dtype,d", [("f16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("hq,n_q", [(2, 3), (4, 4), (8, 8), (3, 2)])
+def test_weights_of_slots_that_a_nan_query_does_not_see(dev, dtype, d, hq, n_q):
+    """The newest slots' weights come from the queries that see them: within
+    their roundings (a row's maximum may be raised at other slots) what they are
+    with a first query of numbers."""
+    rng = np.random.default_rng(hq)
+    lens = [n_q, 50, 3000]
+    c = R.make_cache(rng, lens, 1, d, 16, dtype)
+    c["acc"] = torch.zeros_like(c["acc"])
+    q = torch.from_numpy(2 * rng.standard_normal((len(lens), n_q, hq, d))).to(R.DTYPE[dtype])
+    bad, none = q.clone(), q.clone()
+    bad[:, 0, 0] = float("nan")
+    got = _run(dev, c, bad)[2]
+    _, _, weights, _, _ = R.attention(c, none, 0.125)
+    for b, n in enumerate(lens):
+        new = R.rows(c, got, b, n)[0]
+        assert torch.isnan(new[: n - n_q + 1]).all()
+        want = torch.from_numpy(weights[b][0, n - n_q + 1 :])  # the first query adds nothing to them
+        assert ((new[n - n_q + 1 :].double() - want).abs() <= 1e-4 * want).all()
+
+
 @pytest.mark.parametrize("hq,n_q", [(4, 1), (8, 8)])
 @pytest.mark.parametrize("where", ["query", "value"])
 def test_what_is_not_finite_costs_little(dev, hq, n_q, where):
