@@ -128,15 +128,20 @@ class PagedDecoder:
         self.seen.append(0)
         return len(self.pages) - 1
 
-    def _grow(self, b: int, n: int) -> None:
-        """Pages for n more slots of conversation b; the lengths count them."""
-        self.lens[b] += n
-        self.seen[b] += n
-        while len(self.pages[b]) * self.page < self.lens[b]:
-            if not self.free:
-                raise RuntimeError("the pool of pages is used up")
-            self.pages[b].append(self.free.pop())
-            self.table[b, len(self.pages[b]) - 1] = self.pages[b][-1]
+    def _grow(self, lo: int, hi: int, n: int) -> None:
+        """Pages for n more slots of each of the conversations; the lengths count
+        them.  All or, with an error, none."""
+        if max(self.seen[lo:hi]) + n > len(self.rope):
+            raise ValueError(f"a conversation would be longer than max_len ({len(self.rope)})")
+        need = [-(-(self.lens[b] + n) // self.page) - len(self.pages[b]) for b in range(lo, hi)]
+        if sum(max(0, x) for x in need) > len(self.free):
+            raise RuntimeError("the pool of pages is used up")
+        for b, more in zip(range(lo, hi), need):
+            self.lens[b] += n
+            self.seen[b] += n
+            for _ in range(more):
+                self.pages[b].append(self.free.pop())
+                self.table[b, len(self.pages[b]) - 1] = self.pages[b][-1]
 
     def _handles(self, lo: int, hi: int) -> list[A.PagedKV]:
         """The layers' caches of conversations lo .. hi - 1."""
@@ -152,8 +157,7 @@ class PagedDecoder:
         appended to their caches; logits [n, m, vocab]."""
         s, (n, m) = self.shape, tokens.shape
         cols = n * m
-        for b in range(lo, lo + n):
-            self._grow(b, m)
+        self._grow(lo, lo + n, m)
         self._publish()
         caches = self._handles(lo, lo + n)
         dev, hd = self.device, s.heads * s.head_dim
