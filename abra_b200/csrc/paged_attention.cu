@@ -535,6 +535,7 @@ template <typename T> __device__ __forceinline__ void accumulate(const JoinArgs 
     do {
         const Segment &sg = w.s;
         const int first = sg.tile0 * STEP + tid / lanes;  // this thread's slot, and every `slots` after it
+        const int64_t seq_scores = score_at(p, sg.seq, sg.head, 0, -1);  // of slot 0, or -1: they lie as the pages do
         auto page_of = [&](int t) { return t < sg.slot_end ? paged_page(p.kv, sg.seq, p.kv.page.div(t)) : -1; };
         for (int r0 = 0; r0 < p.rows; r0 += ACC_ROWS) {
             const int nr = min(ACC_ROWS, p.rows - r0);
@@ -577,7 +578,7 @@ template <typename T> __device__ __forceinline__ void accumulate(const JoinArgs 
                 for (int y = 0; y < 2; ++y) {
                     x[y] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                     if (meta >= 0 && mine + 4 * y < nr)
-                        x[y] = __ldcg(reinterpret_cast<const float4 *>(p.scores + score_at(p, sg.seq, sg.head, t, meta) * padded + r0 + mine + 4 * y));
+                        x[y] = __ldcg(reinterpret_cast<const float4 *>(p.scores + (seq_scores < 0 ? meta : seq_scores + t) * padded + r0 + mine + 4 * y));
                 }
                 page = page_of(t + slots);
                 float sum = 0.0f;
