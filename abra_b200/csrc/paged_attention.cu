@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
         m[0] = m[1] = -INFINITY;
         sub[0] = sub[1] = l[0] = l[1] = 0.0f;
         bool odd = false;  // an infinity or NaN was taken out of a tile
+        const int64_t seq_scores = SCORES ? score_at(p, sg.seq, head, 0, -1) : 0;
 
         for (int base = sg.tile0 * STEP + warp * TILE; base < sg.slot_end; base += STEP) {
             // scores: slots g, g + 8 of the tile by rows 2c, 2c + 1; two sums, for
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
                     const int t = base + g + 8 * x, e = p.kv.page.div(t);
                     const int page = t < sg.slot_end ? paged_page(p.kv, sg.seq, e) : -1;
                     if (page >= 0) {  // a page outside the pool has no place for them
-                        float *to = p.scores + score_at(p, sg.seq, head, t, paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size)) * ROWS;
+                        float *to = p.scores + (seq_scores < 0 ? paged_meta_at(p.kv, page, head, t - e * p.kv.a.page_size) : seq_scores + t) * ROWS;
                         *reinterpret_cast<float2 *>(to + 2 * c) = make_float2(sc[2 * x], sc[2 * x + 1]);
                     }
                 }
