@@ -81,8 +81,14 @@ __device__ __forceinline__ uint32_t trans8x8(uint32_t a) {
     return d;
 }
 // --------------------------------------------------------------- kernel ---
-constexpr int ROWS = 8;   // of a block; more rows a kv head go to paged_attention_wide.cu (98 against 158 us here for 16
-                          // rows, 32 sequences of up to 8,192 slots; 31 against 22 us there for four, 32 of up to 4,096)
+// Rows of a block.  More rows a kv head go to paged_attention_wide.cu, which reads
+// the slots once for 16 to 64 of them: 16 rows over 131,072 slots 99 us there, 153
+// here in two blocks; 32 sequences of up to 8,192 33 and 40.  With many short
+// sequences its rows' ends cost more than that gains (64 of up to 512 slots 26.9
+// there, 25.1 here; 128 of up to 1,000 55.6 and 49.2), but lengths are on the
+// device when the kernel is chosen.  Up to eight rows are one block here, and
+// faster (four rows, 32 sequences of up to 4,096 slots: 18.0 us here, 24.7 there).
+constexpr int ROWS = 8;
 constexpr int CTAS = 3;   // on a multiprocessor, with rings of two tiles (two CTAs with rings of three: 188 against 179 us for
                           // 64 sequences of up to 16,384 slots, 24 against 21 for 32 of up to 4,096)
 template <int D> struct Shape {
@@ -131,6 +137,8 @@ __global__ void __launch_bounds__(AT_THREADS, CTAS) attend_kernel(const __grid_c
     const bool by8 = p.kv.a.page_size % 8 == 0;
     Walk<STEP> f = w;
     int f_base = f.s.tile0 * STEP + warp * TILE, f_valid = 0;
+    // (a table entry for every tile where eight does not divide the page size: 32
+    // sequences of up to 4,096 slots 18.5 us with pages of 7, 18.1 with 16)
     int f_page = 0;    // of half l % 2 of the batch's tile l / 2, or (by8 false) of row l % 16 of this tile
     int f_tile = 16;   // this tile's place in its batch of 16; 16: the next batch is to be read
     uint32_t f_at = ring;

@@ -6,8 +6,8 @@
 
 namespace abra {
 
-constexpr int PIECE = 16;                 // steps of a piece, where there are enough to fill the GPU (131,071 slots: 101 us;
-                                          // with 8, and so twice the parts to join, 111)
+constexpr int PIECE = 16;                 // steps of a piece, where there are enough to fill the GPU (131,071 slots: 93 us;
+                                          // with 8, and so twice the parts to join, 99)
 constexpr int WAVES = 4;                  // pieces for each CTA that the GPU holds, at most; the wide kernel's CTA fills its
                                           // multiprocessor, so that nothing runs beside a new one's start, and takes one
 // A row's weights are 2^(s - m + SHIFT) of its running maximum m, and so are its
@@ -34,8 +34,8 @@ template <> struct Weigh<__nv_bfloat16> {
 constexpr float power_of_two(int n) { return n < 0 ? 1.0f / power_of_two(-n) : n == 0 ? 1.0f : 2.0f * power_of_two(n - 1); }
 // What beginning and ending a row costs beside its steps, in steps (its
 // queries, the join of its warps): with 1 the pieces full of short rows end
-// last (25.8 against 23.9 us for 32 sequences of 1 to 4,096 slots), with 3
-// the long rows do.
+// last (21.7 against 20.8 us for 32 sequences of 1 to 4,096 slots), with 3
+// the long rows do (21.8).
 constexpr int ROW_COST = 2;
 
 struct AttendArgs {

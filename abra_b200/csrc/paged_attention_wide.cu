@@ -31,7 +31,9 @@
 // 8,192 slots 26 us (mma.sync with 32 rows a block: 68); 16 heads of one token
 // over 131,072 slots, 0.54 GB, 100 us = 5.4 TB/s.  A step of 64 rows takes 1.2
 // us of softmax and 1.7 of copies; a CTA's start, 3.5 us to its first scores,
-// and a row's end, 2 us, run beside nothing and bound the smaller calls.
+// and a row's end, 2 us, run beside nothing and bound the smaller calls.  A prompt's
+// blocks of rows each take all of their sequence's slots, also those that none of
+// them sees: 4,096 tokens of 32 heads 1.5 ms, half of it for nothing.
 #include "paged_attention.cuh"
 #include "tc_common.cuh"
 
@@ -43,7 +45,7 @@ constexpr int W_LOAD = 96;  // three loader warps
 template <int D, int N> struct Wide {
     // compute warps: four, or eight that share the rows of a slot where these
     // are so many that four take longer than the copies (2.0 us a step of 64
-    // rows; 16 queries of 4 sequences 31.7 us with four, 27.2 with eight)
+    // rows; 16 queries of 4 sequences 32.0 us with four, 26.3 with eight)
     static constexpr int CW = N >= 64 ? 8 : 4, COMPUTE = 32 * CW, THREADS = COMPUTE + W_LOAD + 32;
     static constexpr int NH = N / (CW / 4);             // rows of a compute thread
     static constexpr int CHUNKS = D / 8;                // of 16 bytes in a row

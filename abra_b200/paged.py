@@ -12,8 +12,9 @@ step,
 Buffers are torch CUDA tensors; every call is asynchronous on ``stream``
 (default: torch's current stream) and allocates nothing when its outputs and
 workspace are given.  Bad arguments raise ValueError before any launch.
-Lengths and page numbers live on the device: one outside its range sets bit 4
-of :func:`abra_b200.device_error`.
+Lengths, page numbers and offsets of new tokens live on the device: one outside
+its range sets bit 4 of :func:`abra_b200.device_error`.  Results share no memory
+with what a call reads, except where it says so.
 
     kv = PagedKV(k, v, table, lens, pos=pos, acc=acc)
     lens += 1                                   # the step's token
@@ -185,9 +186,11 @@ def paged_append(kv: PagedKV, k, v, q=None, q_out=None, cu_new=None, q_norm=None
     k, v: [n_tokens, kv heads * head_dim] (or split by heads), q: [n_tokens,
     heads * head_dim], all float32, float16 or bfloat16, rows at any stride (so
     slices of one fused projection will do), sequence after sequence.  cu_new:
-    int32 [n_seqs + 1], the sequences' first tokens (None: equally many each).
-    q_norm, k_norm: float32 [head_dim] RMSNorm weights; rope: float32 [length,
-    head_dim / 2, 2], cos and sin of each position.
+    int32 [n_seqs + 1], the sequences' first tokens, from 0 to n_tokens (None:
+    equally many each).  q_norm, k_norm: float32 [head_dim] RMSNorm weights; rope:
+    float32 [length, head_dim / 2, 2], cos and sin of each position (a position
+    beyond it is reported, its token not rotated).  q_out may be other columns of
+    the tokens' rows, or q itself where that has 16 bits.
     """
     dev, hd, types = kv._index, kv.head_dim, kv._types
     kvw = kv.n_kv_heads * hd
@@ -259,8 +262,9 @@ def paged_attention(kv: PagedKV, q, scale: float, out=None, lse=None, accumulate
     """Attention of each sequence's newest n_q tokens over its cached slots
     (abra_paged_attention): q [n_seqs, n_q, heads, head_dim] (or [n_seqs,
     heads, head_dim] for one token) in the cache's type; query j sees the slots
-    before lens - n_q + j + 1.  Returns out, of q's shape and the cache's type
-    unless a float32 ``out`` is given.  lse: float32 [n_seqs, n_q, heads], log
+    before lens - n_q + j + 1; up to 4,096 of them, though the work is that of all
+    slots for each.  Returns out, of q's shape and the cache's type unless a
+    float32 ``out`` is given (it may be other columns of q's rows).  lse: float32 [n_seqs, n_q, heads], log
     of the softmax's denominator.  accumulate: add every slot's weight to
     kv.acc."""
     dev, hd, shape = kv._index, kv.head_dim, q.shape
