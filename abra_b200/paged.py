@@ -98,7 +98,18 @@ class PagedKV:
     newest token (None: lens, while nothing has been evicted); pos (int32) and
     acc (float32): [n_pages, kv heads, page size], each slot's position and
     accumulated attention weight (eviction needs both).
+
+    The calls go to the memory of these tensors, so they are filled in place
+    (``kv.lens += 1``); another tensor needs another PagedKV.
     """
+
+    _TENSORS = frozenset(("k", "v", "table", "lens", "next_pos", "pos", "acc"))
+
+    def __setattr__(self, name, value):
+        # an attribute put in a tensor's place would leave the calls with the old one's memory
+        if name in self._TENSORS and getattr(self, name, value) is not value:
+            raise AttributeError(f"PagedKV.{name} is filled in place; another tensor needs another PagedKV")
+        super().__setattr__(name, value)
 
     def __init__(self, k, v, table, lens, next_pos=None, pos=None, acc=None):
         import torch
