@@ -27,7 +27,7 @@
 // 16,384 slots, 1.06 GB, 179 us = 5.9 TB/s, 0.91 of the measured HBM copy; one
 // of 131,071, 0.54 GB, 94 us = 5.7 TB/s; 32 of up to 4,096, 65 MB, 21 us; one of
 // 600, 8.9 us, of which 3 are the join's.  DRAM reads are the cache's bytes
-// (537.0 of 536.9 MB); issue slots 42 % used, tensor pipe 13 %.
+// (537.0 of 536.9 MB); issue slots 40 % used, tensor pipe 12 %.
 #include <algorithm>
 
 #include "paged_attention.cuh"
